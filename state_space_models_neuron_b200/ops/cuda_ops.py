@@ -15,6 +15,7 @@ import torch
 from torch.autograd import forward_ad as _forward_ad
 
 from . import native
+from .kv_pages import HEAD_DIMS
 
 _c = ctypes
 _status = {}
@@ -1344,3 +1345,195 @@ def attention(q, k, v, causal=True):
     if q.shape[-1] != 128 or q.shape[1] % 128 or q.shape[1] != k.shape[1]:
         raise ValueError("the GPU attention kernel needs head_dim 128 and equal q/k lengths that are multiples of 128")
     return _apply(_Attention, q, k, v)
+
+
+# ======================================================================================
+# norms of queries and keys with rotation, paged key-value cache, attention of one new token
+# ======================================================================================
+_KV_TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1, torch.int8: 2}
+
+
+def _head_view(t: torch.Tensor):
+    """t [B, L, H, Dh] with unit channel stride, other strides multiples of 8 and a 16-byte base, and its strides (a copy only
+    where it must be).  The stride of a dimension of one element says nothing and counts as 0."""
+    sb, sl, sh = [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
+    if t.stride(3) != 1 or (sb | sl | sh) & 7 or t.data_ptr() & 15:
+        t = t.contiguous()
+        if t.data_ptr() & 15:
+            t = t.clone()
+        _, L, H, D = t.shape
+        sb, sl, sh = L * H * D, H * D, D
+    return t, (sb, sl, sh)
+
+
+def _strides(*each):
+    flat = [s for strides in each for s in strides]
+    return (_c.c_longlong * len(flat))(*flat)
+
+
+def _aligned(t: Optional[torch.Tensor]):
+    """t contiguous on a 16-byte base."""
+    if t is None or (t.is_contiguous() and not t.data_ptr() & 15):
+        return t
+    return t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+
+
+def _require_head_dim(dim: int, rotary: int) -> None:
+    if dim not in HEAD_DIMS:
+        raise ValueError(f"the kernels are written for heads of {HEAD_DIMS} channels, got {dim}")
+    if rotary % 16:
+        raise ValueError(f"the kernels rotate a multiple of 16 channels, got {rotary}")
+
+
+def _require_norm_weight(w) -> None:
+    if w is not None and w.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"norm weights are bfloat16 or float32, got {w.dtype}")
+
+
+def _require_one_device(*ts) -> torch.device:
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+    return dev
+
+
+def _on_device(op):
+    """`op` launched on the current stream of its first tensor's device, whichever device is current."""
+    @functools.wraps(op)
+    def call(first, *args):
+        if first.get_device() == torch._C._cuda_getDevice():
+            return op(first, *args)
+        with torch.cuda.device(first.device):
+            return op(first, *args)
+    return call
+
+
+class _QKNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, qw, kw, eps, cos, sin, positions):
+        (B, L, Hq, D), Hk = q.shape, k.shape[2]
+        (q2, qs), (k2, ks) = _head_view(q), _head_view(k)
+        qw2, kw2 = _aligned(qw), _aligned(kw)
+        qo = torch.empty(B, L, Hq, D, dtype=torch.bfloat16, device=q.device)
+        ko = torch.empty(B, L, Hk, D, dtype=torch.bfloat16, device=q.device)
+        if B and L:
+            _run("ssm_qk_norm_fwd", _p(q2), _p(k2), _strides(qs, ks), _p(qo), _p(ko), _p(qw2), _p(kw2), _is32(qw), _is32(kw), _p(cos),
+                 _p(sin), _p(positions), int(positions is not None and positions.dtype == torch.int64), B, L, Hq, Hk, D,
+                 0 if cos is None else 2 * cos.shape[1], 0 if cos is None else cos.shape[0], _c.c_float(eps),
+                 _p(status_tensor(q.device)), _st())
+        ctx.save_for_backward(q2, k2, qw, kw, cos, sin, positions)
+        ctx.eps, ctx.strides = eps, (qs, ks)
+        return qo, ko
+
+    @staticmethod
+    def backward(ctx, dqo, dko):
+        q2, k2, qw, kw, cos, sin, positions = ctx.saved_tensors
+        (B, L, Hq, D), Hk, dev = q2.shape, k2.shape[2], q2.device
+        (g, gs), (h, hs) = _head_view(dqo), _head_view(dko)
+        dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q2, k2))
+        grads, targets, adds = [], [], []
+        for w, need in ((qw, ctx.needs_input_grad[2]), (kw, ctx.needs_input_grad[3])):
+            mg = getattr(w, "main_grad", None) if need and w.is_leaf else None
+            if mg is not None and mg.dtype == torch.float32 and B and L:
+                # the optimizer's fp32 gradient: stored by the first contribution of a step, added to by the others
+                targets.append(mg)
+                adds.append(int(not getattr(w, "grad_stale", False)))
+                w.grad_stale = False
+                grads.append(None)
+                continue
+            grads.append(torch.empty(D, dtype=w.dtype, device=dev) if need else None)
+            targets.append(grads[-1])
+            adds.append(0)
+        if not (B and L):
+            return dq, dk, *[None if t is None else t.zero_() for t in grads], None, None, None, None
+        blocks = (_c.c_int * 2)()
+        _lib().ssm_qk_norm_bwd_blocks(_ll(B * L), Hq, Hk, D, blocks)
+        part = torch.empty(blocks[1], D, dtype=torch.float32, device=dev)
+        _run("ssm_qk_norm_bwd", _p(q2), _p(k2), _p(g), _p(h), _strides(*ctx.strides, gs, hs), _p(dq), _p(dk), _p(_aligned(qw)),
+             _p(_aligned(kw)), _is32(qw), _is32(kw), _p(cos), _p(sin), _p(positions),
+             int(positions is not None and positions.dtype == torch.int64), B, L, Hq, Hk, D, 0 if cos is None else 2 * cos.shape[1],
+             0 if cos is None else cos.shape[0], _c.c_float(ctx.eps), _p(status_tensor(dev)), _p(part), _p(targets[0]), _p(targets[1]),
+             _is32(targets[0]), _is32(targets[1]), *adds, _st())
+        return dq, dk, *grads, None, None, None, None
+
+
+def _is32(t) -> int:
+    return int(t is not None and t.dtype == torch.float32)
+
+
+@_on_device
+def qk_norm_rotary(q, k, q_weight, k_weight, eps, cos, sin, positions):
+    _require_bf16(q, k)
+    _require_norm_weight(q_weight)
+    _require_norm_weight(k_weight)
+    _require_one_device(q, k, q_weight, k_weight, cos, sin, positions)
+    _require_head_dim(q.shape[3], 0 if cos is None else 2 * cos.shape[1])
+    if positions is not None:
+        positions = positions.contiguous()
+    return _apply(_QKNormRotary, q, k, q_weight, k_weight, float(eps), _aligned(cos), _aligned(sin), positions)
+
+
+def _page_args(pages):
+    t = _KV_TYPES.get(pages.k.dtype)
+    if t is None:
+        raise TypeError(f"GPU pages hold bfloat16, float8_e4m3fn or int8, got {pages.k.dtype}")
+    if (pages.k.data_ptr() | pages.v.data_ptr()) & 15:
+        raise ValueError("pages begin on 16 bytes")
+    return (_p(pages.k), _p(pages.v), _p(pages.k_scale), _p(pages.v_scale), t, pages.k.shape[0], pages.k.shape[2])
+
+
+@_on_device
+def kv_cache_write(k, v, pages, block_table, lengths, counts, q, q_weight, k_weight, eps, cos, sin):
+    _require_bf16(k, v, q)
+    _require_norm_weight(q_weight)
+    _require_norm_weight(k_weight)
+    dev = _require_one_device(k, v, pages.k, q, q_weight, k_weight, cos, sin)
+    B, L, Hk, D = k.shape
+    rotary, rows = (0, 0) if cos is None else (2 * cos.shape[1], cos.shape[0])
+    _require_head_dim(D, rotary)
+    held = _page_args(pages)
+    (k, ks), (v, vs) = _head_view(k), _head_view(v)
+    q, qs = (None, (0, 0, 0)) if q is None else _head_view(q)
+    Hq = 0 if q is None else q.shape[2]
+    out = None if q is None else torch.empty(B, L, Hq, D, dtype=torch.bfloat16, device=dev)
+    if B and L:
+        _run("ssm_kv_write", _p(q), _p(k), _p(v), _strides(qs, ks, vs), _p(out), _p(_aligned(q_weight)), _p(_aligned(k_weight)),
+             _is32(q_weight), _is32(k_weight), _p(_aligned(cos)), _p(_aligned(sin)), rotary, rows, _c.c_float(eps), *held,
+             _p(block_table), block_table.shape[1], _p(lengths), _p(counts), B, L, Hq, Hk, D, _p(status_tensor(dev)), _st())
+        torch.autograd.graph.increment_version([t for t in pages if t is not None])
+    return out
+
+
+def kv_cache_read(pages, block_table, lengths, max_length, dtype):
+    return _kv_cache_read(pages.k, pages, block_table, lengths, int(max_length), dtype)
+
+
+@_on_device
+def _kv_cache_read(first, pages, block_table, lengths, max_length, dtype):
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"cached values are read as bfloat16 or float32, got {dtype}")
+    _, Hk, _, D = first.shape
+    _require_head_dim(D, 0)
+    held = _page_args(pages)
+    B = block_table.shape[0]
+    k, v = (torch.empty(B, max_length, Hk, D, dtype=dtype, device=first.device) for _ in range(2))
+    if B and max_length:
+        _run("ssm_kv_read", *held, _p(block_table), block_table.shape[1], _p(lengths), _p(k), _p(v), int(dtype == torch.float32), B,
+             max_length, Hk, D, _p(status_tensor(first.device)), _st())
+    return k, v
+
+
+@_on_device
+def paged_attention(q, pages, block_table, lengths, scale):
+    _require_bf16(q)
+    dev = _require_one_device(q, pages.k)
+    B, _, Hq, D = q.shape
+    _require_head_dim(D, 0)
+    held = _page_args(pages)
+    q, (qb, _, qh) = _head_view(q)
+    out = torch.empty(B, 1, Hq, D, dtype=torch.bfloat16, device=dev)
+    if B:
+        _run("ssm_paged_attn", _p(q), _ll(qb), _ll(qh), _p(out), *held, _p(block_table), block_table.shape[1], _p(lengths), B, Hq,
+             pages.k.shape[1], D, _c.c_float(1.0 / D ** 0.5 if scale is None else scale), _p(status_tensor(dev)), _st())
+    return out

@@ -19,6 +19,8 @@ from typing import Optional, Tuple
 import torch
 import torch.nn.functional as F
 
+from .kv_pages import QUANT_MAX, QUANT_TINY
+
 
 def softplus(x: torch.Tensor, threshold: float = 20.0) -> torch.Tensor:
     """log(1+exp(x)) with the identity above `threshold` (finite in fp32)."""
@@ -204,6 +206,126 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     p = torch.softmax(s, dim=-1)
     o = torch.matmul(p, vf)
     return o.permute(0, 2, 1, 3).to(q.dtype)
+
+
+# --------------------------------------------------------------------------------------
+# norms of queries and keys with rotation, paged key-value cache, attention of one new token
+# --------------------------------------------------------------------------------------
+def head_norm_rotary(x, weight, eps: float, cos=None, sin=None):
+    """RMS norm of every head of x [B, L, H, Dh] (weight None: no norm), then rotation by cos / sin [B or 1, L, rd / 2]
+    (None: no rotation), in fp32 (fp64 stays)."""
+    xf = x if x.dtype == torch.float64 else x.float()
+    if weight is not None:
+        xf = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps) * weight.to(xf.dtype)
+    if cos is None:
+        return xf
+    half = cos.shape[-1]
+    c, s = cos[:, :, None].to(xf.dtype), sin[:, :, None].to(xf.dtype)
+    a, b = xf[..., :half], xf[..., half:2 * half]
+    return torch.cat([a * c - b * s, b * c + a * s, xf[..., 2 * half:]], dim=-1)
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, eps: float, cos=None, sin=None, positions=None):
+    if cos is not None:
+        if positions is not None:
+            if positions.numel() and not (0 <= int(positions.min()) and int(positions.max()) < cos.shape[0]):
+                raise ValueError(f"positions outside the tables of {cos.shape[0]} rows")
+            cos, sin = cos[positions.long()], sin[positions.long()]
+        else:
+            cos, sin = cos[None, :q.shape[1]], sin[None, :q.shape[1]]
+    return (head_norm_rotary(q, q_weight, eps, cos, sin).to(q.dtype), head_norm_rotary(k, k_weight, eps, cos, sin).to(k.dtype))
+
+
+def quantise_rows(x, dtype):
+    """(stored, scale [...]) of the rows x [..., Dh]: scale = max |x| / largest value of the type, stored = x / scale rounded to
+    nearest even.  A row with a value that is not finite gets the scale NaN and reads back as NaN."""
+    xf = x if x.dtype == torch.float64 else x.float()
+    amax = xf.abs().amax(-1)
+    amax = torch.where(amax < QUANT_TINY, torch.zeros_like(amax), amax)
+    fine = torch.isfinite(amax)
+    scale = torch.where(fine, amax / QUANT_MAX[dtype], torch.full_like(amax, float("nan")))
+    y = xf / torch.where(fine & (amax > 0), scale, torch.ones_like(scale))[..., None]
+    y = torch.where((fine & (amax > 0))[..., None], y, torch.zeros_like(y))
+    return (y.round().to(dtype) if dtype == torch.int8 else y.float().to(dtype)), scale.float()
+
+
+def _bits(t):
+    """8-bit floats as bytes: indexing is not written for them."""
+    return t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
+
+
+def _page_of(pages, block_table, seq, at):
+    """Page ids of positions `at` of the sequences `seq` (same shape); raises for a position without a page."""
+    if at.numel() and int(at.max()) // pages.page_size >= block_table.shape[1]:
+        raise ValueError("a position lies behind the pages of the block table")
+    ids = block_table.long()[seq, at // pages.page_size]
+    if ids.numel() and not (0 <= int(ids.min()) and int(ids.max()) < pages.k.shape[0]):
+        raise ValueError("the block table names a page that does not exist")
+    return ids
+
+
+def kv_cache_write(k, v, pages, block_table, lengths, counts=None, q=None, q_weight=None, k_weight=None, eps: float = 1e-6,
+                   cos=None, sin=None):
+    B, L = k.shape[:2]
+    count = torch.full_like(lengths, L) if counts is None else counts
+    if B and not (0 <= int(count.min()) and int(count.max()) <= L):
+        raise ValueError(f"counts lie in [0, {L}]")
+    step = torch.arange(L, device=k.device)
+    at = (lengths - count).long()[:, None] + step
+    real = (step < count[:, None]) & (at >= 0)
+    c = s = None
+    if cos is not None:
+        if bool(real.any()) and int(at[real].max()) >= cos.shape[0]:
+            raise ValueError(f"positions outside the tables of {cos.shape[0]} rows")
+        rows = torch.where(real, at, torch.zeros_like(at))
+        c, s = cos[rows], sin[rows]
+    seq = torch.arange(B, device=k.device)[:, None].expand(B, L)[real]
+    ids, slot = _page_of(pages, block_table, seq, at[real]), at[real] % pages.page_size
+    for x, held, scales in ((head_norm_rotary(k, k_weight, eps, c, s), pages.k, pages.k_scale), (v, pages.v, pages.v_scale)):
+        x = x[real]
+        if scales is not None:
+            x, scale = quantise_rows(x, held.dtype)
+            scales[ids, :, slot] = scale
+        _bits(held)[ids, :, slot] = _bits(x.to(held.dtype))
+    if q is None:
+        return None
+    return torch.where(real[:, :, None, None], head_norm_rotary(q, q_weight, eps, c, s), torch.zeros(())).to(q.dtype)
+
+
+def _cached(pages, block_table, lengths, b: int):
+    """(k, v) of sequence b as [tokens, kv_heads, Dh] in fp32 (fp64 pages stay)."""
+    n = max(0, int(lengths[b]))
+    at = torch.arange(n, device=pages.k.device)
+    ids, slot = _page_of(pages, block_table, torch.full_like(at, b), at), at % pages.page_size
+    out = []
+    for held, scales in ((pages.k, pages.k_scale), (pages.v, pages.v_scale)):
+        x = _bits(held)[ids, :, slot].view(held.dtype)
+        x = x if x.dtype == torch.float64 else x.float()
+        out.append(x if scales is None else x * scales[ids, :, slot][..., None])
+    return out
+
+
+def kv_cache_read(pages, block_table, lengths, max_length: int, dtype=torch.bfloat16):
+    B, (_, Hkv, _, Dh) = block_table.shape[0], pages.k.shape
+    out = [torch.zeros(B, max_length, Hkv, Dh, dtype=dtype, device=pages.k.device) for _ in range(2)]
+    for b in range(B):
+        for x, into in zip(_cached(pages, block_table, lengths.clamp(max=max_length), b), out):
+            into[b, :x.shape[0]] = x.to(dtype)
+    return tuple(out)
+
+
+def paged_attention(q, pages, block_table, lengths, scale: Optional[float] = None):
+    B, _, Hq, Dh = q.shape
+    Hkv = pages.k.shape[1]
+    scale = 1.0 / math.sqrt(Dh) if scale is None else scale
+    out = torch.zeros_like(q, memory_format=torch.contiguous_format)
+    for b in range(B):
+        k, v = _cached(pages, block_table, lengths, b)
+        if k.shape[0]:
+            qb = q[b, 0].to(k.dtype).view(Hkv, Hq // Hkv, Dh)
+            p = torch.softmax(torch.einsum("kgd,tkd->kgt", qb, k) * scale, dim=-1)
+            out[b, 0] = torch.einsum("kgt,tkd->kgd", p, v).reshape(Hq, Dh).to(q.dtype)
+    return out
 
 
 # --------------------------------------------------------------------------------------
