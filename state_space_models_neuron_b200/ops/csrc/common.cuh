@@ -366,6 +366,8 @@ __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.lau
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // ---------------------------------------------------------------- misc
+// records a bad index of the caller's data; the access was skipped
+__device__ __forceinline__ void report_bad_index(int* status) { *status = SSM_ERR_BAD_ARG; }
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 __device__ __forceinline__ void unpack8(const uint4 u, float (&f)[8]) {

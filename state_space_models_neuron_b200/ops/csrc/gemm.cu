@@ -1148,7 +1148,7 @@ static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
   std::unique_lock<std::mutex> scratch_held;
   if (sc.split > 1 && p.mode != 2) {             // slices exchange fp32 partial sums through the stream's scratch
     Scratch s;
-    ScratchPool& pool = ScratchPool::get();
+    ScratchPool<SCRATCH_GEMM>& pool = ScratchPool<SCRATCH_GEMM>::get();
     scratch_held = std::unique_lock<std::mutex>(pool.lock);
     if (pool.take(stream, (size_t)MAX_UNITS * GEMM_BM * 256 * sizeof(float), MAX_UNITS, &s)) {
       p.ws = s.ws; p.ws_counters = s.counters;
@@ -1225,7 +1225,7 @@ extern "C" int ssm_gemm_ce_tiles(int M, int N, int K, int rows_per_shard) {
 }
 
 // out[3]: scratches of split tiles that are kept for streams, that belong to graphs, and that are spare
-extern "C" int ssm_gemm_scratch_count(int* out) { ssm::ScratchPool::get().count(out); return 0; }
+extern "C" int ssm_gemm_scratch_count(int* out) { ssm::ScratchPool<ssm::SCRATCH_GEMM>::get().count(out); return 0; }
 
 // The tiling and work distribution that a plain GEMM of this shape gets, without launching anything (host only; also
 // callable without a GPU, where 148 SMs are assumed): out[8] = {tile width BN, 1 if CTA-pair tiles, tiles along M,

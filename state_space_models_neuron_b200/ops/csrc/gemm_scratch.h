@@ -1,5 +1,5 @@
-// Scratch of the GEMM's split tail: fp32 partial sums and arrival counters (zero between launches).  Launches that may run at
-// once never share one: every stream has its own, and so has every stream of every graph capture, because a graph is replayed
+// Scratch of kernels that share a piece of work between blocks (the GEMM's split tail, the attention over a split cache): partial
+// sums and arrival counters (zero between launches).  Launches that may run at once never share one: every stream has its own, and so has every stream of every graph capture, because a graph is replayed
 // on whichever stream its owner likes.
 //   eager     kept per stream (by the runtime's id, which is not used again for a later stream), at most EAGER per device; the
 //             one that was used longest ago is freed for the next, which waits for the device
@@ -19,6 +19,9 @@ namespace ssm {
 
 struct Scratch { float* ws; int* counters; };
 
+// One pool for each use: what is kept there has one size.
+enum { SCRATCH_GEMM = 0, SCRATCH_ATTENTION = 1 };
+template <int USE>
 class ScratchPool {
  public:
   static constexpr int EAGER = 16, SPARE = 4;                // per device

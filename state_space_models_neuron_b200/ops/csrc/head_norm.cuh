@@ -65,7 +65,4 @@ __device__ __forceinline__ void turn16(float (&y)[16], const float (&cs)[8], con
     y[8 + i] = b * cs[i] + a * s;
   }
 }
-// records a bad index of the caller's data; the access was skipped
-__device__ __forceinline__ void report_bad_index(int* status) { *status = SSM_ERR_BAD_ARG; }
-
 }  // namespace ssm

@@ -1,34 +1,9 @@
-// Paged key-value cache: writing new tokens (keys normed and rotated, 8-bit values quantised in the same pass), reading sequences
-// back, and the attention of one new token.
-//
-// Pages are [page][kv head][slot][D]; a token at position p of sequence b is in slot p % page_size of page table[b][p / page_size].
-// 8-bit values have one fp32 scale per token and head, s = max |x| / Qmax; stored = round(x / s).
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
+// Paged key-value cache: writing new tokens (keys normed and rotated, 8-bit values quantised in the same pass) and reading sequences
+// back.  8-bit values have one fp32 scale per token and head, s = max |x| / Qmax; stored = round(x / s).
 #include "head_norm.cuh"
+#include "kv_pages.cuh"
 
 namespace ssm {
-
-enum { KV_BF16 = 0, KV_E4M3 = 1, KV_INT8 = 2 };
-template <int T> struct KvType;
-template <> struct KvType<KV_BF16> { static constexpr int BYTES = 2; };
-template <> struct KvType<KV_E4M3> { static constexpr int BYTES = 1; };
-template <> struct KvType<KV_INT8> { static constexpr int BYTES = 1; };
-
-struct PageTable {
-  const int* ids; const int* lengths;
-  int width, pages, page_shift;                // pages per sequence, pages in the pool, log2 of the page's tokens
-  int* status;
-};
-// page of position p of sequence b; -1 where the caller's table has none
-__device__ __forceinline__ int page_of(const PageTable& t, int b, int p) {
-  const int i = p >> t.page_shift;
-  int id = -1;
-  if (i < t.width) id = t.ids[(long long)b * t.width + i];
-  if (id >= 0 && id < t.pages) return id;
-  report_bad_index(t.status);
-  return -1;
-}
 
 __device__ __forceinline__ uint32_t e4m3x4(const float* f) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3);
@@ -190,100 +165,11 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const void* __restrict__ p
   }
 }
 
-struct AttnArgs {
-  const __nv_bfloat16* q; __nv_bfloat16* out;
-  long long qb, qh;
-  const void* pages[2];
-  const float* scales[2];
-  PageTable table;
-  int B, Hq, Hk;
-  float scale;
-};
-
-// One warp per query head and sequence: the lanes take a token each for the scores, then the channels.
-template <int D, int T>
-__global__ void __launch_bounds__(32) paged_attn_kernel(const AttnArgs a) {
-  const int b = blockIdx.y, hq = blockIdx.x, h = hq / (a.Hq / a.Hk), lane = threadIdx.x;
-  __shared__ float q[D];
-  for (int c = lane; c < D; c += 32) q[c] = __bfloat162float(a.q[b * a.qb + hq * a.qh + c]) * a.scale;
-  __syncwarp();
-  int n = a.table.lengths[b];
-  const long long capacity = (long long)a.table.width << a.table.page_shift;
-  if (n > capacity) { report_bad_index(a.table.status); n = (int)capacity; }
-  float m = -INFINITY, l = 0.f, o[D / 32];
-  #pragma unroll
-  for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
-  for (int t0 = 0; t0 < n; t0 += 32) {
-    const int t = t0 + lane;
-    long long slot = -1;
-    float s = -INFINITY;
-    if (t < n) {
-      const int page = page_of(a.table, b, t);
-      if (page >= 0) {
-        slot = (((long long)page * a.Hk + h) << a.table.page_shift) + (t & ((1 << a.table.page_shift) - 1));
-        s = 0.f;
-        for (int c = 0; c < D; ++c) {
-          const float k = T == KV_BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.pages[0])[slot * D + c])
-                                       : kv_value<T>(reinterpret_cast<const uint8_t*>(a.pages[0])[slot * D + c]);
-          s += q[c] * k;
-        }
-        if (T != KV_BF16) s *= a.scales[0][slot];
-      }
-    }
-    float mx = s;
-    #pragma unroll
-    for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-    const float mn = fmaxf(m, mx), ref = ce_ref(mn), corr = __expf(m - ref);
-    const float p = slot >= 0 ? __expf(s - ref) : 0.f;
-    l = l * corr + row_sum<32>(p);
-    m = mn;
-    #pragma unroll
-    for (int i = 0; i < D / 32; ++i) o[i] *= corr;
-    for (int j = 0; j < 32; ++j) {
-      const float pj = __shfl_sync(0xffffffffu, p, j);
-      const long long sj = __shfl_sync(0xffffffffu, slot, j);
-      if (sj < 0) continue;
-      const float vs = T == KV_BF16 ? pj : pj * a.scales[1][sj];
-      #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const float v = T == KV_BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.pages[1])[sj * D + i * 32 + lane])
-                                     : kv_value<T>(reinterpret_cast<const uint8_t*>(a.pages[1])[sj * D + i * 32 + lane]);
-        o[i] += vs * v;
-      }
-    }
-  }
-  #pragma unroll
-  for (int i = 0; i < D / 32; ++i)
-    a.out[((long long)b * a.Hq + hq) * D + i * 32 + lane] = __float2bfloat16(l == 0.f ? 0.f : o[i] / l);
-}
-
-static bool kv_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-static bool kv_table(PageTable* t, const void* ids, const void* lengths, int width, int pages, int page_size, int* status) {
-  if (width < 0 || pages < 0 || page_size < 16 || (page_size & (page_size - 1))) return false;
-  int shift = 0;
-  while ((1 << shift) < page_size) ++shift;
-  *t = PageTable{reinterpret_cast<const int*>(ids), reinterpret_cast<const int*>(lengths), width, pages, shift, status};
-  return true;
-}
 static unsigned kv_grid(long long blocks) { return (unsigned)(blocks < 148 * 8 ? blocks : 148 * 8); }
 
 }  // namespace ssm
 
 using namespace ssm;
-
-#define KV_DISPATCH(KERNEL)                                        \
-  do {                                                             \
-    if (D == 64 && type == KV_BF16) KERNEL(64, KV_BF16);           \
-    else if (D == 64 && type == KV_E4M3) KERNEL(64, KV_E4M3);      \
-    else if (D == 64 && type == KV_INT8) KERNEL(64, KV_INT8);      \
-    else if (D == 128 && type == KV_BF16) KERNEL(128, KV_BF16);    \
-    else if (D == 128 && type == KV_E4M3) KERNEL(128, KV_E4M3);    \
-    else if (D == 128 && type == KV_INT8) KERNEL(128, KV_INT8);    \
-    else if (D == 256 && type == KV_BF16) KERNEL(256, KV_BF16);    \
-    else if (D == 256 && type == KV_E4M3) KERNEL(256, KV_E4M3);    \
-    else if (D == 256 && type == KV_INT8) KERNEL(256, KV_INT8);    \
-    else return -SSM_ERR_BAD_ARG;                                  \
-  } while (0)
 
 // strides: (batch, token, head) of queries, keys and values
 extern "C" int ssm_kv_write(const void* q, const void* k, const void* v, const long long* strides, void* qo, const void* qw, const void* kw,
@@ -336,24 +222,5 @@ extern "C" int ssm_kv_read(const void* kp, const void* vp, const void* ks, const
     } while (0)
   KV_DISPATCH(READ);
   #undef READ
-  return (int)cudaGetLastError();
-}
-
-extern "C" int ssm_paged_attn(const void* q, long long qb, long long qh, void* out, const void* kp, const void* vp, const void* ks, const void* vs,
-                              int type, int pages, int page_size, const void* table, int width, const void* lengths, int B, int Hq, int Hk,
-                              int D, float scale, int* status, cudaStream_t st) {
-  AttnArgs a;
-  if (!kv_table(&a.table, table, lengths, width, pages, page_size, status)) return -SSM_ERR_BAD_ARG;
-  if (B < 1 || B > 65535 || Hk < 1 || Hq < Hk || Hq % Hk || qb % 8 || qh % 8 || !kv_aligned(q) || !kv_aligned(out) || !kv_aligned(kp) || !kv_aligned(vp))
-    return -SSM_ERR_BAD_ARG;
-  a.q = reinterpret_cast<const __nv_bfloat16*>(q);
-  a.out = reinterpret_cast<__nv_bfloat16*>(out);
-  a.qb = qb; a.qh = qh;
-  a.pages[0] = kp; a.pages[1] = vp;
-  a.scales[0] = reinterpret_cast<const float*>(ks); a.scales[1] = reinterpret_cast<const float*>(vs);
-  a.B = B; a.Hq = Hq; a.Hk = Hk; a.scale = scale;
-  #define ATTN(DD, TT) paged_attn_kernel<DD, TT><<<dim3(Hq, B), 32, 0, st>>>(a)
-  KV_DISPATCH(ATTN);
-  #undef ATTN
   return (int)cudaGetLastError();
 }

@@ -1,0 +1,637 @@
+// Attention of one new token per sequence over a paged key-value cache.
+//
+//   s_t = scale q . k_t,  o = sum_t 2^(s'_t - m) v_t / sum_t 2^(s'_t - m),  s' = s log2(e), m a running maximum
+//
+// Bound by reading the cache once: 2 D values per token and key head for 4 D operations per query head, so a key head's queries
+// (up to 8, or 16 with two column tiles) meet in one matrix product, tokens as rows and heads as columns:
+//   S^T[16 tokens, 8 heads] = K Q^T,  O^T[D, 8 heads] += V^T P^T     (mma.sync m16n8k16, fp32 sums)
+// The tcgen05 form has 128 rows of tokens, and its operands would have to be laid out in shared memory by TMA boxes of whole pages;
+// here the products take a fifth of the time that the bytes take, and every lane reads exactly the fragments that it multiplies:
+// the channels of a product may be in any order if both operands agree, and so may the rows of V^T.  A lane's 16-byte pieces of K
+// and V go from global memory into its own slots of a ring in shared memory (cp.async, two steps of 16 tokens in flight per warp)
+// and from there into its registers, without a barrier and without bank conflicts.  P^T is the transpose of the fragment in which
+// S^T comes: one movmatrix per 8 tokens.
+//
+// Work is cut into steps of 16 tokens of one key head, which lie in one page.  The steps of all sequences and key heads stand in one
+// row, and each block takes an equal share of it, however the lengths differ; a block's warps take every fourth step and meet at
+// the end of a sequence.  A sequence that several blocks share is joined by the one that finishes last, in the order of the
+// blocks: (m, sum, unnormalised o) of each from the caller's workspace.
+//
+// 8-bit values are multiplied in fp16, which holds them exactly: queries by a power of two per head that brings their largest
+// magnitude to [1, 2) (what is below 2^-24 of it is lost), probabilities with the scale of their value, as shares of a running
+// maximum of their own (M below: scales of tokens may be any numbers).
+#include "kv_pages.cuh"
+#include "gemm_scratch.h"
+
+namespace ssm {
+
+constexpr int PA_WARPS = 4, PA_STEP = 16, PA_COUNTERS = 1024;
+constexpr float PA_GROWTH = 8.f;               // a running maximum moves when scores pass it by 2^8: fp16 and bf16 hold the larger shares as well
+
+struct AttnArgs {
+  const __nv_bfloat16* q; __nv_bfloat16* out;
+  long long qb, qh;
+  const uint8_t* pages[2];
+  const float* scales[2];
+  PageTable table;
+  int B, Hq, Hk, groups, ratio;                // groups: of 8 or 16 query heads that share a key head; ratio: query heads per key head
+  float scale;                                 // times log2(e)
+  float* ws; int* counters;
+};
+
+template <int D, int T, int NT>
+struct PagedAttn {
+  static constexpr int BYTES = KvType<T>::BYTES, ROW = D * BYTES, HEADS = 8 * NT;
+  static constexpr int KCH = ROW / 64;                         // 16-byte pieces of a key row per lane (four lanes share a row)
+  static constexpr int VB = ROW >= 128 ? 16 : ROW / 8;         // bytes of a value piece (eight lanes share a row)
+  static constexpr int VCH = ROW / (8 * VB), VEL = VB / BYTES; // pieces per lane and row, values in a piece
+  static constexpr int K_BYTES = PA_STEP * ROW, SCALE_BYTES = T == KV_BF16 ? 0 : 128;
+  static constexpr int STAGE = 2 * K_BYTES + SCALE_BYTES;      // of one warp
+  static constexpr int STAGES = STAGE > 2304 ? 3 : 6;
+  static constexpr int SMEM = PA_WARPS * STAGES * STAGE;
+  static constexpr int BLOCKS = SMEM > 113 * 1024 ? 1 : SMEM > 56 * 1024 ? 2 : NT == 1 ? 4 : 3;      // per SM
+  static constexpr int SLOT = HEADS * D + 3 * HEADS;           // floats of a part: o, m, sum, M
+  static_assert(PA_WARPS * HEADS * D * 4 <= SMEM, "the warps' results meet in the ring");
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 t = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
+// four 8-bit values -> two pairs of fp16, exact
+template <int T>
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (T == KV_E4M3) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+  } else {
+    // 1024 + (x + 128) is an fp16 number whose low byte is x + 128
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));      // 1152
+    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  }
+}
+__device__ __forceinline__ float zero_if_inf(float m) { return m == -INFINITY ? 0.f : m; }
+// 2^(m - to), 0 for a part without tokens
+__device__ __forceinline__ float part_factor(float m, float to) { return m == -INFINITY ? 0.f : exp2f(m - to); }
+
+// what an unnormalised result is multiplied with; 0 where there are no tokens or all values are zeros
+__device__ __forceinline__ float out_factor(float m, float M, float sum) { return sum == 0.f || M == -INFINITY ? 0.f : exp2f(M - m) / sum; }
+
+// tokens of sequence b: not below 0, not beyond its pages
+__device__ __forceinline__ int tokens_of(const AttnArgs& a, int b) {
+  const int n = a.table.lengths[b];
+  const long long room = (long long)a.table.width << a.table.page_shift;
+  if (n <= room) return n < 0 ? 0 : n;
+  report_bad_index(a.table.status);
+  return (int)room;
+}
+__device__ __forceinline__ int steps_of(const AttnArgs& a, int b) { return (tokens_of(a, b) + PA_STEP - 1) / PA_STEP; }
+
+template <int D, int T, int NT>
+struct AttnWarp {
+  using C = PagedAttn<D, T, NT>;
+  static constexpr bool F16 = T != KV_BF16;
+  uint32_t qf[NT][D / 8];                      // Q^T fragments; [D / 32 or D / 64 blocks of channels][4 or 8 words]
+  float qs[NT][2];                             // what a sum of products of column 2c, 2c + 1 is multiplied with
+  float o[NT][D / 16][4], m[NT][2], l[NT][2], M[NT][2];
+
+  // queries of heads first .. first + HEADS - 1 of a key head; `real` of them exist
+  __device__ __forceinline__ void load_queries(const AttnArgs& a, const __nv_bfloat16* q, int real) {
+    const int g = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3;
+    #pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const bool some = nt * 8 + g < real;
+      const __nv_bfloat16* p = q + (nt * 8 + g) * a.qh;
+      if (!F16) {
+        #pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const uint4 u = some ? *reinterpret_cast<const uint4*>(p + i * 32 + c * 8) : make_uint4(0, 0, 0, 0);
+          qf[nt][i * 4] = u.x; qf[nt][i * 4 + 1] = u.y; qf[nt][i * 4 + 2] = u.z; qf[nt][i * 4 + 3] = u.w;
+        }
+        qs[nt][0] = qs[nt][1] = a.scale;
+      } else {
+        uint32_t top = 0;
+        #pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          #pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint4 u = some ? *reinterpret_cast<const uint4*>(p + i * 64 + c * 16 + j * 8) : make_uint4(0, 0, 0, 0);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              qf[nt][i * 8 + j * 4 + k] = w[k];
+              top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+            }
+          }
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // exponent of the head's largest magnitude; where it is not finite the values stay what they are
+        int e = (int)(top >> 7);
+        e = top == 0 || e == 255 ? 127 : min(e, 253);
+        const float down = __uint_as_float((uint32_t)(254 - e) << 23);                        // 2^(127 - e)
+        #pragma unroll
+        for (int k = 0; k < D / 8; ++k) qf[nt][k] = pack_f16(bf16_lo(qf[nt][k]) * down, bf16_hi(qf[nt][k]) * down);
+        // the columns of this lane's sums are heads 2c, 2c + 1, whose exponents lanes 8c and 8c + 4 know
+        #pragma unroll
+        for (int j = 0; j < 2; ++j) qs[nt][j] = a.scale * __uint_as_float((uint32_t)max(1, __shfl_sync(0xffffffffu, e, c * 8 + j * 4)) << 23);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void reset() {
+    #pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      #pragma unroll
+      for (int t = 0; t < D / 16; ++t) o[nt][t][0] = o[nt][t][1] = o[nt][t][2] = o[nt][t][3] = 0.f;
+      m[nt][0] = m[nt][1] = M[nt][0] = M[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+  }
+
+  // 16 tokens, of which the first `valid` count, from this warp's stage of the ring
+  __device__ __forceinline__ void step(const uint8_t* stage, int valid) {
+    const int lane = threadIdx.x & 31, g = lane >> 2;
+    float s[NT][4], s2[NT][4];
+    #pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) s[nt][i] = s2[nt][i] = 0.f;
+    }
+    #pragma unroll
+    for (int i = 0; i < C::KCH; ++i) {
+      const uint4 u = *reinterpret_cast<const uint4*>(stage + (i * 2) * 512 + lane * 16);
+      const uint4 v = *reinterpret_cast<const uint4*>(stage + (i * 2 + 1) * 512 + lane * 16);
+      const uint32_t a[4] = {u.x, u.y, u.z, u.w}, b[4] = {v.x, v.y, v.z, v.w};
+      if (!F16) {
+        #pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816<false>(s[nt], a[0], b[0], a[1], b[1], qf[nt][i * 4], qf[nt][i * 4 + 1]);
+          mma16816<false>(s2[nt], a[2], b[2], a[3], b[3], qf[nt][i * 4 + 2], qf[nt][i * 4 + 3]);
+        }
+      } else {
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a0, a1, b0, b1;
+          widen4<T>(a[j], a0, a1);
+          widen4<T>(b[j], b0, b1);
+          #pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma16816<true>(j & 1 ? s2[nt] : s[nt], a0, b0, a1, b1, qf[nt][i * 8 + j * 2], qf[nt][i * 8 + j * 2 + 1]);
+        }
+      }
+    }
+    // lane (g, c): tokens g and g + 8, heads 2c and 2c + 1 of each tile
+    float4 sc;                                  // scales of keys g, g + 8, of values g, g + 8
+    float lv[2], vn[2];                         // a value's scale is vn 2^lv
+    if (F16) {
+      sc = *reinterpret_cast<const float4*>(stage + 2 * C::K_BYTES + g * 16);
+      const float vs[2] = {sc.z, sc.w};
+      #pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t bits = __float_as_uint(vs[i]), e = (bits >> 23) & 255;
+        lv[i] = e == 0 ? -INFINITY : (float)((int)e - 126);
+        vn[i] = e == 0 ? 0.f : e == 255 ? vs[i] : __uint_as_float((bits & 0x807fffffu) | (126u << 23));
+      }
+    }
+    bool grows = false;
+    #pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = (s[nt][i] + s2[nt][i]) * qs[nt][i & 1];
+        if (F16) x *= i < 2 ? sc.x : sc.y;
+        if (valid < PA_STEP && g + (i >> 1) * 8 >= valid) x = -INFINITY;
+        s[nt][i] = x;
+        grows |= x > m[nt][i & 1] + PA_GROWTH;
+        if (F16) grows |= x + lv[i >> 1] > M[nt][i & 1] + PA_GROWTH;
+      }
+    }
+    if (__any_sync(0xffffffffu, grows)) {
+      #pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        #pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float x = fmaxf(s[nt][j], s[nt][j + 2]), y = F16 ? fmaxf(s[nt][j] + lv[0], s[nt][j + 2] + lv[1]) : 0.f;
+          #pragma unroll
+          for (int d = 4; d < 32; d <<= 1) {
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+            if (F16) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
+          }
+          x = fmaxf(x, m[nt][j]);
+          const float f = part_factor(m[nt][j], x);
+          l[nt][j] *= f;
+          m[nt][j] = x;
+          float fo = f;
+          if (F16) {
+            y = fmaxf(y, M[nt][j]);
+            fo = part_factor(M[nt][j], y);
+            M[nt][j] = y;
+          }
+          #pragma unroll
+          for (int t = 0; t < D / 16; ++t) { o[nt][t][j] *= fo; o[nt][t][j + 2] *= fo; }
+        }
+      }
+    }
+    uint32_t p[NT][2];
+    #pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float w[4];
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = exp2f(s[nt][i] - zero_if_inf(m[nt][i & 1]));
+        l[nt][i & 1] += w[i];
+        if (F16) w[i] = exp2f(s[nt][i] + lv[i >> 1] - zero_if_inf(M[nt][i & 1])) * vn[i >> 1];
+      }
+      p[nt][0] = transpose8x8(F16 ? pack_f16(w[0], w[1]) : pack_bf16(w[0], w[1]));
+      p[nt][1] = transpose8x8(F16 ? pack_f16(w[2], w[3]) : pack_bf16(w[2], w[3]));
+    }
+    const uint8_t* vst = stage + C::K_BYTES;
+    #pragma unroll
+    for (int k = 0; k < C::VCH; ++k) {
+      uint32_t x[4][C::VB / 4];                 // this lane's channels of tokens 2c, 2c + 1, 2c + 8, 2c + 9
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* src = vst + (k * 4 + i) * 32 * C::VB + lane * C::VB;
+        if (C::VB == 16) {
+          const uint4 u = *reinterpret_cast<const uint4*>(src);
+          x[i][0] = u.x; x[i][1] = u.y; x[i][2 % (C::VB / 4)] = u.z; x[i][3 % (C::VB / 4)] = u.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(src);
+          x[i][0] = u.x; x[i][1] = u.y;
+        }
+      }
+      #pragma unroll
+      for (int t = 0; t < C::VB / 4; ++t) {
+        if (!F16) {
+          const uint32_t a0 = __byte_perm(x[0][t], x[1][t], 0x5410), a1 = __byte_perm(x[0][t], x[1][t], 0x7632);
+          const uint32_t a2 = __byte_perm(x[2][t], x[3][t], 0x5410), a3 = __byte_perm(x[2][t], x[3][t], 0x7632);
+          #pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[nt][k * (C::VEL / 2) + t], a0, a1, a2, a3, p[nt][0], p[nt][1]);
+        } else {
+          uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
+          widen4<T>(__byte_perm(x[0][t], x[1][t], 0x5140), a0, a1);
+          widen4<T>(__byte_perm(x[2][t], x[3][t], 0x5140), a2, a3);
+          widen4<T>(__byte_perm(x[0][t], x[1][t], 0x7362), b0, b1);
+          widen4<T>(__byte_perm(x[2][t], x[3][t], 0x7362), b2, b3);
+          #pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816<true>(o[nt][k * (C::VEL / 2) + 2 * t], a0, a1, a2, a3, p[nt][0], p[nt][1]);
+            mma16816<true>(o[nt][k * (C::VEL / 2) + 2 * t + 1], b0, b1, b2, b3, p[nt][0], p[nt][1]);
+          }
+        }
+      }
+    }
+  }
+
+  // o[head][channel] into `to`; lanes with g == 0 put (m, sum, M) of their heads into `stats`
+  __device__ __forceinline__ void leave(float* to, float* stats) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    #pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      #pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int head = nt * 8 + 2 * c + j;
+        #pragma unroll
+        for (int t = 0; t < D / 16; ++t) {
+          const int k = t / (C::VEL / 2), e = t % (C::VEL / 2);
+          *reinterpret_cast<float2*>(to + head * D + k * 8 * C::VEL + g * C::VEL + 2 * e) = make_float2(o[nt][t][j], o[nt][t][j + 2]);
+        }
+        float sum = l[nt][j];
+        #pragma unroll
+        for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (g == 0) {
+          stats[head] = m[nt][j];
+          stats[C::HEADS + head] = sum;
+          stats[2 * C::HEADS + head] = F16 ? M[nt][j] : m[nt][j];
+        }
+      }
+    }
+  }
+};
+
+template <int D, int T, int NT>
+__global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) paged_attn_kernel(const AttnArgs a) {
+  using C = PagedAttn<D, T, NT>;
+  constexpr int HEADS = C::HEADS, THREADS = PA_WARPS * 32;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float stats[PA_WARPS][3 * HEADS];
+  __shared__ long long scan[PA_WARPS + 1];
+  __shared__ int found[2], arrived;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int items = a.Hk * a.groups;
+
+  // sequences without tokens
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    if (a.table.lengths[b] > 0 && a.table.width > 0) continue;
+    for (int i = threadIdx.x; i < a.Hq * D / 8; i += THREADS) reinterpret_cast<uint4*>(a.out + (long long)b * a.Hq * D)[i] = make_uint4(0, 0, 0, 0);
+  }
+
+  // where this block's share begins: sequence, and step within the sequence's row of steps
+  const int per = (a.B + THREADS - 1) / THREADS, b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += (long long)steps_of(a, b) * items;
+  long long upto = mine;
+  #pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += v;
+  }
+  if (lane == 31) scan[warp] = upto;
+  __syncthreads();
+  long long before = upto - mine, total = 0;
+  #pragma unroll
+  for (int w = 0; w < PA_WARPS; ++w) {
+    if (w < warp) before += scan[w];
+    total += scan[w];
+  }
+  long long share = (total + gridDim.x - 1) / gridDim.x;
+  share = max((long long)2 * PA_WARPS, (share + PA_WARPS - 1) / PA_WARPS * PA_WARPS);
+  long long u = share * blockIdx.x;
+  const long long end = min(total, u + share);
+  if (u >= end) return;
+  if (before <= u && u < before + mine) {
+    long long at = before;
+    int b = b0;
+    for (;; ++b) {
+      const long long n = (long long)steps_of(a, b) * items;
+      if (u < at + n) break;
+      at += n;
+    }
+    found[0] = b;
+    scan[PA_WARPS] = at;
+  }
+  __syncthreads();
+  int b = found[0];
+  long long seq0 = scan[PA_WARPS];             // first step of sequence b in the row
+
+  AttnWarp<D, T, NT> x;
+  uint8_t* my_ring = ring + warp * C::STAGES * C::STAGE;
+  const uint32_t my_ring32 = smem_u32(my_ring);
+  const int page_mask = (1 << a.table.page_shift) - 1, step_shift = a.table.page_shift - 4;
+
+  while (u < end) {
+    const int n = tokens_of(a, b), steps = (n + PA_STEP - 1) / PA_STEP;
+    if (u >= seq0 + (long long)steps * items) { seq0 += (long long)steps * items; ++b; continue; }
+    const int item = (int)((u - seq0) / steps), from = (int)((u - seq0) % steps), to = (int)min((long long)steps, from + (end - u));
+    const int hk = item / a.groups, first = (item % a.groups) * HEADS, real = min(HEADS, a.ratio - first);
+    const int head0 = hk * a.ratio + first;
+    x.load_queries(a, a.q + b * a.qb + head0 * a.qh, real);
+    x.reset();
+
+    const int count = to - from > warp ? (to - from - warp + PA_WARPS - 1) / PA_WARPS : 0;      // steps of this warp: from + warp + 4 j
+    const int* ids = a.table.ids + (long long)b * a.table.width;
+    int id = -1, valid[C::STAGES - 1];
+    auto issue = [&](int j) -> int {
+      int some = 0;
+      if (j < count) {
+        if ((j & 31) == 0) {
+          // the pages of this warp's next 32 steps, one per lane
+          const int k = j + lane;
+          id = -1;
+          if (k < count) {
+            id = ids[(from + warp + PA_WARPS * k) >> step_shift];
+            if (id < 0 || id >= a.table.pages) { report_bad_index(a.table.status); id = -1; }
+          }
+        }
+        const int page = __shfl_sync(0xffffffffu, id, j & 31), t0 = (from + warp + PA_WARPS * j) * PA_STEP;
+        some = page < 0 ? 0 : min(PA_STEP, n - t0);
+        // a page that does not exist reads nothing: all copies fill with zeros
+        const long long slot = (((long long)max(page, 0) * a.Hk + hk) << a.table.page_shift) + (t0 & page_mask);
+        const uint8_t* k0 = a.pages[0] + slot * C::ROW;
+        const uint8_t* v0 = a.pages[1] + slot * C::ROW;
+        const uint32_t dst = my_ring32 + (j % C::STAGES) * C::STAGE;
+        #pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int row = g + 8 * r, bytes = row < some ? 16 : 0;
+          #pragma unroll
+          for (int i = 0; i < C::KCH; ++i) cp_async16(dst + (i * 2 + r) * 512 + lane * 16, k0 + row * C::ROW + i * 64 + c * 16, bytes);
+        }
+        #pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 2 * c + (r & 1) + (r >> 1) * 8, bytes = row < some ? C::VB : 0;
+          #pragma unroll
+          for (int i = 0; i < C::VCH; ++i) {
+            const uint32_t to32 = dst + C::K_BYTES + (i * 4 + r) * 32 * C::VB + lane * C::VB;
+            const uint8_t* src = v0 + row * C::ROW + (i * 8 + g) * C::VB;
+            if (C::VB == 16) cp_async16(to32, src, bytes); else cp_async8(to32, src, bytes);
+          }
+        }
+        if (T != KV_BF16) {
+          const int row = g + 8 * (c & 1);
+          cp_async4(dst + 2 * C::K_BYTES + lane * 4, a.scales[c >> 1] + slot + row, row < some ? 4 : 0);
+        }
+      }
+      cp_async_commit();
+      return some;
+    };
+    #pragma unroll
+    for (int j = 0; j < C::STAGES - 1; ++j) valid[j] = issue(j);
+    for (int j = 0; j < count; ++j) {
+      cp_async_wait<C::STAGES - 2>();
+      __syncwarp();                            // scales come from other lanes' copies
+      const int now = valid[0];
+      #pragma unroll
+      for (int i = 0; i + 1 < C::STAGES - 1; ++i) valid[i] = valid[i + 1];
+      valid[C::STAGES - 2] = issue(j + C::STAGES - 1);
+      x.step(my_ring + (j % C::STAGES) * C::STAGE, now);
+      __syncwarp();                            // before the next copies into this stage
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+
+    // the warps meet
+    float* os = reinterpret_cast<float*>(ring);
+    __syncthreads();
+    x.leave(os + warp * HEADS * D, stats[warp]);
+    __syncthreads();
+    const long long item0 = seq0 + (long long)item * steps;
+    const bool whole = from == 0 && to == steps;
+    const int c0 = (int)(item0 / share), c1 = (int)((item0 + steps - 1) / share);
+    float* slot = whole ? nullptr : a.ws + ((long long)blockIdx.x * 2 + (c0 == (int)blockIdx.x)) * C::SLOT;
+    __nv_bfloat16* out = a.out + ((long long)b * a.Hq + head0) * D;
+    for (int i = threadIdx.x; i < (whole ? real : HEADS) * D / 4; i += THREADS) {
+      const int head = i * 4 / D;
+      float mm = -INFINITY, MM = -INFINITY, sum = 0.f;
+      #pragma unroll
+      for (int w = 0; w < PA_WARPS; ++w) { mm = fmaxf(mm, stats[w][head]); MM = fmaxf(MM, stats[w][2 * HEADS + head]); }
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      #pragma unroll
+      for (int w = 0; w < PA_WARPS; ++w) {
+        sum += stats[w][HEADS + head] * part_factor(stats[w][head], mm);
+        const float f = part_factor(stats[w][2 * HEADS + head], MM);
+        const float4 v = reinterpret_cast<const float4*>(os + w * HEADS * D)[i];
+        acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+      }
+      if (whole) {
+        const float f = out_factor(mm, MM, sum);
+        reinterpret_cast<uint2*>(out)[i] = make_uint2(pack_bf16(acc.x * f, acc.y * f), pack_bf16(acc.z * f, acc.w * f));
+      } else {
+        reinterpret_cast<float4*>(slot)[i] = acc;
+        if (i * 4 % D == 0) {
+          slot[HEADS * D + head] = mm;
+          slot[HEADS * D + HEADS + head] = sum;
+          slot[HEADS * D + 2 * HEADS + head] = MM;
+        }
+      }
+    }
+    if (!whole) {
+      __threadfence();
+      __syncthreads();
+      const int parts = c1 - c0 + 1;
+      if (threadIdx.x == 0) {
+        arrived = atomicAdd(a.counters + c0, 1);
+        if (arrived == parts - 1) a.counters[c0] = 0;
+        __threadfence();
+      }
+      __syncthreads();
+      if (arrived == parts - 1) {
+        // all parts are there: joined in the order of the blocks.  The first block holds its part in its second slot.
+        auto part = [&](int k) -> const float* { return a.ws + ((long long)(c0 + k) * 2 + (k == 0)) * C::SLOT; };
+        for (int i = threadIdx.x; i < real * D / 4; i += THREADS) {
+          const int head = i * 4 / D;
+          float mm = -INFINITY, MM = -INFINITY, sum = 0.f;
+          for (int k = 0; k < parts; ++k) {
+            mm = fmaxf(mm, __ldcg(part(k) + HEADS * D + head));
+            MM = fmaxf(MM, __ldcg(part(k) + HEADS * D + 2 * HEADS + head));
+          }
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          #pragma unroll 4
+          for (int k = 0; k < parts; ++k) {
+            const float* p = part(k);
+            sum += __ldcg(p + HEADS * D + HEADS + head) * part_factor(__ldcg(p + HEADS * D + head), mm);
+            const float f = part_factor(__ldcg(p + HEADS * D + 2 * HEADS + head), MM);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p) + i);
+            acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+          }
+          const float f = out_factor(mm, MM, sum);
+          reinterpret_cast<uint2*>(out)[i] = make_uint2(pack_bf16(acc.x * f, acc.y * f), pack_bf16(acc.z * f, acc.w * f));
+        }
+      }
+    }
+    u += to - from;
+    __syncthreads();                           // the ring and the statistics are free again
+  }
+}
+
+template <int D, int T, int NT>
+static int paged_attn_launch(const AttnArgs& a, int grid, cudaStream_t st) {
+  using C = PagedAttn<D, T, NT>;
+  static SmemOptIn opt;
+  if (int e = opt.ask(reinterpret_cast<const void*>(paged_attn_kernel<D, T, NT>), C::SMEM)) return e;
+  paged_attn_kernel<D, T, NT><<<grid, PA_WARPS * 32, C::SMEM, st>>>(a);
+  return (int)cudaGetLastError();
+}
+
+// Two column tiles for more than 8 query heads per key head; 256 channels leave registers for one.
+static bool two_tiles(int ratio, int D) { return ratio > 8 && D <= 128; }
+
+template <int D, int T, int NT>
+static void paged_attn_shape(int* blocks, int* slot) {
+  *blocks = PagedAttn<D, T, NT>::BLOCKS;
+  *slot = PagedAttn<D, T, NT>::SLOT;
+}
+// blocks of the launch, and floats of its workspace
+static int paged_attn_plan(int type, int width, int page_size, int B, int Hq, int Hk, int D, int* grid, long long* floats) {
+  int blocks = 0, slot = 0, sms = 0, dev = 0;
+  const int ratio = Hq / Hk;
+  const bool two = two_tiles(ratio, D);
+  #define SHAPE(DD, TT)                                                                  \
+    do {                                                                                 \
+      if (two) paged_attn_shape<DD, TT, (DD <= 128 ? 2 : 1)>(&blocks, &slot);            \
+      else paged_attn_shape<DD, TT, 1>(&blocks, &slot);                                  \
+    } while (0)
+  KV_DISPATCH(SHAPE);
+  #undef SHAPE
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return (int)cudaGetLastError();
+  const int group = two ? 16 : 8;
+  // no more blocks than shares of two steps per warp
+  const long long most = (long long)B * Hk * ((ratio + group - 1) / group) * (((long long)width * page_size + PA_STEP - 1) / PA_STEP);
+  const long long shares = (most + 2 * PA_WARPS - 1) / (2 * PA_WARPS);
+  long long n = (long long)sms * blocks;
+  if (n > PA_COUNTERS) n = PA_COUNTERS;
+  if (n > shares) n = shares;
+  *grid = n < 1 ? 1 : (int)n;
+  *floats = (long long)*grid * 2 * slot;
+  return 0;
+}
+
+}  // namespace ssm
+
+using namespace ssm;
+
+// floats of the workspace that ssm_paged_attn wants for these sizes on the current device; negative: an error
+extern "C" long long ssm_paged_attn_workspace(int type, int width, int page_size, int B, int Hq, int Hk, int D) {
+  int grid = 0;
+  long long floats = 0;
+  if (Hk < 1 || Hq < Hk || Hq % Hk || B < 1) return -SSM_ERR_BAD_ARG;
+  const int e = paged_attn_plan(type, width, page_size, B, Hq, Hk, D, &grid, &floats);
+  return e ? (e < 0 ? e : -e) : floats;
+}
+
+extern "C" int ssm_paged_attn(const void* q, long long qb, long long qh, void* out, const void* kp, const void* vp, const void* ks, const void* vs,
+                              int type, int pages, int page_size, const void* table, int width, const void* lengths, int B, int Hq, int Hk,
+                              int D, float scale, void* ws, long long ws_floats, int* status, cudaStream_t st) {
+  AttnArgs a;
+  if (!kv_table(&a.table, table, lengths, width, pages, page_size, status)) return -SSM_ERR_BAD_ARG;
+  if (B < 1 || Hk < 1 || Hq < Hk || Hq % Hk || qb % 8 || qh % 8 || !kv_aligned(q) || !kv_aligned(out) || !kv_aligned(kp) || !kv_aligned(vp) || !kv_aligned(ws))
+    return -SSM_ERR_BAD_ARG;
+  int grid = 0;
+  long long floats = 0;
+  if (int e = paged_attn_plan(type, width, page_size, B, Hq, Hk, D, &grid, &floats)) return e;
+  if (ws_floats < floats) return -SSM_ERR_BAD_ARG;
+  a.q = reinterpret_cast<const __nv_bfloat16*>(q);
+  a.out = reinterpret_cast<__nv_bfloat16*>(out);
+  a.qb = qb; a.qh = qh;
+  a.pages[0] = reinterpret_cast<const uint8_t*>(kp); a.pages[1] = reinterpret_cast<const uint8_t*>(vp);
+  a.scales[0] = reinterpret_cast<const float*>(ks); a.scales[1] = reinterpret_cast<const float*>(vs);
+  a.B = B; a.Hq = Hq; a.Hk = Hk; a.ratio = Hq / Hk;
+  const bool two = two_tiles(a.ratio, D);
+  a.groups = (a.ratio + (two ? 15 : 7)) / (two ? 16 : 8);
+  a.scale = scale * 1.4426950408889634f;
+  a.ws = reinterpret_cast<float*>(ws);
+  using Pool = ScratchPool<SCRATCH_ATTENTION>;
+  Pool& pool = Pool::get();
+  std::lock_guard<std::mutex> hold(pool.lock);
+  Scratch s;
+  if (!pool.take(st, 0, PA_COUNTERS, &s)) return (int)cudaErrorMemoryAllocation;
+  a.counters = s.counters;
+  #define ATTN(DD, TT)                                                                   \
+    do {                                                                                 \
+      if (two) return paged_attn_launch<DD, TT, (DD <= 128 ? 2 : 1)>(a, grid, st);       \
+      return paged_attn_launch<DD, TT, 1>(a, grid, st);                                  \
+    } while (0)
+  KV_DISPATCH(ATTN);
+  #undef ATTN
+  return -SSM_ERR_BAD_ARG;
+}

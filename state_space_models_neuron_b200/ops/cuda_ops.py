@@ -1524,6 +1524,17 @@ def _kv_cache_read(first, pages, block_table, lengths, max_length, dtype):
     return k, v
 
 
+@functools.lru_cache(maxsize=256)
+def _paged_workspace(device: int, *sizes) -> int:
+    """Floats of the attention's workspace for (type, width, page, B, Hq, Hkv, D) on the current device."""
+    fn = _lib().ssm_paged_attn_workspace
+    fn.restype = _c.c_longlong
+    n = int(fn(*sizes))
+    if n < 0:
+        raise RuntimeError(f"ssm_paged_attn_workspace failed with code {n}")
+    return n
+
+
 @_on_device
 def paged_attention(q, pages, block_table, lengths, scale):
     _require_bf16(q)
@@ -1534,6 +1545,8 @@ def paged_attention(q, pages, block_table, lengths, scale):
     q, (qb, _, qh) = _head_view(q)
     out = torch.empty(B, 1, Hq, D, dtype=torch.bfloat16, device=dev)
     if B:
-        _run("ssm_paged_attn", _p(q), _ll(qb), _ll(qh), _p(out), *held, _p(block_table), block_table.shape[1], _p(lengths), B, Hq,
-             pages.k.shape[1], D, _c.c_float(1.0 / D ** 0.5 if scale is None else scale), _p(status_tensor(dev)), _st())
+        Hk, width = pages.k.shape[1], block_table.shape[1]
+        ws = torch.empty(_paged_workspace(dev.index, held[4], width, held[6], B, Hq, Hk, D), dtype=torch.float32, device=dev)
+        _run("ssm_paged_attn", _p(q), _ll(qb), _ll(qh), _p(out), *held, _p(block_table), width, _p(lengths), B, Hq, Hk, D,
+             _c.c_float(1.0 / D ** 0.5 if scale is None else scale), _p(ws), _ll(ws.numel()), _p(status_tensor(dev)), _st())
     return out

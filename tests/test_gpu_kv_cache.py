@@ -132,13 +132,13 @@ def test_write_and_read(dtype, L, Hq, Hk, D, rotary, page, lengths, counts, norm
             assert same.transpose(1, 2)[~touched].all()
 
 
-def attention_bound(q, k, v, scale, lost=2 ** -25):
+def attention_bound(q, k, v, scale, lost=2 ** -24):
     """(result, bound) for one sequence in 64 bits: q [Hq, D], k / v [n, Hk, D].
     bound: an fp32 score is a sum of D products (at most D + 8 roundings), its exponential takes 2^-22 of the exponent more; the
     probabilities may be rounded to bf16 before they meet the values (2^-8 each); the result is rounded to bf16.
-    Beside 8-bit values a probability may be held in fp16, with its value's scale, as a share of the largest such product: fp16
-    steps by 2^-24 below 2^-14, so a share is off by at most half of that, 2^-25 (a share below it may vanish), and n of them by
-    n 2^-25 max_t(p_t max_c |v_tc|).  That can be all of a channel in which the one token with a large share holds a zero.  bf16 and
+    Beside 8-bit values a probability may be held in fp16, with its value's scale, as a share of a number that is at most twice the
+    largest such product (a power of two): fp16 steps by 2^-24 below 2^-14, so a share is off by at most half of that, 2^-25 (one below it may
+    vanish), and n of them by n 2^-24 max_t(p_t max_c |v_tc|).  That can be all of a channel in which the one token with a large share holds a zero.  bf16 and
     fp32 go down to 2^-126 (lost).  An fp32 product of probability and scale below 2^-126 is flushed to zero; a stored value is at
     most 448, so each token that does not hold zeros alone is off by at most 448 * 2^-126 (1e-35) by that."""
     n, Hk, D = k.shape
@@ -163,7 +163,7 @@ def check_attention(q, pages, table, lengths, out, scale=None):
             assert not out[b].any()
             continue
         k, v = stands_for(pages, table, b, n)
-        ref, bound = attention_bound(q[b, 0].double(), k, v, scale, 2 ** -126 if pages.k_scale is None else 2 ** -25)
+        ref, bound = attention_bound(q[b, 0].double(), k, v, scale, 2 ** -126 if pages.k_scale is None else 2 ** -24)
         far = (out[b, 0].double() - ref).abs()
         assert (far <= bound).all(), (b, n, (far - bound).max().item(), (far / bound).max().item())
 
