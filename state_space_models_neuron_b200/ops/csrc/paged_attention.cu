@@ -5,12 +5,11 @@
 // Bound by reading the cache once: 2 D values per token and key head for 4 D operations per query head, so a key head's queries
 // (up to 8, or 16 with two column tiles) meet in one matrix product, tokens as rows and heads as columns:
 //   S^T[16 tokens, 8 heads] = K Q^T,  O^T[D, 8 heads] += V^T P^T     (mma.sync m16n8k16, fp32 sums)
-// The tcgen05 form has 128 rows of tokens, and its operands would have to be laid out in shared memory by TMA boxes of whole pages;
-// here the products take a fifth of the time that the bytes take, and every lane reads exactly the fragments that it multiplies:
-// the channels of a product may be in any order if both operands agree, and so may the rows of V^T.  A lane's 16-byte pieces of K
-// and V go from global memory into its own slots of a ring in shared memory (cp.async, two steps of 16 tokens in flight per warp)
-// and from there into its registers, without a barrier and without bank conflicts.  P^T is the transpose of the fragment in which
-// S^T comes: one movmatrix per 8 tokens.
+// The products take a fraction of the time that the bytes take, so they need no tcgen05 and its tiles of 128 tokens.  Each warp
+// has a ring of its own in shared memory, which TMA fills (two steps of 16 tokens under way, a box of 16 rows x 128 swizzled bytes
+// for each), so no warp waits for another one.  Fragments are read as 16-byte vectors: the channels of a product may be in any order if both
+// operands agree, and so may the rows of V^T and, if P^T follows, the tokens; the orders below (sigma) are those without bank
+// conflicts.  P^T is the transpose of the fragment in which S^T comes: one movmatrix per 8 tokens.
 //
 // Work is cut into steps of 16 tokens of one key head, which lie in one page.  The steps of all sequences and key heads stand in one
 // row, and each block takes an equal share of it, however the lengths differ; a block's warps take every fourth step and meet at
@@ -42,30 +41,25 @@ struct AttnArgs {
 template <int D, int T, int NT>
 struct PagedAttn {
   static constexpr int BYTES = KvType<T>::BYTES, ROW = D * BYTES, HEADS = 8 * NT;
+  static constexpr int TILE = ROW >= 128 ? 128 : 64, TILES = ROW / TILE;      // bytes of a box's rows (and of its swizzle), boxes of a row
   static constexpr int KCH = ROW / 64;                         // 16-byte pieces of a key row per lane (four lanes share a row)
-  static constexpr int VB = ROW >= 128 ? 16 : ROW / 8;         // bytes of a value piece (eight lanes share a row)
-  static constexpr int VCH = ROW / (8 * VB), VEL = VB / BYTES; // pieces per lane and row, values in a piece
-  static constexpr int K_BYTES = PA_STEP * ROW, SCALE_BYTES = T == KV_BF16 ? 0 : 128;
-  static constexpr int STAGE = 2 * K_BYTES + SCALE_BYTES;      // of one warp
-  static constexpr int STAGES = STAGE > 2304 ? 3 : 6;
-  static constexpr int SMEM = PA_WARPS * STAGES * STAGE;
-  static constexpr int BLOCKS = SMEM > 113 * 1024 ? 1 : SMEM > 56 * 1024 ? 2 : NT == 1 ? 4 : 3;      // per SM
+  static constexpr int VB = TILE / 8, VEL = VB / BYTES;        // bytes and values of a lane's piece of a value row's tile (eight lanes share it)
+  static constexpr int K_BYTES = PA_STEP * ROW;
+  static constexpr int STAGE = 2 * K_BYTES;                    // of one warp: keys, values
+  static constexpr int LOADED = STAGE + (T == KV_BF16 ? 0 : 2 * PA_STEP * 4);  // with the scales
+  static constexpr int STAGES = STAGE > 2048 ? 3 : 6;
+  static constexpr int RING = PA_WARPS * STAGES * STAGE;
+  static constexpr int SMEM = RING + 1024;                     // boxes begin on 1024 bytes
+  static constexpr int BLOCKS = SMEM > 113 * 1024 ? 1 : SMEM > 55 * 1024 ? 2 : NT == 1 ? 4 : 3;      // per SM
   static constexpr int SLOT = HEADS * D + 3 * HEADS;           // floats of a part: o, m, sum, M
-  static_assert(PA_WARPS * HEADS * D * 4 <= SMEM, "the warps' results meet in the ring");
+  static_assert(PA_WARPS * HEADS * D * 4 <= RING, "the warps' results meet in the ring");
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// Token of row g of S^T (and of row g + 8, eight further), and 16-byte piece of a 128-byte row of V that lane group g takes: 0 4 1 5
+// 2 6 3 7.  The eight lanes of one access are two neighbouring groups; their rows (of K) or pieces (of V) differ in bit 2, so that the
+// swizzle, piece ^ row, sends them to eight different 16-byte columns.  Rows of 64 bytes keep their order.
+template <int TILE>
+__device__ __forceinline__ int sigma(int g) { return TILE == 128 ? ((g & 1) << 2) | (g >> 1) : g; }
 
 template <bool F16>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -180,8 +174,8 @@ struct AttnWarp {
   }
 
   // 16 tokens, of which the first `valid` count, from this warp's stage of the ring
-  __device__ __forceinline__ void step(const uint8_t* stage, int valid) {
-    const int lane = threadIdx.x & 31, g = lane >> 2;
+  __device__ __forceinline__ void step(const uint8_t* stage, const float* scales, int valid) {
+    const int g = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3, tok = sigma<C::TILE>(g);
     float s[NT][4], s2[NT][4];
     #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -190,8 +184,10 @@ struct AttnWarp {
     }
     #pragma unroll
     for (int i = 0; i < C::KCH; ++i) {
-      const uint4 u = *reinterpret_cast<const uint4*>(stage + (i * 2) * 512 + lane * 16);
-      const uint4 v = *reinterpret_cast<const uint4*>(stage + (i * 2 + 1) * 512 + lane * 16);
+      // piece c or 4 + c of the tile's row
+      const int at = C::TILE == 128 ? (i >> 1) * PA_STEP * 128 + tok * 128 + ((((i & 1) * 4 + c) ^ tok) << 4) : tok * 64 + ((c ^ ((tok >> 1) & 3)) << 4);
+      const uint4 u = *reinterpret_cast<const uint4*>(stage + at);
+      const uint4 v = *reinterpret_cast<const uint4*>(stage + at + 8 * C::TILE);
       const uint32_t a[4] = {u.x, u.y, u.z, u.w}, b[4] = {v.x, v.y, v.z, v.w};
       if (!F16) {
         #pragma unroll
@@ -211,17 +207,17 @@ struct AttnWarp {
         }
       }
     }
-    // lane (g, c): tokens g and g + 8, heads 2c and 2c + 1 of each tile
-    float4 sc;                                  // scales of keys g, g + 8, of values g, g + 8
-    float lv[2], vn[2];                         // a value's scale is vn 2^lv
+    // lane (g, c): tokens tok and tok + 8, heads 2c and 2c + 1 of each tile
+    float ks[2], lv[2], vn[2];                  // scales of the keys; a value's scale is vn 2^lv
     if (F16) {
-      sc = *reinterpret_cast<const float4*>(stage + 2 * C::K_BYTES + g * 16);
-      const float vs[2] = {sc.z, sc.w};
       #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint32_t bits = __float_as_uint(vs[i]), e = (bits >> 23) & 255;
-        lv[i] = e == 0 ? -INFINITY : (float)((int)e - 126);
-        vn[i] = e == 0 ? 0.f : e == 255 ? vs[i] : __uint_as_float((bits & 0x807fffffu) | (126u << 23));
+        ks[i] = scales[tok + 8 * i];
+        const float vs = scales[PA_STEP + tok + 8 * i];
+        const uint32_t bits = __float_as_uint(vs), e = (bits >> 23) & 255;
+        const bool none = e == 0 || tok + 8 * i >= valid;
+        lv[i] = none ? -INFINITY : (float)((int)e - 126);
+        vn[i] = none ? 0.f : e == 255 ? vs : __uint_as_float((bits & 0x807fffffu) | (126u << 23));
       }
     }
     bool grows = false;
@@ -230,8 +226,8 @@ struct AttnWarp {
       #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float x = (s[nt][i] + s2[nt][i]) * qs[nt][i & 1];
-        if (F16) x *= i < 2 ? sc.x : sc.y;
-        if (valid < PA_STEP && g + (i >> 1) * 8 >= valid) x = -INFINITY;
+        if (F16) x *= ks[i >> 1];
+        if (tok + (i >> 1) * 8 >= valid) x = -INFINITY;
         s[nt][i] = x;
         grows |= x > m[nt][i & 1] + PA_GROWTH;
         if (F16) grows |= x + lv[i >> 1] > M[nt][i & 1] + PA_GROWTH;
@@ -278,17 +274,23 @@ struct AttnWarp {
     }
     const uint8_t* vst = stage + C::K_BYTES;
     #pragma unroll
-    for (int k = 0; k < C::VCH; ++k) {
-      uint32_t x[4][C::VB / 4];                 // this lane's channels of tokens 2c, 2c + 1, 2c + 8, 2c + 9
+    for (int k = 0; k < C::TILES; ++k) {
+      // this lane's channels of the tokens that are P^T's rows 2c, 2c + 1, 2c + 8, 2c + 9
+      uint32_t x[4][C::VB / 4];
       #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint8_t* src = vst + (k * 4 + i) * 32 * C::VB + lane * C::VB;
-        if (C::VB == 16) {
-          const uint4 u = *reinterpret_cast<const uint4*>(src);
+        const int row = (C::TILE == 128 ? c + 4 * (i & 1) : 2 * c + (i & 1)) + 8 * (i >> 1);
+        const uint8_t* src = vst + k * PA_STEP * C::TILE + row * C::TILE;
+        if (C::TILE == 128) {
+          const uint4 u = *reinterpret_cast<const uint4*>(src + ((sigma<128>(g) ^ (row & 7)) << 4));
           x[i][0] = u.x; x[i][1] = u.y; x[i][2 % (C::VB / 4)] = u.z; x[i][3 % (C::VB / 4)] = u.w;
         } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(src);
+          const uint2 u = *reinterpret_cast<const uint2*>(src + (((g >> 1) ^ c) << 4) + (g & 1) * 8);
           x[i][0] = u.x; x[i][1] = u.y;
+        }
+        if (valid < PA_STEP && row >= valid) {  // what lies behind a sequence may be NaN, which no zero share takes away
+          #pragma unroll
+          for (int t = 0; t < C::VB / 4; ++t) x[i][t] = 0;
         }
       }
       #pragma unroll
@@ -325,7 +327,7 @@ struct AttnWarp {
         #pragma unroll
         for (int t = 0; t < D / 16; ++t) {
           const int k = t / (C::VEL / 2), e = t % (C::VEL / 2);
-          *reinterpret_cast<float2*>(to + head * D + k * 8 * C::VEL + g * C::VEL + 2 * e) = make_float2(o[nt][t][j], o[nt][t][j + 2]);
+          *reinterpret_cast<float2*>(to + head * D + k * 8 * C::VEL + sigma<C::TILE>(g) * C::VEL + 2 * e) = make_float2(o[nt][t][j], o[nt][t][j + 2]);
         }
         float sum = l[nt][j];
         #pragma unroll
@@ -341,16 +343,25 @@ struct AttnWarp {
 };
 
 template <int D, int T, int NT>
-__global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) paged_attn_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) paged_attn_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
+                                                                                            const __grid_constant__ CUtensorMap vmap) {
   using C = PagedAttn<D, T, NT>;
   constexpr int HEADS = C::HEADS, THREADS = PA_WARPS * 32;
-  extern __shared__ __align__(16) uint8_t ring[];
+  extern __shared__ uint8_t dynamic[];
+  uint8_t* ring = dynamic + (1024 - (smem_u32(dynamic) & 1023)) % 1024;
+  __shared__ __align__(16) float scales[T == KV_BF16 ? 1 : PA_WARPS * C::STAGES][2 * PA_STEP];
+  __shared__ uint64_t full[PA_WARPS][C::STAGES];
   __shared__ float stats[PA_WARPS][3 * HEADS];
   __shared__ long long scan[PA_WARPS + 1];
   __shared__ int found[2], arrived;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int items = a.Hk * a.groups;
 
+  if (lane == 0) {
+    #pragma unroll
+    for (int i = 0; i < C::STAGES; ++i) mbar_init(&full[warp][i], 1);
+    mbar_fence_init();
+  }
   // sequences without tokens
   for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
     if (a.table.lengths[b] > 0 && a.table.width > 0) continue;
@@ -397,8 +408,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
 
   AttnWarp<D, T, NT> x;
   uint8_t* my_ring = ring + warp * C::STAGES * C::STAGE;
-  const uint32_t my_ring32 = smem_u32(my_ring);
   const int page_mask = (1 << a.table.page_shift) - 1, step_shift = a.table.page_shift - 4;
+  int put = 0, got = 0;                        // stages of the ring: next to fill, next to read
+  uint32_t parity = 0;                         // of the next to read
+  bool alive = true;                           // no wait of this warp has run out
 
   while (u < end) {
     const int n = tokens_of(a, b), steps = (n + PA_STEP - 1) / PA_STEP;
@@ -412,63 +425,58 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
     const int count = to - from > warp ? (to - from - warp + PA_WARPS - 1) / PA_WARPS : 0;      // steps of this warp: from + warp + 4 j
     const int* ids = a.table.ids + (long long)b * a.table.width;
     int id = -1, valid[C::STAGES - 1];
+    // starts the copies of step j; its tokens, 0 where it has no page
     auto issue = [&](int j) -> int {
-      int some = 0;
-      if (j < count) {
-        if ((j & 31) == 0) {
-          // the pages of this warp's next 32 steps, one per lane
-          const int k = j + lane;
-          id = -1;
-          if (k < count) {
-            id = ids[(from + warp + PA_WARPS * k) >> step_shift];
-            if (id < 0 || id >= a.table.pages) { report_bad_index(a.table.status); id = -1; }
-          }
-        }
-        const int page = __shfl_sync(0xffffffffu, id, j & 31), t0 = (from + warp + PA_WARPS * j) * PA_STEP;
-        some = page < 0 ? 0 : min(PA_STEP, n - t0);
-        // a page that does not exist reads nothing: all copies fill with zeros
-        const long long slot = (((long long)max(page, 0) * a.Hk + hk) << a.table.page_shift) + (t0 & page_mask);
-        const uint8_t* k0 = a.pages[0] + slot * C::ROW;
-        const uint8_t* v0 = a.pages[1] + slot * C::ROW;
-        const uint32_t dst = my_ring32 + (j % C::STAGES) * C::STAGE;
-        #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int row = g + 8 * r, bytes = row < some ? 16 : 0;
-          #pragma unroll
-          for (int i = 0; i < C::KCH; ++i) cp_async16(dst + (i * 2 + r) * 512 + lane * 16, k0 + row * C::ROW + i * 64 + c * 16, bytes);
-        }
-        #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 2 * c + (r & 1) + (r >> 1) * 8, bytes = row < some ? C::VB : 0;
-          #pragma unroll
-          for (int i = 0; i < C::VCH; ++i) {
-            const uint32_t to32 = dst + C::K_BYTES + (i * 4 + r) * 32 * C::VB + lane * C::VB;
-            const uint8_t* src = v0 + row * C::ROW + (i * 8 + g) * C::VB;
-            if (C::VB == 16) cp_async16(to32, src, bytes); else cp_async8(to32, src, bytes);
-          }
-        }
-        if (T != KV_BF16) {
-          const int row = g + 8 * (c & 1);
-          cp_async4(dst + 2 * C::K_BYTES + lane * 4, a.scales[c >> 1] + slot + row, row < some ? 4 : 0);
+      if (j >= count) return 0;
+      if ((j & 31) == 0) {
+        // the pages of this warp's next 32 steps, one per lane
+        const int k = j + lane;
+        id = -1;
+        if (k < count) {
+          id = ids[(from + warp + PA_WARPS * k) >> step_shift];
+          if (id < 0 || id >= a.table.pages) { report_bad_index(a.table.status); id = -1; }
         }
       }
-      cp_async_commit();
-      return some;
+      const int page = __shfl_sync(0xffffffffu, id, j & 31), t0 = (from + warp + PA_WARPS * j) * PA_STEP;
+      if (page < 0 || !alive) return 0;
+      if (lane == 0) {
+        const long long slot = (((long long)page * a.Hk + hk) << a.table.page_shift) + (t0 & page_mask);     // below 2^31: the host sees to it
+        uint64_t* bar = &full[warp][put];
+        uint8_t* dst = my_ring + put * C::STAGE;
+        mbar_expect_tx(bar, C::LOADED);
+        #pragma unroll
+        for (int i = 0; i < C::TILES; ++i) {
+          tma_load_2d(dst + i * PA_STEP * C::TILE, &kmap, i * C::TILE / C::BYTES, (int)slot, bar);
+          tma_load_2d(dst + C::K_BYTES + i * PA_STEP * C::TILE, &vmap, i * C::TILE / C::BYTES, (int)slot, bar);
+        }
+        if (T != KV_BF16) {
+          float* sc = scales[warp * C::STAGES + put];
+          bulk_load(sc, a.scales[0] + slot, PA_STEP * 4, bar);
+          bulk_load(sc + PA_STEP, a.scales[1] + slot, PA_STEP * 4, bar);
+        }
+      }
+      put = put + 1 == C::STAGES ? 0 : put + 1;
+      return min(PA_STEP, n - t0);
     };
     #pragma unroll
     for (int j = 0; j < C::STAGES - 1; ++j) valid[j] = issue(j);
     for (int j = 0; j < count; ++j) {
-      cp_async_wait<C::STAGES - 2>();
-      __syncwarp();                            // scales come from other lanes' copies
       const int now = valid[0];
       #pragma unroll
       for (int i = 0; i + 1 < C::STAGES - 1; ++i) valid[i] = valid[i + 1];
-      valid[C::STAGES - 2] = issue(j + C::STAGES - 1);
-      x.step(my_ring + (j % C::STAGES) * C::STAGE, now);
+      valid[C::STAGES - 2] = issue(j + C::STAGES - 1);         // into the stage that was read last
+      if (now == 0) continue;
+      // also a warp that has given up waits for each of its copies: none is under way when the block ends
+      if (!mbar_try_wait(&full[warp][got], parity) && !mbar_wait(&full[warp][got], parity, nullptr)) {
+        atomicCAS(a.table.status, 0, SSM_ERR_TIMEOUT_MBAR);
+        alive = false;
+      }
+      alive = __all_sync(0xffffffffu, alive);
+      if (alive) x.step(my_ring + got * C::STAGE, T == KV_BF16 ? nullptr : scales[warp * C::STAGES + got], now);
+      got = got + 1 == C::STAGES ? 0 : got + 1;
+      parity ^= got == 0;
       __syncwarp();                            // before the next copies into this stage
     }
-    cp_async_wait<0>();
-    __syncwarp();
 
     // the warps meet
     float* os = reinterpret_cast<float*>(ring);
@@ -540,7 +548,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
       }
     }
     u += to - from;
-    __syncthreads();                           // the ring and the statistics are free again
+    fence_proxy_async_smem();
+    __syncthreads();                           // the ring, for TMA to write, and the statistics are free again
   }
 }
 
@@ -549,7 +558,13 @@ static int paged_attn_launch(const AttnArgs& a, int grid, cudaStream_t st) {
   using C = PagedAttn<D, T, NT>;
   static SmemOptIn opt;
   if (int e = opt.ask(reinterpret_cast<const void*>(paged_attn_kernel<D, T, NT>), C::SMEM)) return e;
-  paged_attn_kernel<D, T, NT><<<grid, PA_WARPS * 32, C::SMEM, st>>>(a);
+  CUtensorMap map[2];
+  const uint64_t rows = ((uint64_t)a.table.pages * a.Hk) << a.table.page_shift;
+  for (int i = 0; i < 2; ++i)
+    if (make_tmap_2d(&map[i], C::BYTES == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, C::BYTES, a.pages[i], D, rows, C::ROW,
+                     C::TILE / C::BYTES, PA_STEP, C::TILE == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
+      return -SSM_ERR_BAD_ARG;
+  paged_attn_kernel<D, T, NT><<<grid, PA_WARPS * 32, C::SMEM, st>>>(a, map[0], map[1]);
   return (int)cudaGetLastError();
 }
 
@@ -606,6 +621,7 @@ extern "C" int ssm_paged_attn(const void* q, long long qb, long long qh, void* o
   if (!kv_table(&a.table, table, lengths, width, pages, page_size, status)) return -SSM_ERR_BAD_ARG;
   if (B < 1 || Hk < 1 || Hq < Hk || Hq % Hk || qb % 8 || qh % 8 || !kv_aligned(q) || !kv_aligned(out) || !kv_aligned(kp) || !kv_aligned(vp) || !kv_aligned(ws))
     return -SSM_ERR_BAD_ARG;
+  if (pages < 1 || (long long)pages * Hk * page_size > 0x7fffffffll || !kv_aligned(ks) || !kv_aligned(vs)) return -SSM_ERR_BAD_ARG;
   int grid = 0;
   long long floats = 0;
   if (int e = paged_attn_plan(type, width, page_size, B, Hq, Hk, D, &grid, &floats)) return e;

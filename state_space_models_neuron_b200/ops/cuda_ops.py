@@ -1546,6 +1546,8 @@ def paged_attention(q, pages, block_table, lengths, scale):
     out = torch.empty(B, 1, Hq, D, dtype=torch.bfloat16, device=dev)
     if B:
         Hk, width = pages.k.shape[1], block_table.shape[1]
+        if pages.k.numel() // D >= 2 ** 31:
+            raise ValueError("the attention kernel reads pools of less than 2^31 rows (pages x key heads x page size)")
         ws = torch.empty(_paged_workspace(dev.index, held[4], width, held[6], B, Hq, Hk, D), dtype=torch.float32, device=dev)
         _run("ssm_paged_attn", _p(q), _ll(qb), _ll(qh), _p(out), *held, _p(block_table), width, _p(lengths), B, Hq, Hk, D,
              _c.c_float(1.0 / D ** 0.5 if scale is None else scale), _p(ws), _ll(ws.numel()), _p(status_tensor(dev)), _st())
