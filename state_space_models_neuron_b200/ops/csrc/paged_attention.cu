@@ -24,7 +24,9 @@
 
 namespace ssm {
 
-constexpr int PA_WARPS = 4, PA_STEP = 16, PA_COUNTERS = 1024;
+constexpr int PA_WARPS = 4, PA_STEP = 16, PA_COUNTERS = 768;
+constexpr int PA_MIN_SHARE = 2 * PA_WARPS;     // steps: two per warp
+constexpr int FEW_ITEMS = 8;                   // blocks per item, see the kernel
 constexpr float PA_GROWTH = 8.f;               // a running maximum moves when scores pass it by 2^8: fp16 and bf16 hold the larger shares as well
 
 struct AttnArgs {
@@ -33,7 +35,7 @@ struct AttnArgs {
   const uint8_t* pages[2];
   const float* scales[2];
   PageTable table;
-  int B, Hq, Hk, groups, ratio;                // groups: of 8 or 16 query heads that share a key head; ratio: query heads per key head
+  int B, Hq, Hk, most_blocks, groups, ratio;   // groups: of 8 or 16 query heads that share a key head; ratio: query heads per key head
   float scale;                                 // times log2(e)
   float* ws; int* counters;
 };
@@ -52,7 +54,7 @@ struct PagedAttn {
   static constexpr int SMEM = RING + 1024;                     // boxes begin on 1024 bytes
   static constexpr int BLOCKS = SMEM > 113 * 1024 ? 1 : SMEM > 55 * 1024 ? 2 : NT == 1 ? 4 : 3;      // per SM
   static constexpr int SLOT = HEADS * D + 3 * HEADS;           // floats of a part: o, m, sum, M
-  static_assert(PA_WARPS * HEADS * D * 4 <= RING, "the warps' results meet in the ring");
+  static_assert(PA_WARPS * HEADS * D * 4 <= RING && PA_COUNTERS * HEADS * 4 <= RING, "the warps' results, and factors of parts, meet in the ring");
 };
 
 // Token of row g of S^T (and of row g + 8, eight further), and 16-byte piece of a 128-byte row of V that lane group g takes: 0 4 1 5
@@ -110,6 +112,36 @@ __device__ __forceinline__ int tokens_of(const AttnArgs& a, int b) {
   return (int)room;
 }
 __device__ __forceinline__ int steps_of(const AttnArgs& a, int b) { return (tokens_of(a, b) + PA_STEP - 1) / PA_STEP; }
+
+// inclusive sum over the block's threads, and of all
+template <int WARPS>
+__device__ __forceinline__ void block_scan(long long& upto, long long& total, long long* sums) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  #pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += v;
+  }
+  __syncthreads();
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  total = 0;
+  #pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) upto += sums[w];
+    total += sums[w];
+  }
+}
+template <int WARPS>
+__device__ __forceinline__ int block_count(int n, int* sums) {
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x / 32] = n;
+  __syncthreads();
+  int all = 0;
+  #pragma unroll
+  for (int w = 0; w < WARPS; ++w) all += sums[w];
+  return all;
+}
 
 template <int D, int T, int NT>
 struct AttnWarp {
@@ -352,8 +384,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
   __shared__ __align__(16) float scales[T == KV_BF16 ? 1 : PA_WARPS * C::STAGES][2 * PA_STEP];
   __shared__ uint64_t full[PA_WARPS][C::STAGES];
   __shared__ float stats[PA_WARPS][3 * HEADS];
-  __shared__ long long scan[PA_WARPS + 1];
-  __shared__ int found[2], arrived;
+  __shared__ long long scan[PA_WARPS], seq_start;
+  __shared__ int counts[PA_WARPS], found, arrived;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int items = a.Hk * a.groups;
 
@@ -368,43 +400,45 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
     for (int i = threadIdx.x; i < a.Hq * D / 8; i += THREADS) reinterpret_cast<uint4*>(a.out + (long long)b * a.Hq * D)[i] = make_uint4(0, 0, 0, 0);
   }
 
-  // where this block's share begins: sequence, and step within the sequence's row of steps
+  // Where this block's share begins.  The steps of all sequences and heads stand in a row, each sequence's heads one behind the other.
+  // Many of them (items): blocks cut the row at equal distances, wherever that is.  Few: every item is cut by itself, so that no
+  // block has parts of two, at the price of up to one shorter share per item.
   const int per = (a.B + THREADS - 1) / THREADS, b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
   long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += (long long)steps_of(a, b) * items;
-  long long upto = mine;
-  #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, upto, d);
-    if (lane >= d) upto += v;
-  }
-  if (lane == 31) scan[warp] = upto;
-  __syncthreads();
-  long long before = upto - mine, total = 0;
-  #pragma unroll
-  for (int w = 0; w < PA_WARPS; ++w) {
-    if (w < warp) before += scan[w];
-    total += scan[w];
-  }
+  int some = 0;
+  for (int b = b0; b < b1; ++b) { const int n = steps_of(a, b); mine += (long long)n * items; some += n > 0; }
+  long long upto = mine, total;
+  block_scan<PA_WARPS>(upto, total, scan);
+  const long long used = (long long)block_count<PA_WARPS>(some, counts) * items;     // items with steps
+  const bool few = used * FEW_ITEMS <= a.most_blocks;
   long long share = (total + gridDim.x - 1) / gridDim.x;
-  share = max((long long)2 * PA_WARPS, (share + PA_WARPS - 1) / PA_WARPS * PA_WARPS);
-  long long u = share * blockIdx.x;
-  const long long end = min(total, u + share);
+  if (few) share = (total + a.most_blocks - used - 1) / (a.most_blocks - used);       // at most most_blocks in all
+  share = max((long long)PA_MIN_SHARE, (share + PA_WARPS - 1) / PA_WARPS * PA_WARPS);
+  if (few) {
+    // counted in shares from here on
+    mine = 0;
+    for (int b = b0; b < b1; ++b) mine += (steps_of(a, b) + share - 1) / share * items;
+    upto = mine;
+    block_scan<PA_WARPS>(upto, total, scan);
+  }
+  const long long unit = few ? 1 : share;       // of the row, per block
+  long long u = unit * blockIdx.x;
+  const long long end = min(total, u + unit), before = upto - mine;
   if (u >= end) return;
-  if (before <= u && u < before + mine) {
+  if (before <= u && u < upto) {
     long long at = before;
     int b = b0;
     for (;; ++b) {
-      const long long n = (long long)steps_of(a, b) * items;
+      const long long n = (few ? (steps_of(a, b) + share - 1) / share : (long long)steps_of(a, b)) * items;
       if (u < at + n) break;
       at += n;
     }
-    found[0] = b;
-    scan[PA_WARPS] = at;
+    found = b;
+    seq_start = at;
   }
   __syncthreads();
-  int b = found[0];
-  long long seq0 = scan[PA_WARPS];             // first step of sequence b in the row
+  int b = found;
+  long long seq0 = seq_start;                  // first step (share) of sequence b in the row
 
   AttnWarp<D, T, NT> x;
   uint8_t* my_ring = ring + warp * C::STAGES * C::STAGE;
@@ -414,9 +448,12 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
   bool alive = true;                           // no wait of this warp has run out
 
   while (u < end) {
-    const int n = tokens_of(a, b), steps = (n + PA_STEP - 1) / PA_STEP;
-    if (u >= seq0 + (long long)steps * items) { seq0 += (long long)steps * items; ++b; continue; }
-    const int item = (int)((u - seq0) / steps), from = (int)((u - seq0) % steps), to = (int)min((long long)steps, from + (end - u));
+    const int n = tokens_of(a, b), steps = (n + PA_STEP - 1) / PA_STEP, row = few ? (int)((steps + share - 1) / share) : steps;   // of an item
+    if (u >= seq0 + (long long)row * items) { seq0 += (long long)row * items; ++b; continue; }
+    const int item = (int)((u - seq0) / row), at = (int)((u - seq0) % row);
+    const int from = few ? (int)(at * share) : at, to = (int)min((long long)steps, from + (few ? share : end - u));
+    const long long item0 = seq0 + (long long)item * row;
+    const int c0 = (int)(item0 / unit), parts = (int)((item0 + row - 1) / unit) - c0 + 1;       // blocks that share the item
     const int hk = item / a.groups, first = (item % a.groups) * HEADS, real = min(HEADS, a.ratio - first);
     const int head0 = hk * a.ratio + first;
     x.load_queries(a, a.q + b * a.qb + head0 * a.qh, real);
@@ -483,9 +520,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
     __syncthreads();
     x.leave(os + warp * HEADS * D, stats[warp]);
     __syncthreads();
-    const long long item0 = seq0 + (long long)item * steps;
-    const bool whole = from == 0 && to == steps;
-    const int c0 = (int)(item0 / share), c1 = (int)((item0 + steps - 1) / share);
+    const bool whole = parts == 1;
     float* slot = whole ? nullptr : a.ws + ((long long)blockIdx.x * 2 + (c0 == (int)blockIdx.x)) * C::SLOT;
     __nv_bfloat16* out = a.out + ((long long)b * a.Hq + head0) * D;
     for (int i = threadIdx.x; i < (whole ? real : HEADS) * D / 4; i += THREADS) {
@@ -516,7 +551,6 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
     if (!whole) {
       __threadfence();
       __syncthreads();
-      const int parts = c1 - c0 + 1;
       if (threadIdx.x == 0) {
         arrived = atomicAdd(a.counters + c0, 1);
         if (arrived == parts - 1) a.counters[c0] = 0;
@@ -524,30 +558,47 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
       }
       __syncthreads();
       if (arrived == parts - 1) {
-        // all parts are there: joined in the order of the blocks.  The first block holds its part in its second slot.
+        // All parts are there: joined in the order of the blocks (the first one holds its part in its second slot).  First a warp per
+        // head finds the largest m and M and leaves each part's factor in the ring, then every thread takes four channels.
         auto part = [&](int k) -> const float* { return a.ws + ((long long)(c0 + k) * 2 + (k == 0)) * C::SLOT; };
+        float* factors = os;                   // [head][parts]
+        for (int head = warp; head < real; head += PA_WARPS) {
+          float mm = -INFINITY, MM = -INFINITY, sum = 0.f;
+          for (int k = lane; k < parts; k += 32) {
+            const float* p = part(k) + HEADS * D + head;
+            mm = fmaxf(mm, __ldcg(p));
+            MM = fmaxf(MM, __ldcg(p + 2 * HEADS));
+          }
+          #pragma unroll
+          for (int d = 16; d > 0; d >>= 1) {
+            mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+            MM = fmaxf(MM, __shfl_xor_sync(0xffffffffu, MM, d));
+          }
+          for (int k = lane; k < parts; k += 32) {
+            const float* p = part(k) + HEADS * D + head;
+            sum += __ldcg(p + HEADS) * part_factor(__ldcg(p), mm);
+            factors[head * parts + k] = part_factor(__ldcg(p + 2 * HEADS), MM);
+          }
+          #pragma unroll
+          for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+          if (lane == 0) stats[0][head] = out_factor(mm, MM, sum);
+        }
+        __syncthreads();
         for (int i = threadIdx.x; i < real * D / 4; i += THREADS) {
           const int head = i * 4 / D;
-          float mm = -INFINITY, MM = -INFINITY, sum = 0.f;
-          for (int k = 0; k < parts; ++k) {
-            mm = fmaxf(mm, __ldcg(part(k) + HEADS * D + head));
-            MM = fmaxf(MM, __ldcg(part(k) + HEADS * D + 2 * HEADS + head));
-          }
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          #pragma unroll 4
+          #pragma unroll 8
           for (int k = 0; k < parts; ++k) {
-            const float* p = part(k);
-            sum += __ldcg(p + HEADS * D + HEADS + head) * part_factor(__ldcg(p + HEADS * D + head), mm);
-            const float f = part_factor(__ldcg(p + HEADS * D + 2 * HEADS + head), MM);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p) + i);
+            const float f = factors[head * parts + k];
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(part(k)) + i);
             acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
           }
-          const float f = out_factor(mm, MM, sum);
+          const float f = stats[0][head];
           reinterpret_cast<uint2*>(out)[i] = make_uint2(pack_bf16(acc.x * f, acc.y * f), pack_bf16(acc.z * f, acc.w * f));
         }
       }
     }
-    u += to - from;
+    u += few ? 1 : to - from;
     fence_proxy_async_smem();
     __syncthreads();                           // the ring, for TMA to write, and the statistics are free again
   }
@@ -577,7 +628,7 @@ static void paged_attn_shape(int* blocks, int* slot) {
   *slot = PagedAttn<D, T, NT>::SLOT;
 }
 // blocks of the launch, and floats of its workspace
-static int paged_attn_plan(int type, int width, int page_size, int B, int Hq, int Hk, int D, int* grid, long long* floats) {
+static int paged_attn_plan(int type, int width, int page_size, int B, int Hq, int Hk, int D, int* grid, int* most_blocks, long long* floats) {
   int blocks = 0, slot = 0, sms = 0, dev = 0;
   const int ratio = Hq / Hk;
   const bool two = two_tiles(ratio, D);
@@ -590,11 +641,12 @@ static int paged_attn_plan(int type, int width, int page_size, int B, int Hq, in
   #undef SHAPE
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return (int)cudaGetLastError();
   const int group = two ? 16 : 8;
-  // no more blocks than shares of two steps per warp
+  // no more blocks than there can be shares
   const long long most = (long long)B * Hk * ((ratio + group - 1) / group) * (((long long)width * page_size + PA_STEP - 1) / PA_STEP);
-  const long long shares = (most + 2 * PA_WARPS - 1) / (2 * PA_WARPS);
+  const long long shares = (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE + (long long)B * Hk * ((ratio + group - 1) / group);
   long long n = (long long)sms * blocks;
   if (n > PA_COUNTERS) n = PA_COUNTERS;
+  *most_blocks = (int)n;
   if (n > shares) n = shares;
   *grid = n < 1 ? 1 : (int)n;
   *floats = (long long)*grid * 2 * slot;
@@ -607,10 +659,10 @@ using namespace ssm;
 
 // floats of the workspace that ssm_paged_attn wants for these sizes on the current device; negative: an error
 extern "C" long long ssm_paged_attn_workspace(int type, int width, int page_size, int B, int Hq, int Hk, int D) {
-  int grid = 0;
+  int grid = 0, most = 0;
   long long floats = 0;
   if (Hk < 1 || Hq < Hk || Hq % Hk || B < 1) return -SSM_ERR_BAD_ARG;
-  const int e = paged_attn_plan(type, width, page_size, B, Hq, Hk, D, &grid, &floats);
+  const int e = paged_attn_plan(type, width, page_size, B, Hq, Hk, D, &grid, &most, &floats);
   return e ? (e < 0 ? e : -e) : floats;
 }
 
@@ -624,7 +676,7 @@ extern "C" int ssm_paged_attn(const void* q, long long qb, long long qh, void* o
   if (pages < 1 || (long long)pages * Hk * page_size > 0x7fffffffll || !kv_aligned(ks) || !kv_aligned(vs)) return -SSM_ERR_BAD_ARG;
   int grid = 0;
   long long floats = 0;
-  if (int e = paged_attn_plan(type, width, page_size, B, Hq, Hk, D, &grid, &floats)) return e;
+  if (int e = paged_attn_plan(type, width, page_size, B, Hq, Hk, D, &grid, &a.most_blocks, &floats)) return e;
   if (ws_floats < floats) return -SSM_ERR_BAD_ARG;
   a.q = reinterpret_cast<const __nv_bfloat16*>(q);
   a.out = reinterpret_cast<__nv_bfloat16*>(out);
