@@ -24,10 +24,11 @@
 
 namespace ssm {
 
-constexpr int PA_WARPS = 4, PA_STEP = 16, PA_COUNTERS = 768;
+constexpr int PA_WARPS = 4, PA_BOX = 16, PA_COUNTERS = 768;      // PA_BOX: tokens of a box
 constexpr int PA_MIN_SHARE = 2 * PA_WARPS;     // steps: two per warp
 constexpr int FEW_ITEMS = 8;                   // blocks per item, see the kernel
-constexpr float PA_GROWTH = 8.f;               // a running maximum moves when scores pass it by 2^8: fp16 and bf16 hold the larger shares as well
+// A running maximum moves when scores pass it by 2^8: bf16 and fp16 hold larger shares as well.
+constexpr float PA_GROWTH = 8.f, PA_SHARE = 256.f;
 
 struct AttnArgs {
   const __nv_bfloat16* q; __nv_bfloat16* out;
@@ -43,18 +44,21 @@ struct AttnArgs {
 template <int D, int T, int NT>
 struct PagedAttn {
   static constexpr int BYTES = KvType<T>::BYTES, ROW = D * BYTES, HEADS = 8 * NT;
+  static constexpr int SUB = ROW <= 128 ? 2 : 1, STEP = PA_BOX * SUB;         // boxes and tokens of a warp's step: 4 KB of keys and values or more
   static constexpr int TILE = ROW >= 128 ? 128 : 64, TILES = ROW / TILE;      // bytes of a box's rows (and of its swizzle), boxes of a row
   static constexpr int KCH = ROW / 64;                         // 16-byte pieces of a key row per lane (four lanes share a row)
   static constexpr int VB = TILE / 8, VEL = VB / BYTES;        // bytes and values of a lane's piece of a value row's tile (eight lanes share it)
-  static constexpr int K_BYTES = PA_STEP * ROW;
-  static constexpr int STAGE = 2 * K_BYTES;                    // of one warp: keys, values
-  static constexpr int LOADED = STAGE + (T == KV_BF16 ? 0 : 2 * PA_STEP * 4);  // with the scales
-  static constexpr int STAGES = STAGE > 2048 ? 3 : 6;
+  static constexpr int BOX = PA_BOX * ROW;                     // bytes of a box's keys, or values
+  static constexpr int STAGE = SUB * 2 * BOX;                  // of one warp: keys and values of each box
+  static constexpr int LOADED = 2 * BOX + (T == KV_BF16 ? 0 : 2 * PA_BOX * 4); // of one box, with the scales
+  static constexpr int STAGES = 3;
   static constexpr int RING = PA_WARPS * STAGES * STAGE;
   static constexpr int SMEM = RING + 1024;                     // boxes begin on 1024 bytes
-  static constexpr int BLOCKS = SMEM > 113 * 1024 ? 1 : SMEM > 55 * 1024 ? 2 : NT == 1 ? 4 : 3;      // per SM
-  static constexpr int SLOT = HEADS * D + 3 * HEADS;           // floats of a part: o, m, sum, M
-  static_assert(PA_WARPS * HEADS * D * 4 <= RING && PA_COUNTERS * HEADS * 4 <= RING, "the warps' results, and factors of parts, meet in the ring");
+  // per SM: as many as 96 KB, or more than one, of loads under way ask for, and registers leave
+  static constexpr int BLOCKS = SMEM > 113 * 1024 ? 1 : SMEM > 73 * 1024 || NT == 2 ? 2 : 3;
+  static constexpr int SLOT = HEADS * D + 3 * HEADS;           // floats of a part: o [channel][head], m, sum, M
+  static constexpr int MEET = D * HEADS + D / VEL * 8;         // floats of a warp's o where the warps meet, see leave()
+  static_assert(PA_WARPS * MEET * 4 <= RING && PA_COUNTERS * HEADS * 4 <= RING, "the warps' results meet in the ring");
 };
 
 // Token of row g of S^T (and of row g + 8, eight further), and 16-byte piece of a 128-byte row of V that lane group g takes: 0 4 1 5
@@ -96,12 +100,10 @@ __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
     hi = *reinterpret_cast<const uint32_t*>(&y);
   }
 }
-__device__ __forceinline__ float zero_if_inf(float m) { return m == -INFINITY ? 0.f : m; }
 // 2^(m - to), 0 for a part without tokens
 __device__ __forceinline__ float part_factor(float m, float to) { return m == -INFINITY ? 0.f : exp2f(m - to); }
-
-// what an unnormalised result is multiplied with; 0 where there are no tokens or all values are zeros
-__device__ __forceinline__ float out_factor(float m, float M, float sum) { return sum == 0.f || M == -INFINITY ? 0.f : exp2f(M - m) / sum; }
+// what an unnormalised result is multiplied with; 0 where there are no tokens
+__device__ __forceinline__ float out_factor(float m, float M, float sum) { return sum == 0.f ? 0.f : exp2f(M - m) / sum; }
 
 // tokens of sequence b: not below 0, not beyond its pages
 __device__ __forceinline__ int tokens_of(const AttnArgs& a, int b) {
@@ -111,36 +113,11 @@ __device__ __forceinline__ int tokens_of(const AttnArgs& a, int b) {
   report_bad_index(a.table.status);
   return (int)room;
 }
-__device__ __forceinline__ int steps_of(const AttnArgs& a, int b) { return (tokens_of(a, b) + PA_STEP - 1) / PA_STEP; }
-
-// inclusive sum over the block's threads, and of all
-template <int WARPS>
-__device__ __forceinline__ void block_scan(long long& upto, long long& total, long long* sums) {
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, upto, d);
-    if (lane >= d) upto += v;
-  }
-  __syncthreads();
-  if (lane == 31) sums[warp] = upto;
-  __syncthreads();
-  total = 0;
-  #pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) upto += sums[w];
-    total += sums[w];
-  }
-}
-template <int WARPS>
-__device__ __forceinline__ int block_count(int n, int* sums) {
-  n = __reduce_add_sync(0xffffffffu, n);
-  if ((threadIdx.x & 31) == 0) sums[threadIdx.x / 32] = n;
-  __syncthreads();
-  int all = 0;
-  #pragma unroll
-  for (int w = 0; w < WARPS; ++w) all += sums[w];
-  return all;
+// adds one to a counter; what the block wrote before its barrier is visible to whoever sees the sum, and the other way round
+__device__ __forceinline__ int arrive(int* counter) {
+  int before;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+  return before;
 }
 
 template <int D, int T, int NT>
@@ -149,7 +126,10 @@ struct AttnWarp {
   static constexpr bool F16 = T != KV_BF16;
   uint32_t qf[NT][D / 8];                      // Q^T fragments; [D / 32 or D / 64 blocks of channels][4 or 8 words]
   float qs[NT][2];                             // what a sum of products of column 2c, 2c + 1 is multiplied with
-  float o[NT][D / 16][4], m[NT][2], l[NT][2], M[NT][2];
+  // Relative to the running maximum m, sums of 2^(s' - m); o relative to M, which is m for 16-bit values.  With 8 bits o sums
+  // 2^(s' - M) times the value's scale: G = 2^(m - M), and M is at least m - 120, so that G is an fp32 number.
+  float o[NT][D / 16][4], m[NT][2], l[NT][2], M[NT][2], G[NT][2];
+  bool fresh;                                  // no tokens yet
 
   // queries of heads first .. first + HEADS - 1 of a key head; `real` of them exist
   __device__ __forceinline__ void load_queries(const AttnArgs& a, const __nv_bfloat16* q, int real) {
@@ -200,174 +180,242 @@ struct AttnWarp {
     for (int nt = 0; nt < NT; ++nt) {
       #pragma unroll
       for (int t = 0; t < D / 16; ++t) o[nt][t][0] = o[nt][t][1] = o[nt][t][2] = o[nt][t][3] = 0.f;
-      m[nt][0] = m[nt][1] = M[nt][0] = M[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
+      #pragma unroll
+      for (int j = 0; j < 2; ++j) { m[nt][j] = l[nt][j] = M[nt][j] = 0.f; G[nt][j] = 1.f; }
     }
+    fresh = true;
   }
 
-  // 16 tokens, of which the first `valid` count, from this warp's stage of the ring
+  // largest of a lane's tokens and of the lanes with the same columns
+  __device__ __forceinline__ float column_max(float x) {
+    #pragma unroll
+    for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    return x;
+  }
+  __device__ __forceinline__ void scale_o(int nt, int j, float f) {
+    #pragma unroll
+    for (int t = 0; t < D / 16; ++t) { o[nt][t][j] *= f; o[nt][t][j + 2] *= f; }
+  }
+
+  // The boxes of a stage of this warp's ring; the first `valid & 255` tokens of the first box count, and so on for the second.
   __device__ __forceinline__ void step(const uint8_t* stage, const float* scales, int valid) {
+    constexpr int SUB = C::SUB, FULL = SUB == 2 ? PA_BOX | PA_BOX << 8 : PA_BOX;
     const int g = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3, tok = sigma<C::TILE>(g);
-    float s[NT][4], s2[NT][4];
+    float s[SUB][NT][4];
     #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int u = 0; u < SUB; ++u) {
       #pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] = s2[nt][i] = 0.f;
-    }
-    #pragma unroll
-    for (int i = 0; i < C::KCH; ++i) {
-      // piece c or 4 + c of the tile's row
-      const int at = C::TILE == 128 ? (i >> 1) * PA_STEP * 128 + tok * 128 + ((((i & 1) * 4 + c) ^ tok) << 4) : tok * 64 + ((c ^ ((tok >> 1) & 3)) << 4);
-      const uint4 u = *reinterpret_cast<const uint4*>(stage + at);
-      const uint4 v = *reinterpret_cast<const uint4*>(stage + at + 8 * C::TILE);
-      const uint32_t a[4] = {u.x, u.y, u.z, u.w}, b[4] = {v.x, v.y, v.z, v.w};
-      if (!F16) {
-        #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma16816<false>(s[nt], a[0], b[0], a[1], b[1], qf[nt][i * 4], qf[nt][i * 4 + 1]);
-          mma16816<false>(s2[nt], a[2], b[2], a[3], b[3], qf[nt][i * 4 + 2], qf[nt][i * 4 + 3]);
-        }
-      } else {
-        #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t a0, a1, b0, b1;
-          widen4<T>(a[j], a0, a1);
-          widen4<T>(b[j], b0, b1);
+      for (int nt = 0; nt < NT; ++nt) s[u][nt][0] = s[u][nt][1] = s[u][nt][2] = s[u][nt][3] = 0.f;
+      #pragma unroll
+      for (int i = 0; i < C::KCH; ++i) {
+        // piece c or 4 + c of the tile's row
+        const int at = C::TILE == 128 ? (i >> 1) * PA_BOX * 128 + tok * 128 + ((((i & 1) * 4 + c) ^ tok) << 4) : tok * 64 + ((c ^ ((tok >> 1) & 3)) << 4);
+        const uint4 x = *reinterpret_cast<const uint4*>(stage + u * 2 * C::BOX + at);
+        const uint4 y = *reinterpret_cast<const uint4*>(stage + u * 2 * C::BOX + at + 8 * C::TILE);
+        const uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
+        if (!F16) {
           #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma16816<true>(j & 1 ? s2[nt] : s[nt], a0, b0, a1, b1, qf[nt][i * 8 + j * 2], qf[nt][i * 8 + j * 2 + 1]);
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816<false>(s[u][nt], a[0], b[0], a[1], b[1], qf[nt][i * 4], qf[nt][i * 4 + 1]);
+            mma16816<false>(s[u][nt], a[2], b[2], a[3], b[3], qf[nt][i * 4 + 2], qf[nt][i * 4 + 3]);
+          }
+        } else {
+          #pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t a0, a1, b0, b1;
+            widen4<T>(a[j], a0, a1);
+            widen4<T>(b[j], b0, b1);
+            #pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<true>(s[u][nt], a0, b0, a1, b1, qf[nt][i * 8 + j * 2], qf[nt][i * 8 + j * 2 + 1]);
+          }
         }
       }
     }
-    // lane (g, c): tokens tok and tok + 8, heads 2c and 2c + 1 of each tile
-    float ks[2], lv[2], vn[2];                  // scales of the keys; a value's scale is vn 2^lv
-    if (F16) {
-      #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        ks[i] = scales[tok + 8 * i];
-        const float vs = scales[PA_STEP + tok + 8 * i];
-        const uint32_t bits = __float_as_uint(vs), e = (bits >> 23) & 255;
-        const bool none = e == 0 || tok + 8 * i >= valid;
-        lv[i] = none ? -INFINITY : (float)((int)e - 126);
-        vn[i] = none ? 0.f : e == 255 ? vs : __uint_as_float((bits & 0x807fffffu) | (126u << 23));
-      }
-    }
+    // lane (g, c): tokens tok and tok + 8 of each box, heads 2c and 2c + 1 of each tile: s' - m
+    float vs[SUB][2];                           // scales of the values
     bool grows = false;
     #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int u = 0; u < SUB; ++u) {
+      float ks[2] = {1.f, 1.f};
+      if (F16) {
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          ks[i] = scales[u * 2 * PA_BOX + tok + 8 * i];
+          vs[u][i] = scales[u * 2 * PA_BOX + PA_BOX + tok + 8 * i];
+        }
+      }
       #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = (s[nt][i] + s2[nt][i]) * qs[nt][i & 1];
-        if (F16) x *= ks[i >> 1];
-        if (tok + (i >> 1) * 8 >= valid) x = -INFINITY;
-        s[nt][i] = x;
-        grows |= x > m[nt][i & 1] + PA_GROWTH;
-        if (F16) grows |= x + lv[i >> 1] > M[nt][i & 1] + PA_GROWTH;
+      for (int nt = 0; nt < NT; ++nt) {
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) s[u][nt][i] = fmaf(s[u][nt][i], F16 ? qs[nt][i & 1] * ks[i >> 1] : qs[nt][i & 1], -m[nt][i & 1]);
       }
     }
-    if (__any_sync(0xffffffffu, grows)) {
+    if (valid != FULL) {
+      #pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (tok + 8 * i < ((valid >> (8 * u)) & 255)) continue;
+          vs[u][i] = 0.f;
+          #pragma unroll
+          for (int nt = 0; nt < NT; ++nt) s[u][nt][2 * i] = s[u][nt][2 * i + 1] = -INFINITY;
+        }
+      }
+    }
+    #pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      #pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) grows |= s[u][nt][i] > PA_GROWTH;
+      }
+    }
+    const bool moves = __any_sync(0xffffffffu, grows) || fresh;
+    if (moves) {
       #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float x = fmaxf(s[nt][j], s[nt][j + 2]), y = F16 ? fmaxf(s[nt][j] + lv[0], s[nt][j + 2] + lv[1]) : 0.f;
+          float x = -INFINITY;
           #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) {
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-            if (F16) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
-          }
-          x = fmaxf(x, m[nt][j]);
-          const float f = part_factor(m[nt][j], x);
+          for (int u = 0; u < SUB; ++u) x = fmaxf(x, fmaxf(s[u][nt][j], s[u][nt][j + 2]));
+          x = column_max(x);
+          if (!fresh) x = fmaxf(x, 0.f);
+          if (x == -INFINITY) x = 0.f;
+          const float f = fresh ? 1.f : exp2f(-x);
+          m[nt][j] += x;
           l[nt][j] *= f;
-          m[nt][j] = x;
-          float fo = f;
-          if (F16) {
-            y = fmaxf(y, M[nt][j]);
-            fo = part_factor(M[nt][j], y);
-            M[nt][j] = y;
+          if (!F16) scale_o(nt, j, f);
+          #pragma unroll
+          for (int u = 0; u < SUB; ++u) { s[u][nt][j] -= x; s[u][nt][j + 2] -= x; }
+        }
+      }
+    }
+    uint32_t p[SUB][NT][2];
+    bool large = false;
+    #pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      #pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = exp2f(s[u][nt][i]);
+          l[nt][i & 1] += e;
+          s[u][nt][i] = e;
+          if (F16) large |= e * (vs[u][i >> 1] * G[nt][i & 1]) > PA_SHARE;
+        }
+      }
+    }
+    if (F16) {
+      if (__any_sync(0xffffffffu, large) || moves) {
+        #pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          #pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float x = -120.f;                   // above the logarithms of all shares: 2^e > scale
+            #pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+              #pragma unroll
+              for (int i = 0; i < 2; ++i) x = fmaxf(x, log2f(s[u][nt][2 * i + j]) + (float)(int)((__float_as_uint(vs[u][i]) >> 23) & 255) - 126.f);
+            }
+            x = column_max(x) + m[nt][j];
+            if (!fresh) {
+              x = fmaxf(x, M[nt][j]);
+              scale_o(nt, j, exp2f(M[nt][j] - x));
+            }
+            M[nt][j] = x;
+            G[nt][j] = exp2f(m[nt][j] - x);
           }
-          #pragma unroll
-          for (int t = 0; t < D / 16; ++t) { o[nt][t][j] *= fo; o[nt][t][j + 2] *= fo; }
         }
       }
     }
-    uint32_t p[NT][2];
     #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float w[4];
+    for (int u = 0; u < SUB; ++u) {
       #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = exp2f(s[nt][i] - zero_if_inf(m[nt][i & 1]));
-        l[nt][i & 1] += w[i];
-        if (F16) w[i] = exp2f(s[nt][i] + lv[i >> 1] - zero_if_inf(M[nt][i & 1])) * vn[i >> 1];
+      for (int nt = 0; nt < NT; ++nt) {
+        float w[4];
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = F16 ? s[u][nt][i] * (vs[u][i >> 1] * G[nt][i & 1]) : s[u][nt][i];
+        p[u][nt][0] = transpose8x8(F16 ? pack_f16(w[0], w[1]) : pack_bf16(w[0], w[1]));
+        p[u][nt][1] = transpose8x8(F16 ? pack_f16(w[2], w[3]) : pack_bf16(w[2], w[3]));
       }
-      p[nt][0] = transpose8x8(F16 ? pack_f16(w[0], w[1]) : pack_bf16(w[0], w[1]));
-      p[nt][1] = transpose8x8(F16 ? pack_f16(w[2], w[3]) : pack_bf16(w[2], w[3]));
     }
-    const uint8_t* vst = stage + C::K_BYTES;
+    fresh = false;
     #pragma unroll
-    for (int k = 0; k < C::TILES; ++k) {
-      // this lane's channels of the tokens that are P^T's rows 2c, 2c + 1, 2c + 8, 2c + 9
-      uint32_t x[4][C::VB / 4];
+    for (int u = 0; u < SUB; ++u) {
+      const uint8_t* vst = stage + u * 2 * C::BOX + C::BOX;
       #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = (C::TILE == 128 ? c + 4 * (i & 1) : 2 * c + (i & 1)) + 8 * (i >> 1);
-        const uint8_t* src = vst + k * PA_STEP * C::TILE + row * C::TILE;
-        if (C::TILE == 128) {
-          const uint4 u = *reinterpret_cast<const uint4*>(src + ((sigma<128>(g) ^ (row & 7)) << 4));
-          x[i][0] = u.x; x[i][1] = u.y; x[i][2 % (C::VB / 4)] = u.z; x[i][3 % (C::VB / 4)] = u.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(src + (((g >> 1) ^ c) << 4) + (g & 1) * 8);
-          x[i][0] = u.x; x[i][1] = u.y;
+      for (int k = 0; k < C::TILES; ++k) {
+        // this lane's channels of the tokens that are P^T's rows 2c, 2c + 1, 2c + 8, 2c + 9
+        uint32_t x[4][C::VB / 4];
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = (C::TILE == 128 ? c + 4 * (i & 1) : 2 * c + (i & 1)) + 8 * (i >> 1);
+          const uint8_t* src = vst + k * PA_BOX * C::TILE + row * C::TILE;
+          if (C::TILE == 128) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src + ((sigma<128>(g) ^ (row & 7)) << 4));
+            x[i][0] = v.x; x[i][1] = v.y; x[i][2 % (C::VB / 4)] = v.z; x[i][3 % (C::VB / 4)] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(src + (((g >> 1) ^ c) << 4) + (g & 1) * 8);
+            x[i][0] = v.x; x[i][1] = v.y;
+          }
         }
-        if (valid < PA_STEP && row >= valid) {  // what lies behind a sequence may be NaN, which no zero share takes away
+        if (valid != FULL) {                    // what lies behind a sequence may be NaN, which no zero share takes away
           #pragma unroll
-          for (int t = 0; t < C::VB / 4; ++t) x[i][t] = 0;
+          for (int i = 0; i < 4; ++i) {
+            const int row = (C::TILE == 128 ? c + 4 * (i & 1) : 2 * c + (i & 1)) + 8 * (i >> 1);
+            if (row < ((valid >> (8 * u)) & 255)) continue;
+            #pragma unroll
+            for (int t = 0; t < C::VB / 4; ++t) x[i][t] = 0;
+          }
         }
-      }
-      #pragma unroll
-      for (int t = 0; t < C::VB / 4; ++t) {
-        if (!F16) {
-          const uint32_t a0 = __byte_perm(x[0][t], x[1][t], 0x5410), a1 = __byte_perm(x[0][t], x[1][t], 0x7632);
-          const uint32_t a2 = __byte_perm(x[2][t], x[3][t], 0x5410), a3 = __byte_perm(x[2][t], x[3][t], 0x7632);
-          #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[nt][k * (C::VEL / 2) + t], a0, a1, a2, a3, p[nt][0], p[nt][1]);
-        } else {
-          uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
-          widen4<T>(__byte_perm(x[0][t], x[1][t], 0x5140), a0, a1);
-          widen4<T>(__byte_perm(x[2][t], x[3][t], 0x5140), a2, a3);
-          widen4<T>(__byte_perm(x[0][t], x[1][t], 0x7362), b0, b1);
-          widen4<T>(__byte_perm(x[2][t], x[3][t], 0x7362), b2, b3);
-          #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma16816<true>(o[nt][k * (C::VEL / 2) + 2 * t], a0, a1, a2, a3, p[nt][0], p[nt][1]);
-            mma16816<true>(o[nt][k * (C::VEL / 2) + 2 * t + 1], b0, b1, b2, b3, p[nt][0], p[nt][1]);
+        #pragma unroll
+        for (int t = 0; t < C::VB / 4; ++t) {
+          if (!F16) {
+            const uint32_t a0 = __byte_perm(x[0][t], x[1][t], 0x5410), a1 = __byte_perm(x[0][t], x[1][t], 0x7632);
+            const uint32_t a2 = __byte_perm(x[2][t], x[3][t], 0x5410), a3 = __byte_perm(x[2][t], x[3][t], 0x7632);
+            #pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[nt][k * (C::VEL / 2) + t], a0, a1, a2, a3, p[u][nt][0], p[u][nt][1]);
+          } else {
+            uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
+            widen4<T>(__byte_perm(x[0][t], x[1][t], 0x5140), a0, a1);
+            widen4<T>(__byte_perm(x[2][t], x[3][t], 0x5140), a2, a3);
+            widen4<T>(__byte_perm(x[0][t], x[1][t], 0x7362), b0, b1);
+            widen4<T>(__byte_perm(x[2][t], x[3][t], 0x7362), b2, b3);
+            #pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<true>(o[nt][k * (C::VEL / 2) + 2 * t], a0, a1, a2, a3, p[u][nt][0], p[u][nt][1]);
+              mma16816<true>(o[nt][k * (C::VEL / 2) + 2 * t + 1], b0, b1, b2, b3, p[u][nt][0], p[u][nt][1]);
+            }
           }
         }
       }
     }
   }
 
-  // o[head][channel] into `to`; lanes with g == 0 put (m, sum, M) of their heads into `stats`
+  // o into `to`, [channel][head] with 8 floats between the pieces of neighbouring lane groups (their banks would be the same);
+  // lanes with g == 0 put (m, sum, M) of their heads into `stats`
   __device__ __forceinline__ void leave(float* to, float* stats) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      const int head = nt * 8 + 2 * c;
+      #pragma unroll
+      for (int t = 0; t < D / 16; ++t) {
+        const int piece = t / (C::VEL / 2) * 8 + sigma<C::TILE>(g), e = t % (C::VEL / 2);
+        float* at = to + piece * (C::VEL * C::HEADS + 8) + 2 * e * C::HEADS + head;
+        *reinterpret_cast<float2*>(at) = make_float2(o[nt][t][0], o[nt][t][1]);
+        *reinterpret_cast<float2*>(at + C::HEADS) = make_float2(o[nt][t][2], o[nt][t][3]);
+      }
       #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int head = nt * 8 + 2 * c + j;
-        #pragma unroll
-        for (int t = 0; t < D / 16; ++t) {
-          const int k = t / (C::VEL / 2), e = t % (C::VEL / 2);
-          *reinterpret_cast<float2*>(to + head * D + k * 8 * C::VEL + sigma<C::TILE>(g) * C::VEL + 2 * e) = make_float2(o[nt][t][j], o[nt][t][j + 2]);
-        }
         float sum = l[nt][j];
         #pragma unroll
         for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (g == 0) {
-          stats[head] = m[nt][j];
-          stats[C::HEADS + head] = sum;
-          stats[2 * C::HEADS + head] = F16 ? M[nt][j] : m[nt][j];
+          stats[head + j] = fresh ? -INFINITY : m[nt][j];
+          stats[C::HEADS + head + j] = sum;
+          stats[2 * C::HEADS + head + j] = fresh ? -INFINITY : F16 ? M[nt][j] : m[nt][j];
         }
       }
     }
@@ -378,125 +426,146 @@ template <int D, int T, int NT>
 __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) paged_attn_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                                                                                             const __grid_constant__ CUtensorMap vmap) {
   using C = PagedAttn<D, T, NT>;
-  constexpr int HEADS = C::HEADS, THREADS = PA_WARPS * 32;
+  constexpr int HEADS = C::HEADS, THREADS = PA_WARPS * 32, SUB = C::SUB, PER = 32 / SUB;       // PER: steps whose pages a warp's lanes hold
   extern __shared__ uint8_t dynamic[];
   uint8_t* ring = dynamic + (1024 - (smem_u32(dynamic) & 1023)) % 1024;
-  __shared__ __align__(16) float scales[T == KV_BF16 ? 1 : PA_WARPS * C::STAGES][2 * PA_STEP];
+  __shared__ __align__(16) float scales[T == KV_BF16 ? 1 : PA_WARPS * C::STAGES][SUB * 2 * PA_BOX];
   __shared__ uint64_t full[PA_WARPS][C::STAGES];
-  __shared__ float stats[PA_WARPS][3 * HEADS];
-  __shared__ long long scan[PA_WARPS], seq_start;
-  __shared__ int counts[PA_WARPS], found, arrived;
+  __shared__ __align__(16) float stats[PA_WARPS][3 * HEADS];
+  __shared__ int arrived;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int items = a.Hk * a.groups;
-
   if (lane == 0) {
     #pragma unroll
     for (int i = 0; i < C::STAGES; ++i) mbar_init(&full[warp][i], 1);
     mbar_fence_init();
   }
-  // sequences without tokens
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-    if (a.table.lengths[b] > 0 && a.table.width > 0) continue;
-    for (int i = threadIdx.x; i < a.Hq * D / 8; i += THREADS) reinterpret_cast<uint4*>(a.out + (long long)b * a.Hq * D)[i] = make_uint4(0, 0, 0, 0);
-  }
+  __syncwarp();
 
-  // Where this block's share begins.  The steps of all sequences and heads stand in a row, each sequence's heads one behind the other.
+  // Where this block's share begins.  The steps of all sequences and heads stand in a row, each sequence's heads one behind the other;
+  // sequences in the order lane, lane + 32, ... of the lanes that look at them (every warp finds the same).
   // Many of them (items): blocks cut the row at equal distances, wherever that is.  Few: every item is cut by itself, so that no
   // block has parts of two, at the price of up to one shorter share per item.
-  const int per = (a.B + THREADS - 1) / THREADS, b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
-  long long mine = 0;
-  int some = 0;
-  for (int b = b0; b < b1; ++b) { const int n = steps_of(a, b); mine += (long long)n * items; some += n > 0; }
-  long long upto = mine, total;
-  block_scan<PA_WARPS>(upto, total, scan);
-  const long long used = (long long)block_count<PA_WARPS>(some, counts) * items;     // items with steps
-  const bool few = used * FEW_ITEMS <= a.most_blocks;
-  long long share = (total + gridDim.x - 1) / gridDim.x;
-  if (few) share = (total + a.most_blocks - used - 1) / (a.most_blocks - used);       // at most most_blocks in all
-  share = max((long long)PA_MIN_SHARE, (share + PA_WARPS - 1) / PA_WARPS * PA_WARPS);
+  auto steps_of = [&](int b) -> int { return (tokens_of(a, b) + C::STEP - 1) / C::STEP; };
+  const int first_steps = lane < a.B ? steps_of(lane) : 0;
+  int mine = first_steps * items, some = first_steps > 0;
+  for (int b = lane + 32; b < a.B; b += 32) { const int n = steps_of(b); mine += n * items; some += n > 0; }
+  int upto = mine;
+  #pragma unroll
+  for (int d = 1; d < 32; d <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += v; }
+  int total = __shfl_sync(0xffffffffu, upto, 31);
+  const int filled = __reduce_add_sync(0xffffffffu, some);
+  if (filled < a.B) {
+    // sequences without tokens
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      if (steps_of(b) > 0) continue;
+      for (int i = threadIdx.x; i < a.Hq * D / 8; i += THREADS) reinterpret_cast<uint4*>(a.out + (long long)b * a.Hq * D)[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  const bool few = (long long)filled * items * FEW_ITEMS <= a.most_blocks;
+  const int blocks = few ? a.most_blocks - filled * items : gridDim.x;         // few: at most most_blocks shares in all
+  const int share = max(PA_MIN_SHARE, ((total + blocks - 1) / blocks + PA_WARPS - 1) / PA_WARPS * PA_WARPS);
   if (few) {
     // counted in shares from here on
-    mine = 0;
-    for (int b = b0; b < b1; ++b) mine += (steps_of(a, b) + share - 1) / share * items;
+    mine = (first_steps + share - 1) / share * items;
+    for (int b = lane + 32; b < a.B; b += 32) mine += (steps_of(b) + share - 1) / share * items;
     upto = mine;
-    block_scan<PA_WARPS>(upto, total, scan);
+    #pragma unroll
+    for (int d = 1; d < 32; d <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += v; }
+    total = __shfl_sync(0xffffffffu, upto, 31);
   }
-  const long long unit = few ? 1 : share;       // of the row, per block
-  long long u = unit * blockIdx.x;
-  const long long end = min(total, u + unit), before = upto - mine;
-  if (u >= end) return;
-  if (before <= u && u < upto) {
-    long long at = before;
-    int b = b0;
-    for (;; ++b) {
-      const long long n = (few ? (steps_of(a, b) + share - 1) / share : (long long)steps_of(a, b)) * items;
-      if (u < at + n) break;
-      at += n;
+  const int unit = few ? 1 : share;            // of the row, per block
+  if ((long long)unit * blockIdx.x >= total) return;
+  int u = unit * blockIdx.x;
+  const int end = total - u < unit ? total : u + unit;
+  int b = lane, seq0 = upto - mine;            // first step (share) of sequence b in the row
+  const bool here = seq0 <= u && u < upto;
+  if (here) {
+    for (;;) {
+      const int n = (few ? (steps_of(b) + share - 1) / share : steps_of(b)) * items;
+      if (u < seq0 + n) break;
+      seq0 += n;
+      b += 32;
     }
-    found = b;
-    seq_start = at;
   }
-  __syncthreads();
-  int b = found;
-  long long seq0 = seq_start;                  // first step (share) of sequence b in the row
+  const int owner = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+  b = __shfl_sync(0xffffffffu, b, owner);
+  seq0 = __shfl_sync(0xffffffffu, seq0, owner);
 
   AttnWarp<D, T, NT> x;
   uint8_t* my_ring = ring + warp * C::STAGES * C::STAGE;
-  const int page_mask = (1 << a.table.page_shift) - 1, step_shift = a.table.page_shift - 4;
+  const int page_mask = (1 << a.table.page_shift) - 1;
   int put = 0, got = 0;                        // stages of the ring: next to fill, next to read
   uint32_t parity = 0;                         // of the next to read
   bool alive = true;                           // no wait of this warp has run out
 
   while (u < end) {
-    const int n = tokens_of(a, b), steps = (n + PA_STEP - 1) / PA_STEP, row = few ? (int)((steps + share - 1) / share) : steps;   // of an item
-    if (u >= seq0 + (long long)row * items) { seq0 += (long long)row * items; ++b; continue; }
-    const int item = (int)((u - seq0) / row), at = (int)((u - seq0) % row);
-    const int from = few ? (int)(at * share) : at, to = (int)min((long long)steps, from + (few ? share : end - u));
-    const long long item0 = seq0 + (long long)item * row;
-    const int c0 = (int)(item0 / unit), parts = (int)((item0 + row - 1) / unit) - c0 + 1;       // blocks that share the item
+    const int n = tokens_of(a, b), steps = (n + C::STEP - 1) / C::STEP, row = few ? (steps + share - 1) / share : steps;   // row: of an item
+    if (u >= seq0 + row * items) {
+      seq0 += row * items;
+      b += 32;
+      if (b >= a.B) b = (b & 31) + 1;
+      continue;
+    }
+    const int item = (u - seq0) / row, at = (u - seq0) % row;
+    const int from = few ? at * share : at, to = min(steps, from + (few ? share : end - u));
+    const int item0 = seq0 + item * row;
+    const int c0 = item0 / unit, parts = (item0 + row - 1) / unit - c0 + 1;    // blocks that share the item
     const int hk = item / a.groups, first = (item % a.groups) * HEADS, real = min(HEADS, a.ratio - first);
     const int head0 = hk * a.ratio + first;
-    x.load_queries(a, a.q + b * a.qb + head0 * a.qh, real);
-    x.reset();
 
     const int count = to - from > warp ? (to - from - warp + PA_WARPS - 1) / PA_WARPS : 0;      // steps of this warp: from + warp + 4 j
     const int* ids = a.table.ids + (long long)b * a.table.width;
     int id = -1, valid[C::STAGES - 1];
-    // starts the copies of step j; its tokens, 0 where it has no page
+    // starts the copies of step j; the tokens of its boxes (8 bits each), 0 where there is no page
     auto issue = [&](int j) -> int {
       if (j >= count) return 0;
-      if ((j & 31) == 0) {
-        // the pages of this warp's next 32 steps, one per lane
-        const int k = j + lane;
+      if (j % PER == 0) {
+        // the pages of the boxes of this warp's next steps, one per lane
+        const int k = j + lane / SUB, t = (from + warp + PA_WARPS * k) * C::STEP + lane % SUB * PA_BOX;
         id = -1;
-        if (k < count) {
-          id = ids[(from + warp + PA_WARPS * k) >> step_shift];
+        if (k < count && t < n) {
+          id = ids[t >> a.table.page_shift];
           if (id < 0 || id >= a.table.pages) { report_bad_index(a.table.status); id = -1; }
         }
       }
-      const int page = __shfl_sync(0xffffffffu, id, j & 31), t0 = (from + warp + PA_WARPS * j) * PA_STEP;
-      if (page < 0 || !alive) return 0;
+      int real_tokens = 0, boxes = 0, page[SUB];
+      const int t0 = (from + warp + PA_WARPS * j) * C::STEP;
+      #pragma unroll
+      for (int i = 0; i < SUB; ++i) {
+        page[i] = __shfl_sync(0xffffffffu, id, j % PER * SUB + i);
+        if (page[i] < 0) continue;
+        ++boxes;
+        real_tokens |= min(PA_BOX, n - t0 - i * PA_BOX) << (8 * i);
+      }
+      if (boxes == 0 || !alive) return 0;
       if (lane == 0) {
-        const long long slot = (((long long)page * a.Hk + hk) << a.table.page_shift) + (t0 & page_mask);     // below 2^31: the host sees to it
         uint64_t* bar = &full[warp][put];
-        uint8_t* dst = my_ring + put * C::STAGE;
-        mbar_expect_tx(bar, C::LOADED);
+        mbar_expect_tx(bar, boxes * C::LOADED);
         #pragma unroll
-        for (int i = 0; i < C::TILES; ++i) {
-          tma_load_2d(dst + i * PA_STEP * C::TILE, &kmap, i * C::TILE / C::BYTES, (int)slot, bar);
-          tma_load_2d(dst + C::K_BYTES + i * PA_STEP * C::TILE, &vmap, i * C::TILE / C::BYTES, (int)slot, bar);
-        }
-        if (T != KV_BF16) {
-          float* sc = scales[warp * C::STAGES + put];
-          bulk_load(sc, a.scales[0] + slot, PA_STEP * 4, bar);
-          bulk_load(sc + PA_STEP, a.scales[1] + slot, PA_STEP * 4, bar);
+        for (int i = 0; i < SUB; ++i) {
+          if (page[i] < 0) continue;
+          const int slot = ((page[i] * a.Hk + hk) << a.table.page_shift) + ((t0 + i * PA_BOX) & page_mask);      // below 2^31: the host sees to it
+          uint8_t* dst = my_ring + put * C::STAGE + i * 2 * C::BOX;
+          #pragma unroll
+          for (int k = 0; k < C::TILES; ++k) {
+            tma_load_2d(dst + k * PA_BOX * C::TILE, &kmap, k * C::TILE / C::BYTES, slot, bar);
+            tma_load_2d(dst + C::BOX + k * PA_BOX * C::TILE, &vmap, k * C::TILE / C::BYTES, slot, bar);
+          }
+          if (T != KV_BF16) {
+            float* sc = scales[warp * C::STAGES + put] + i * 2 * PA_BOX;
+            bulk_load(sc, a.scales[0] + slot, PA_BOX * 4, bar);
+            bulk_load(sc + PA_BOX, a.scales[1] + slot, PA_BOX * 4, bar);
+          }
         }
       }
       put = put + 1 == C::STAGES ? 0 : put + 1;
-      return min(PA_STEP, n - t0);
+      return real_tokens;
     };
     #pragma unroll
     for (int j = 0; j < C::STAGES - 1; ++j) valid[j] = issue(j);
+    x.load_queries(a, a.q + b * a.qb + head0 * a.qh, real);
+    x.reset();
     for (int j = 0; j < count; ++j) {
       const int now = valid[0];
       #pragma unroll
@@ -518,83 +587,134 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
     // the warps meet
     float* os = reinterpret_cast<float*>(ring);
     __syncthreads();
-    x.leave(os + warp * HEADS * D, stats[warp]);
+    x.leave(os + warp * C::MEET, stats[warp]);
     __syncthreads();
     const bool whole = parts == 1;
+    // threads take a channel of four heads at a time, always the same heads
+    const int fours = real <= 4 ? 1 : real <= 8 ? 2 : 4, h = threadIdx.x % fours * 4;
     float* slot = whole ? nullptr : a.ws + ((long long)blockIdx.x * 2 + (c0 == (int)blockIdx.x)) * C::SLOT;
     __nv_bfloat16* out = a.out + ((long long)b * a.Hq + head0) * D;
-    for (int i = threadIdx.x; i < (whole ? real : HEADS) * D / 4; i += THREADS) {
-      const int head = i * 4 / D;
-      float mm = -INFINITY, MM = -INFINITY, sum = 0.f;
+    {
+      float f[PA_WARPS][4], mm[4], MM[4], sum[4];
       #pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) { mm = fmaxf(mm, stats[w][head]); MM = fmaxf(MM, stats[w][2 * HEADS + head]); }
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      #pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) {
-        sum += stats[w][HEADS + head] * part_factor(stats[w][head], mm);
-        const float f = part_factor(stats[w][2 * HEADS + head], MM);
-        const float4 v = reinterpret_cast<const float4*>(os + w * HEADS * D)[i];
-        acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+      for (int k = 0; k < 4; ++k) {
+        mm[k] = MM[k] = -INFINITY;
+        sum[k] = 0.f;
+        #pragma unroll
+        for (int w = 0; w < PA_WARPS; ++w) { mm[k] = fmaxf(mm[k], stats[w][h + k]); MM[k] = fmaxf(MM[k], stats[w][2 * HEADS + h + k]); }
+        #pragma unroll
+        for (int w = 0; w < PA_WARPS; ++w) {
+          sum[k] += stats[w][HEADS + h + k] * part_factor(stats[w][h + k], mm[k]);
+          f[w][k] = part_factor(stats[w][2 * HEADS + h + k], MM[k]);
+        }
       }
       if (whole) {
-        const float f = out_factor(mm, MM, sum);
-        reinterpret_cast<uint2*>(out)[i] = make_uint2(pack_bf16(acc.x * f, acc.y * f), pack_bf16(acc.z * f, acc.w * f));
-      } else {
-        reinterpret_cast<float4*>(slot)[i] = acc;
-        if (i * 4 % D == 0) {
-          slot[HEADS * D + head] = mm;
-          slot[HEADS * D + HEADS + head] = sum;
-          slot[HEADS * D + 2 * HEADS + head] = MM;
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float o = out_factor(mm[k], MM[k], sum[k]);
+          #pragma unroll
+          for (int w = 0; w < PA_WARPS; ++w) f[w][k] *= o;
+        }
+      } else if ((int)threadIdx.x < fours) {
+        float* st = slot + HEADS * D + h;
+        *reinterpret_cast<float4*>(st) = make_float4(mm[0], mm[1], mm[2], mm[3]);
+        *reinterpret_cast<float4*>(st + HEADS) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        *reinterpret_cast<float4*>(st + 2 * HEADS) = make_float4(MM[0], MM[1], MM[2], MM[3]);
+      }
+      for (int d = threadIdx.x / fours; d < D; d += THREADS / fours) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        #pragma unroll
+        for (int w = 0; w < PA_WARPS; ++w) {
+          const float4 v = *reinterpret_cast<const float4*>(os + w * C::MEET + d * HEADS + d / C::VEL * 8 + h);
+          acc[0] += v.x * f[w][0]; acc[1] += v.y * f[w][1]; acc[2] += v.z * f[w][2]; acc[3] += v.w * f[w][3];
+        }
+        if (whole) {
+          #pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (h + k < real) out[(h + k) * D + d] = __float2bfloat16(acc[k]);
+        } else {
+          *reinterpret_cast<float4*>(slot + d * HEADS + h) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         }
       }
     }
     if (!whole) {
-      __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
-        arrived = atomicAdd(a.counters + c0, 1);
+        arrived = arrive(a.counters + c0);
         if (arrived == parts - 1) a.counters[c0] = 0;
-        __threadfence();
       }
       __syncthreads();
       if (arrived == parts - 1) {
-        // All parts are there: joined in the order of the blocks (the first one holds its part in its second slot).  First a warp per
-        // head finds the largest m and M and leaves each part's factor in the ring, then every thread takes four channels.
+        // All parts are there: joined in the order of the blocks (the first one holds its part in its second slot).  A thread looks at
+        // one head of every LOOK-th part for the largest m and M, then leaves the parts' factors in the ring.
+        constexpr int LOOK = THREADS / HEADS;
         auto part = [&](int k) -> const float* { return a.ws + ((long long)(c0 + k) * 2 + (k == 0)) * C::SLOT; };
-        float* factors = os;                   // [head][parts]
-        for (int head = warp; head < real; head += PA_WARPS) {
-          float mm = -INFINITY, MM = -INFINITY, sum = 0.f;
-          for (int k = lane; k < parts; k += 32) {
-            const float* p = part(k) + HEADS * D + head;
-            mm = fmaxf(mm, __ldcg(p));
-            MM = fmaxf(MM, __ldcg(p + 2 * HEADS));
-          }
+        float* factors = os;                   // [part][head]
+        const int head = threadIdx.x % HEADS;
+        float mm = -INFINITY, MM = -INFINITY, sum = 0.f;
+        #pragma unroll 4
+        for (int k = threadIdx.x / HEADS; k < parts; k += LOOK) {
+          const float* st = part(k) + HEADS * D + head;
+          mm = fmaxf(mm, st[0]);
+          MM = fmaxf(MM, st[2 * HEADS]);
+        }
+        #pragma unroll
+        for (int d = HEADS; d < 32; d <<= 1) {
+          mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+          MM = fmaxf(MM, __shfl_xor_sync(0xffffffffu, MM, d));
+        }
+        if (lane < HEADS) { stats[warp][head] = mm; stats[warp][2 * HEADS + head] = MM; }
+        __syncthreads();
+        #pragma unroll
+        for (int w = 0; w < PA_WARPS; ++w) { mm = fmaxf(mm, stats[w][head]); MM = fmaxf(MM, stats[w][2 * HEADS + head]); }
+        #pragma unroll 4
+        for (int k = threadIdx.x / HEADS; k < parts; k += LOOK) {
+          const float* st = part(k) + HEADS * D + head;
+          sum += st[HEADS] * part_factor(st[0], mm);
+          factors[k * HEADS + head] = part_factor(st[2 * HEADS], MM);
+        }
+        #pragma unroll
+        for (int d = HEADS; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane < HEADS) stats[warp][HEADS + head] = sum;
+        __syncthreads();
+        if (threadIdx.x < HEADS) {
+          sum = 0.f;
           #pragma unroll
-          for (int d = 16; d > 0; d >>= 1) {
-            mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-            MM = fmaxf(MM, __shfl_xor_sync(0xffffffffu, MM, d));
-          }
-          for (int k = lane; k < parts; k += 32) {
-            const float* p = part(k) + HEADS * D + head;
-            sum += __ldcg(p + HEADS) * part_factor(__ldcg(p), mm);
-            factors[head * parts + k] = part_factor(__ldcg(p + 2 * HEADS), MM);
-          }
-          #pragma unroll
-          for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-          if (lane == 0) stats[0][head] = out_factor(mm, MM, sum);
+          for (int w = 0; w < PA_WARPS; ++w) sum += stats[w][HEADS + head];
+          stats[0][head] = out_factor(mm, MM, sum);
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < real * D / 4; i += THREADS) {
-          const int head = i * 4 / D;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          #pragma unroll 8
-          for (int k = 0; k < parts; ++k) {
-            const float f = factors[head * parts + k];
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(part(k)) + i);
-            acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+        // up to 32 loads of a thread under way: of each of its channels from some parts
+        constexpr int MANY = D * HEADS / 4 / THREADS, AT_ONCE = MANY > 2 ? 8 : 16;
+        float4 acc[MANY];
+        #pragma unroll
+        for (int i = 0; i < MANY; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int d0 = threadIdx.x / fours, dd = THREADS / fours;
+        for (int k0 = 0; k0 < parts; k0 += AT_ONCE) {
+          float4 v[AT_ONCE][MANY];
+          #pragma unroll
+          for (int k = 0; k < AT_ONCE; ++k) {
+            #pragma unroll
+            for (int i = 0; i < MANY; ++i) {
+              v[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (k0 + k < parts && d0 + i * dd < D) v[k][i] = *reinterpret_cast<const float4*>(part(k0 + k) + (d0 + i * dd) * HEADS + h);
+            }
           }
-          const float f = stats[0][head];
-          reinterpret_cast<uint2*>(out)[i] = make_uint2(pack_bf16(acc.x * f, acc.y * f), pack_bf16(acc.z * f, acc.w * f));
+          #pragma unroll
+          for (int k = 0; k < AT_ONCE; ++k) {
+            if (k0 + k >= parts) break;
+            const float4 f = *reinterpret_cast<const float4*>(factors + (k0 + k) * HEADS + h);
+            #pragma unroll
+            for (int i = 0; i < MANY; ++i) { acc[i].x += f.x * v[k][i].x; acc[i].y += f.y * v[k][i].y; acc[i].z += f.z * v[k][i].z; acc[i].w += f.w * v[k][i].w; }
+          }
+        }
+        #pragma unroll
+        for (int i = 0; i < MANY; ++i) {
+          const int d = d0 + i * dd;
+          const float r[4] = {acc[i].x, acc[i].y, acc[i].z, acc[i].w};
+          #pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (d < D && h + k < real) out[(h + k) * D + d] = __float2bfloat16(r[k] * stats[0][h + k]);
         }
       }
     }
@@ -613,7 +733,7 @@ static int paged_attn_launch(const AttnArgs& a, int grid, cudaStream_t st) {
   const uint64_t rows = ((uint64_t)a.table.pages * a.Hk) << a.table.page_shift;
   for (int i = 0; i < 2; ++i)
     if (make_tmap_2d(&map[i], C::BYTES == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, C::BYTES, a.pages[i], D, rows, C::ROW,
-                     C::TILE / C::BYTES, PA_STEP, C::TILE == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
+                     C::TILE / C::BYTES, PA_BOX, C::TILE == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
       return -SSM_ERR_BAD_ARG;
   paged_attn_kernel<D, T, NT><<<grid, PA_WARPS * 32, C::SMEM, st>>>(a, map[0], map[1]);
   return (int)cudaGetLastError();
@@ -623,27 +743,29 @@ static int paged_attn_launch(const AttnArgs& a, int grid, cudaStream_t st) {
 static bool two_tiles(int ratio, int D) { return ratio > 8 && D <= 128; }
 
 template <int D, int T, int NT>
-static void paged_attn_shape(int* blocks, int* slot) {
+static void paged_attn_shape(int* blocks, int* slot, int* step) {
   *blocks = PagedAttn<D, T, NT>::BLOCKS;
   *slot = PagedAttn<D, T, NT>::SLOT;
+  *step = PagedAttn<D, T, NT>::STEP;
 }
 // blocks of the launch, and floats of its workspace
 static int paged_attn_plan(int type, int width, int page_size, int B, int Hq, int Hk, int D, int* grid, int* most_blocks, long long* floats) {
-  int blocks = 0, slot = 0, sms = 0, dev = 0;
+  int blocks = 0, slot = 0, step = 1, sms = 0, dev = 0;
   const int ratio = Hq / Hk;
   const bool two = two_tiles(ratio, D);
   #define SHAPE(DD, TT)                                                                  \
     do {                                                                                 \
-      if (two) paged_attn_shape<DD, TT, (DD <= 128 ? 2 : 1)>(&blocks, &slot);            \
-      else paged_attn_shape<DD, TT, 1>(&blocks, &slot);                                  \
+      if (two) paged_attn_shape<DD, TT, (DD <= 128 ? 2 : 1)>(&blocks, &slot, &step);            \
+      else paged_attn_shape<DD, TT, 1>(&blocks, &slot, &step);                                  \
     } while (0)
   KV_DISPATCH(SHAPE);
   #undef SHAPE
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return (int)cudaGetLastError();
   const int group = two ? 16 : 8;
   // no more blocks than there can be shares
-  const long long most = (long long)B * Hk * ((ratio + group - 1) / group) * (((long long)width * page_size + PA_STEP - 1) / PA_STEP);
-  const long long shares = (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE + (long long)B * Hk * ((ratio + group - 1) / group);
+  const long long items = (long long)B * Hk * ((ratio + group - 1) / group), most = items * (((long long)width * page_size + step - 1) / step);
+  if (most > 0x7fffffffll - (1 << 20)) return -SSM_ERR_BAD_ARG;                // counted in 32 bits
+  const long long shares = (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE + items;
   long long n = (long long)sms * blocks;
   if (n > PA_COUNTERS) n = PA_COUNTERS;
   *most_blocks = (int)n;
