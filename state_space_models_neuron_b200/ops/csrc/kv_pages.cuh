@@ -28,6 +28,22 @@ __device__ __forceinline__ int page_of(const PageTable& t, int b, int p) {
   return -1;
 }
 
+// four 8-bit values -> two pairs of fp16, exact
+template <int T>
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (T == KV_E4M3) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+  } else {
+    // 1024 + (x + 128) is an fp16 number whose low byte is x + 128
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));      // 1152
+    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  }
+}
+
 static bool kv_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 static bool kv_table(PageTable* t, const void* ids, const void* lengths, int width, int pages, int page_size, int* status) {
   if (width < 0 || pages < 0 || page_size < 16 || (page_size & (page_size - 1))) return false;

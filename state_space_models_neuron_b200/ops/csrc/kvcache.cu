@@ -5,21 +5,38 @@
 
 namespace ssm {
 
-__device__ __forceinline__ uint32_t e4m3x4(const float* f) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
-}
-__device__ __forceinline__ uint32_t int8x4(const float* f) {
-  uint32_t u = 0;
+// 16 values times inv, rounded to nearest even, as 16 bytes
+__device__ __forceinline__ void quantise_e4m3(const Pairs& y, uint64_t inv, uint2& lo, uint2& hi) {
+  uint32_t v[4];
   #pragma unroll
-  for (int i = 0; i < 4; ++i) u |= (uint32_t)(__float2int_rn(f[i]) & 0xff) << (8 * i);
-  return u;
+  for (int i = 0; i < 4; ++i) {
+    float a, b, c, d;
+    unpack2(mul2(y[2 * i], inv), a, b);
+    unpack2(mul2(y[2 * i + 1], inv), c, d);
+    asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\tmov.b32 %0, {l, h};\n\t}"
+        : "=r"(v[i]) : "f"(a), "f"(b), "f"(c), "f"(d));
+  }
+  lo = make_uint2(v[0], v[1]);
+  hi = make_uint2(v[2], v[3]);
 }
-template <int T>
-__device__ __forceinline__ float kv_value(uint32_t byte) {
-  if (T == KV_INT8) return (float)(int8_t)byte;
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
+// The sum of a number of at most 127 and 1.5 * 2^23 is rounded to an integer whose low byte is the number's.
+__device__ __forceinline__ void quantise_int8(const Pairs& y, uint64_t inv, uint2& lo, uint2& hi) {
+  uint32_t v[4];
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a, b, c, d;
+    unpack2(fma2(y[2 * i], inv, both(12582912.f)), a, b);
+    unpack2(fma2(y[2 * i + 1], inv, both(12582912.f)), c, d);
+    v[i] = __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040), __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
+  }
+  lo = make_uint2(v[0], v[1]);
+  hi = make_uint2(v[2], v[3]);
+}
+// the larger magnitude; NaN if there is one
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 struct WriteArgs {
@@ -38,134 +55,181 @@ struct WriteArgs {
   float eps;
 };
 
+constexpr int KV_THREADS = 256, KV_WARPS = KV_THREADS / 32;
+
+// A warp takes `each` heads of one tensor for as many tokens as rows fit a warp, all asked for first, as in the norms' own kernel.
 template <int D, int T>
-__global__ void __launch_bounds__(256) kv_write_kernel(const WriteArgs a) {
-  constexpr int LANES = D / 16;
-  const int lane = threadIdx.x % LANES, heads = a.heads[0] + a.heads[1] + a.heads[2];
+__global__ void __launch_bounds__(KV_THREADS, 3) kv_write_kernel(const WriteArgs a, int each) {
+  constexpr int LANES = D / 16, TOKENS = 32 / LANES;
+  extern __shared__ uint4 slots[];             // [row][vector][thread]
+  const int lane = threadIdx.x % LANES;
   const HeadRow<D> at(lane, a.rot);
-  const long long rows = (long long)a.B * a.L * heads, step = (long long)gridDim.x * (256 / LANES);
-  for (long long first = (long long)blockIdx.x * (256 / LANES); first < rows; first += step) {
-    const long long mine = first + threadIdx.x / LANES;
-    const long long row = mine < rows ? mine : rows - 1;
-    const long long token = row / heads;
-    int h = (int)(row % heads), which = 0;
-    if (h >= a.heads[0]) { h -= a.heads[0]; which = 1; }
-    if (which == 1 && h >= a.heads[1]) { h -= a.heads[1]; which = 2; }
-    const int b = (int)(token / a.L), l = (int)(token % a.L);
-    const int given = a.counts == nullptr ? a.L : a.counts[b];
-    const int count = given < 0 ? 0 : given > a.L ? a.L : given;
-    if (count != given) report_bad_index(a.table.status);
-    const int pos = a.table.lengths[b] - count + l;
-    bool real = l < count && pos >= 0;
-    int page = -1;
-    if (real) page = page_of(a.table, b, pos);
-    real = page >= 0;
-    if (real && a.rot && pos >= a.table_rows) { report_bad_index(a.table.status); real = false; }
-    const __nv_bfloat16* x = a.x[which] + b * a.sb[which] + l * a.sl[which] + h * a.sh[which];
-    float y[16];
-    unpack16(*reinterpret_cast<const uint4*>(x + at.c0), *reinterpret_cast<const uint4*>(x + at.c1), y);
-    const bool normed = which < 2 && a.w[which] != nullptr;
-    float ss = 0.f;
-    #pragma unroll
-    for (int i = 0; i < 16; ++i) ss += y[i] * y[i];
-    ss = row_sum<LANES>(ss);
-    if (normed) {
-      float w[16];
-      load_weight<D>(a.w[which], a.w32[which], at, w);
-      const float r = rsqrtf(ss * (1.f / D) + a.eps);
+  const int qu = (a.heads[0] + each - 1) / each, ku = (a.heads[1] + each - 1) / each, units = qu + 2 * ku;
+  const long long warp = (long long)blockIdx.x * KV_WARPS + threadIdx.x / 32, block = warp / units;
+  int part = (int)(warp - block * units);
+  const int which = part < qu ? 0 : part < qu + ku ? 1 : 2;                     // the same for the whole warp
+  part -= which == 0 ? 0 : which == 1 ? qu : qu + ku;
+  const long long mine = block * TOKENS + threadIdx.x % 32 / LANES;
+  const bool exists = mine < (long long)a.B * a.L;
+  const int token = exists ? (int)mine : 0;
+  const int b = token / a.L, l = token - b * a.L, h0 = part * each, h1 = exists ? min(a.heads[which], h0 + each) : 0;
+  const __nv_bfloat16* x = a.x[which] + b * a.sb[which] + l * a.sl[which] + h0 * a.sh[which];
+  for (int i = 0; i < each; ++i) {
+    const __nv_bfloat16* src = h0 + i < h1 ? x + i * a.sh[which] : x;
+    fetch16(slots + (i * 2) * KV_THREADS + threadIdx.x, src + at.c0, h0 + i < h1);
+    fetch16(slots + (i * 2 + 1) * KV_THREADS + threadIdx.x, src + at.c1, h0 + i < h1);
+    if (i == each / 2 - 1) fetch_commit();
+  }
+  fetch_commit();
+  // where the token goes
+  const int given = a.counts == nullptr ? a.L : a.counts[b];
+  const int count = given < 0 ? 0 : given > a.L ? a.L : given;
+  if (count != given) report_bad_index(a.table.status);
+  const int pos = a.table.lengths[b] - count + l;
+  int page = -1;
+  if (l < count && pos >= 0) {
+    page = page_of(a.table, b, pos);
+    if (a.rot && pos >= a.table_rows) { report_bad_index(a.table.status); page = -1; }
+  }
+  const void* weight = which < 2 ? a.w[which] : nullptr;
+  const bool turns = which < 2 && page >= 0 && at.turns;
+  Pairs w;
+  uint64_t cs[4], sn[4];
+  load_weight<D>(weight, which < 2 ? a.w32[which] : 0, at, w);
+  if (turns) {
+    load_pairs(a.cs + (long long)pos * (a.rot / 2) + at.c0, cs);
+    load_pairs(a.sn + (long long)pos * (a.rot / 2) + at.c0, sn);
+  }
+  fetch_wait<1>();                             // the first half
+  for (int i = 0; i < each; ++i) {
+    if (i == each / 2) fetch_wait<0>();
+    Pairs y;
+    unpack_pairs(slots[(i * 2) * KV_THREADS + threadIdx.x], slots[(i * 2 + 1) * KV_THREADS + threadIdx.x], y);
+    if (weight != nullptr) {
+      uint64_t ss = mul2(y[0], y[0]);
       #pragma unroll
-      for (int i = 0; i < 16; ++i) y[i] *= r * w[i];
+      for (int k = 1; k < 8; ++k) ss = fma2(y[k], y[k], ss);
+      const uint64_t r = both(rms_factor<D>(row_sum<LANES>(pair_sum(ss)), a.eps));
+      #pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] = mul2(mul2(y[k], r), w[k]);
     }
-    if (which < 2 && real && at.turns) {
-      float cs[8], sn[8];
-      load8(a.cs + (long long)pos * (a.rot / 2) + at.c0, cs);
-      load8(a.sn + (long long)pos * (a.rot / 2) + at.c0, sn);
-      turn16(y, cs, sn, 1.f);
-    }
-    uint32_t top = 0;                            // largest magnitude as bits: NaN is above infinity, which is above all numbers
-    #pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
-    #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (mine >= rows) continue;
-    if (which == 0) {
-      __nv_bfloat16* o = a.qo + (token * a.heads[0] + h) * D;
+    if (turns) turn_pairs<false>(y, cs, sn);
+    const long long slot = (((long long)page * a.heads[1] + h0 + i) << a.table.page_shift) + (pos & ((1 << a.table.page_shift) - 1));
+    if (which == 0 || T == KV_BF16) {
+      const bool real = page >= 0;
+      if (h0 + i >= h1 || (which != 0 && !real)) continue;
       const uint4 zero = make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4*>(o + at.c0) = real ? pack8(y) : zero;
-      *reinterpret_cast<uint4*>(o + at.c1) = real ? pack8(y + 8) : zero;
-      continue;
-    }
-    if (!real) continue;
-    const long long slot = (((long long)page * a.heads[1] + h) << a.table.page_shift) + (pos & ((1 << a.table.page_shift) - 1));
-    if (T == KV_BF16) {
-      __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.pages[which - 1]) + slot * D;
-      *reinterpret_cast<uint4*>(o + at.c0) = pack8(y);
-      *reinterpret_cast<uint4*>(o + at.c1) = pack8(y + 8);
+      __nv_bfloat16* o = which == 0 ? a.qo + ((long long)token * a.heads[0] + h0 + i) * D : reinterpret_cast<__nv_bfloat16*>(a.pages[which - 1]) + slot * D;
+      *reinterpret_cast<uint4*>(o + at.c0) = real ? pack_pairs(y) : zero;
+      *reinterpret_cast<uint4*>(o + at.c1) = real ? pack_pairs(y + 4) : zero;
     } else {
       constexpr float QMAX = T == KV_E4M3 ? 448.f : 127.f;
-      const bool fine = top < 0x7f800000u, some = fine && top >= (27u << 23);     // 2^-100
-      const float amax = __uint_as_float(top);
-      const float inv = some ? __fdiv_rn(QMAX, amax) : 0.f;
+      float top = 0.f;
       #pragma unroll
-      for (int i = 0; i < 16; ++i) y[i] = some ? y[i] * inv : 0.f;
-      uint8_t* o = reinterpret_cast<uint8_t*>(a.pages[which - 1]) + slot * D;
-      uint2 lo, hi;
-      if (T == KV_E4M3) {
-        lo = make_uint2(e4m3x4(y), e4m3x4(y + 4)); hi = make_uint2(e4m3x4(y + 8), e4m3x4(y + 12));
-      } else {
-        lo = make_uint2(int8x4(y), int8x4(y + 4)); hi = make_uint2(int8x4(y + 8), int8x4(y + 12));
+      for (int k = 0; k < 8; ++k) {
+        float lo, hi;
+        unpack2(y[k], lo, hi);
+        top = max_nan(max_nan(top, fabsf(lo)), fabsf(hi));
       }
+      #pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (h0 + i >= h1 || page < 0) continue;
+      const bool some = __float_as_uint(top) - (27u << 23) < 0x7f800000u - (27u << 23);      // finite and at least 2^-100
+      const uint64_t inv = both(some ? __fdiv_rn(QMAX, top) : 0.f);
+      uint2 lo, hi;
+      if (T == KV_E4M3) quantise_e4m3(y, inv, lo, hi); else quantise_int8(y, inv, lo, hi);
+      uint8_t* o = reinterpret_cast<uint8_t*>(a.pages[which - 1]) + slot * D;
       *reinterpret_cast<uint2*>(o + at.c0) = lo;
       *reinterpret_cast<uint2*>(o + at.c1) = hi;
-      if (lane == 0) a.scales[which - 1][slot] = some ? __fdiv_rn(amax, QMAX) : fine ? 0.f : __uint_as_float(0x7fc00000u);
+      // a row with a value that is not finite reads back as NaN whatever is stored
+      if (lane == 0) a.scales[which - 1][slot] = some ? __fdiv_rn(top, QMAX) : top < 1.f ? 0.f : __uint_as_float(0x7fc00000u);
     }
   }
 }
 
-// 16 channels per thread
+// A block takes rows (token, head) of one sequence, D / 16 lanes a row of keys and the same of values, two rows under way.
+constexpr int READ_ROWS = 2;
 template <int D, int T, typename Out>
-__global__ void __launch_bounds__(256) kv_read_kernel(const void* __restrict__ pages0, const void* __restrict__ pages1, const float* __restrict__ scale0,
-                                                      const float* __restrict__ scale1, Out* __restrict__ out0, Out* __restrict__ out1,
-                                                      PageTable table, int B, int most, int heads) {
-  constexpr int LANES = D / 16;
-  const long long total = (long long)B * most * heads * LANES, both = 2 * total;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < both; i += (long long)gridDim.x * 256) {
-    const bool second = i >= total;
-    const long long at = second ? i - total : i;
-    const int lane = (int)(at % LANES);
-    const long long row = at / LANES;
-    const int h = (int)(row % heads);
-    const long long tok = row / heads;
-    const int b = (int)(tok / most), p = (int)(tok % most);
-    float y[16];
+__global__ void __launch_bounds__(KV_THREADS, 5) kv_read_kernel(const void* __restrict__ pages0, const void* __restrict__ pages1, const float* __restrict__ scale0,
+                                                                const float* __restrict__ scale1, Out* __restrict__ out0, Out* __restrict__ out1,
+                                                                PageTable table, int most, int heads) {
+  constexpr int LANES = D / 16, GROUPS = KV_THREADS / LANES, VECS = T == KV_BF16 ? 2 : 1;
+  const int lane = threadIdx.x % LANES, b = blockIdx.y, n = table.lengths[b];
+  const unsigned rows = (unsigned)most * heads, first = blockIdx.x * (GROUPS * READ_ROWS) + threadIdx.x / LANES;
+  uint4 u[READ_ROWS][2][VECS];
+  float s[READ_ROWS][2];
+  #pragma unroll
+  for (int i = 0; i < READ_ROWS; ++i) {
+    const unsigned row = first + i * GROUPS;
+    const int p = row / heads, h = row - p * heads;
     #pragma unroll
-    for (int k = 0; k < 16; ++k) y[k] = 0.f;
-    const int page = p < table.lengths[b] ? page_of(table, b, p) : -1;
-    if (page >= 0) {
-      const long long slot = (((long long)page * heads + h) << table.page_shift) + (p & ((1 << table.page_shift) - 1));
-      const uint8_t* src = reinterpret_cast<const uint8_t*>(second ? pages1 : pages0) + (slot * D + lane * 16) * KvType<T>::BYTES;
+    for (int k = 0; k < VECS; ++k) u[i][0][k] = u[i][1][k] = make_uint4(0, 0, 0, 0);
+    s[i][0] = s[i][1] = 0.f;
+    const int page = row < rows && p < n ? page_of(table, b, p) : -1;
+    if (page < 0) continue;
+    const long long slot = (((long long)page * heads + h) << table.page_shift) + (p & ((1 << table.page_shift) - 1));
+    const long long at = (slot * D + lane * 16) * KvType<T>::BYTES;
+    #pragma unroll
+    for (int k = 0; k < VECS; ++k) {
+      u[i][0][k] = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(pages0) + at)[k];
+      u[i][1][k] = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(pages1) + at)[k];
+    }
+    if (T != KV_BF16) { s[i][0] = scale0[slot]; s[i][1] = scale1[slot]; }
+  }
+  #pragma unroll
+  for (int i = 0; i < READ_ROWS; ++i) {
+    const unsigned row = first + i * GROUPS;
+    if (row >= rows) break;
+    #pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      Out* o = (j ? out1 : out0) + ((long long)b * rows + row) * D + lane * 16;
+      if (T == KV_BF16 && sizeof(Out) == 2) {
+        reinterpret_cast<uint4*>(o)[0] = u[i][j][0];
+        reinterpret_cast<uint4*>(o)[1] = u[i][j][VECS - 1];
+        continue;
+      }
+      Pairs y;
       if (T == KV_BF16) {
-        unpack16(reinterpret_cast<const uint4*>(src)[0], reinterpret_cast<const uint4*>(src)[1], y);
+        unpack_pairs(u[i][j][0], u[i][j][VECS - 1], y);
       } else {
-        const uint4 u = *reinterpret_cast<const uint4*>(src);
-        const float s = (second ? scale1 : scale0)[slot];
-        const uint32_t words[4] = {u.x, u.y, u.z, u.w};
+        const uint32_t words[4] = {u[i][j][0].x, u[i][j][0].y, u[i][j][0].z, u[i][j][0].w};
+        const uint64_t s2 = both(s[i][j]);
         #pragma unroll
-        for (int k = 0; k < 16; ++k) y[k] = kv_value<T>((words[k / 4] >> (8 * (k % 4))) & 0xff) * s;
+        for (int k = 0; k < 4; ++k) {
+          uint32_t lo, hi;
+          widen4<T>(words[k], lo, hi);
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&lo)), g = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+          y[2 * k] = mul2(pack2(f.x, f.y), s2);
+          y[2 * k + 1] = mul2(pack2(g.x, g.y), s2);
+        }
+      }
+      if (sizeof(Out) == 2) {
+        reinterpret_cast<uint4*>(o)[0] = pack_pairs(y);
+        reinterpret_cast<uint4*>(o)[1] = pack_pairs(y + 4);
+      } else {
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) reinterpret_cast<ulonglong2*>(o)[k] = make_ulonglong2(y[2 * k], y[2 * k + 1]);
       }
     }
-    Out* o = (second ? out1 : out0) + row * D + lane * 16;
-    if (sizeof(Out) == 2) {
-      reinterpret_cast<uint4*>(o)[0] = pack8(y);
-      reinterpret_cast<uint4*>(o)[1] = pack8(y + 8);
-    } else {
-      #pragma unroll
-      for (int k = 0; k < 4; ++k) reinterpret_cast<float4*>(o)[k] = make_float4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
-    }
   }
 }
 
-static unsigned kv_grid(long long blocks) { return (unsigned)(blocks < 148 * 8 ? blocks : 148 * 8); }
+// Heads that a warp takes one after the other: 8, or fewer where that would leave less than three blocks per SM.
+static long long write_warps(long long tokens, int Hq, int Hk, int each, int D) {
+  return (tokens * (D / 16) + 31) / 32 * ((Hq + each - 1) / each + 2 * ((Hk + each - 1) / each));
+}
+template <int D, int T>
+static int kv_write_launch(const WriteArgs& a, int Hq, int Hk, cudaStream_t st) {
+  const long long tokens = (long long)a.B * a.L;
+  int each = EACH;
+  while (each > 1 && write_warps(tokens, Hq, Hk, each, D) < 148ll * 3 * KV_WARPS) each /= 2;
+  const long long grid = (write_warps(tokens, Hq, Hk, each, D) + KV_WARPS - 1) / KV_WARPS;
+  if (grid > 0x7fffffffll) return -SSM_ERR_BAD_ARG;
+  static SmemOptIn opt;
+  if (int e = opt.ask(reinterpret_cast<const void*>(kv_write_kernel<D, T>), EACH * 2 * KV_THREADS * 16)) return e;
+  kv_write_kernel<D, T><<<(unsigned)grid, KV_THREADS, each * 2 * KV_THREADS * 16, st>>>(a, each);
+  return (int)cudaGetLastError();
+}
 
 }  // namespace ssm
 
@@ -178,7 +242,7 @@ extern "C" int ssm_kv_write(const void* q, const void* k, const void* v, const l
                             const void* counts, int B, int L, int Hq, int Hk, int D, int* status, cudaStream_t st) {
   WriteArgs a;
   if (!kv_table(&a.table, table, lengths, width, pages, page_size, status)) return -SSM_ERR_BAD_ARG;
-  if (B < 1 || L < 1 || Hq < 0 || Hk < 1 || rot < 0 || rot % 16 || rot > D) return -SSM_ERR_BAD_ARG;
+  if (B < 1 || L < 1 || (long long)B * L > 0x7fffffffll || Hq < 0 || Hk < 1 || rot < 0 || rot % 16 || rot > D) return -SSM_ERR_BAD_ARG;
   const void* all[] = {q, k, v, qo, qw, kw, cs, sn, kp, vp};
   for (const void* p : all) if (!kv_aligned(p)) return -SSM_ERR_BAD_ARG;
   for (int i = 0; i < 9; ++i) if (strides[i] % 8) return -SSM_ERR_BAD_ARG;
@@ -196,12 +260,10 @@ extern "C" int ssm_kv_write(const void* q, const void* k, const void* v, const l
   a.counts = reinterpret_cast<const int*>(counts);
   a.cs = reinterpret_cast<const float*>(cs); a.sn = reinterpret_cast<const float*>(sn);
   a.B = B; a.L = L; a.rot = rot; a.table_rows = table_rows; a.eps = eps;
-  const int per = 256 / (D / 16 > 0 ? D / 16 : 1);
-  const unsigned grid = kv_grid(((long long)B * L * (Hq + 2 * Hk) + per - 1) / per);
-  #define WRITE(DD, TT) kv_write_kernel<DD, TT><<<grid, 256, 0, st>>>(a)
+  #define WRITE(DD, TT) return kv_write_launch<DD, TT>(a, Hq, Hk, st)
   KV_DISPATCH(WRITE);
   #undef WRITE
-  return (int)cudaGetLastError();
+  return -SSM_ERR_BAD_ARG;
 }
 
 extern "C" int ssm_kv_read(const void* kp, const void* vp, const void* ks, const void* vs, int type, int pages, int page_size, const void* table,
@@ -210,15 +272,17 @@ extern "C" int ssm_kv_read(const void* kp, const void* vp, const void* ks, const
   PageTable t;
   if (!kv_table(&t, table, lengths, width, pages, page_size, status)) return -SSM_ERR_BAD_ARG;
   if (B < 1 || most < 1 || Hk < 1 || !kv_aligned(kp) || !kv_aligned(vp) || !kv_aligned(ko) || !kv_aligned(vo)) return -SSM_ERR_BAD_ARG;
-  const unsigned grid = kv_grid((2ll * B * most * Hk * (D / 16) + 255) / 256);
+  if (B > 65535 || (long long)most * Hk > 0x7fffffffll || (D != 64 && D != 128 && D != 256)) return -SSM_ERR_BAD_ARG;
+  const long long per = KV_THREADS / (D / 16) * READ_ROWS;
+  const dim3 grid((unsigned)(((long long)most * Hk + per - 1) / per), B);
   const float* s0 = reinterpret_cast<const float*>(ks);
   const float* s1 = reinterpret_cast<const float*>(vs);
   #define READ(DD, TT)                                                                                                             \
     do {                                                                                                                           \
-      if (out32) kv_read_kernel<DD, TT, float><<<grid, 256, 0, st>>>(kp, vp, s0, s1, reinterpret_cast<float*>(ko),                 \
-                                                                     reinterpret_cast<float*>(vo), t, B, most, Hk);                \
-      else kv_read_kernel<DD, TT, __nv_bfloat16><<<grid, 256, 0, st>>>(kp, vp, s0, s1, reinterpret_cast<__nv_bfloat16*>(ko),       \
-                                                                       reinterpret_cast<__nv_bfloat16*>(vo), t, B, most, Hk);      \
+      if (out32) kv_read_kernel<DD, TT, float><<<grid, KV_THREADS, 0, st>>>(kp, vp, s0, s1, reinterpret_cast<float*>(ko),                 \
+                                                                     reinterpret_cast<float*>(vo), t, most, Hk);                   \
+      else kv_read_kernel<DD, TT, __nv_bfloat16><<<grid, KV_THREADS, 0, st>>>(kp, vp, s0, s1, reinterpret_cast<__nv_bfloat16*>(ko),       \
+                                                                       reinterpret_cast<__nv_bfloat16*>(vo), t, most, Hk);         \
     } while (0)
   KV_DISPATCH(READ);
   #undef READ

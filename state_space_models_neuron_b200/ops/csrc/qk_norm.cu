@@ -22,135 +22,196 @@ struct NormArgs {
   int* status;
 };
 
-// row of the tables of token (b, l); -1 where the caller's position is outside
-__device__ __forceinline__ int table_row(const NormArgs& a, long long token, int l) {
-  if (a.positions == nullptr) return l;
-  const long long p = a.pos64 ? reinterpret_cast<const long long*>(a.positions)[token] : reinterpret_cast<const int*>(a.positions)[token];
-  if (p >= 0 && p < a.table_rows) return (int)p;
-  report_bad_index(a.status);
-  return -1;
+// cosines and sines of the lane's pairs for token (b, l); false where the caller's position is outside the tables
+__device__ __forceinline__ bool load_angles(const NormArgs& a, int token, int l, int c0, bool turns, uint64_t (&cs)[4], uint64_t (&sn)[4]) {
+  long long p = l;
+  if (a.positions != nullptr) p = a.pos64 ? reinterpret_cast<const long long*>(a.positions)[token] : reinterpret_cast<const int*>(a.positions)[token];
+  if (p < 0 || p >= a.table_rows) {
+    report_bad_index(a.status);
+    return false;
+  }
+  if (turns) {
+    load_pairs(a.cs + p * (a.rot / 2) + c0, cs);
+    load_pairs(a.sn + p * (a.rot / 2) + c0, sn);
+  }
+  return true;
 }
 
+constexpr int NORM_THREADS = 256, NORM_WARPS = NORM_THREADS / 32;
+
+// A warp takes `each` heads of one tensor for as many tokens as rows fit a warp (`units` such parts for them).  All its rows are asked
+// for first; positions, angles and weights come while they are under way.
 template <int D>
-__global__ void __launch_bounds__(256) qk_norm_fwd_kernel(const NormArgs a) {
-  constexpr int LANES = D / 16;
-  const int lane = threadIdx.x % LANES, heads = a.t[0].heads + a.t[1].heads;
+__global__ void __launch_bounds__(NORM_THREADS, 3) qk_norm_fwd_kernel(const NormArgs a, int each) {
+  constexpr int LANES = D / 16, TOKENS = 32 / LANES;
+  extern __shared__ uint4 slots[];             // [row][vector][thread]
+  const int lane = threadIdx.x % LANES;
   const HeadRow<D> at(lane, a.rot);
-  const long long rows = (long long)a.B * a.L * heads, step = (long long)gridDim.x * (256 / LANES);
-  // whole warps take part in the shuffles: a row behind the last one is computed as the last and not stored
-  for (long long first = (long long)blockIdx.x * (256 / LANES); first < rows; first += step) {
-    const long long mine = first + threadIdx.x / LANES;
-    const long long row = mine < rows ? mine : rows - 1;
-    const long long token = row / heads;
-    const int head = (int)(row % heads), which = head >= a.t[0].heads, h = which ? head - a.t[0].heads : head;
-    const int b = (int)(token / a.L), l = (int)(token % a.L);
-    const HeadRows& t = a.t[which];
-    const __nv_bfloat16* x = t.x + b * t.xb + l * t.xl + h * t.xh;
-    float y[16];
-    unpack16(*reinterpret_cast<const uint4*>(x + at.c0), *reinterpret_cast<const uint4*>(x + at.c1), y);
+  const int q_units = (a.t[0].heads + each - 1) / each, units = q_units + (a.t[1].heads + each - 1) / each;
+  const long long warp = (long long)blockIdx.x * NORM_WARPS + threadIdx.x / 32;
+  const long long block = warp / units;
+  int part = (int)(warp - block * units);
+  const int which = part >= q_units;
+  if (which) part -= q_units;
+  const HeadRows& t = a.t[which];
+  const long long mine = block * TOKENS + threadIdx.x % 32 / LANES;
+  const bool real = mine < (long long)a.B * a.L;
+  const int token = real ? (int)mine : 0;
+  const int b = token / a.L, l = token - b * a.L, h0 = part * each, h1 = real ? min(t.heads, h0 + each) : 0;
+  const __nv_bfloat16* x = t.x + b * t.xb + l * t.xl + h0 * t.xh;
+  for (int i = 0; i < each; ++i) {
+    const __nv_bfloat16* src = h0 + i < h1 ? x + i * t.xh : x;
+    fetch16(slots + (i * 2) * NORM_THREADS + threadIdx.x, src + at.c0, h0 + i < h1);
+    fetch16(slots + (i * 2 + 1) * NORM_THREADS + threadIdx.x, src + at.c1, h0 + i < h1);
+    if (i == each / 2 - 1) fetch_commit();
+  }
+  fetch_commit();
+  __nv_bfloat16* out = t.out + ((long long)token * t.heads + h0) * D;
+  Pairs w;
+  uint64_t cs[4], sn[4];
+  load_weight<D>(t.w, t.w32, at, w);
+  bool inside = true;
+  if (a.rot && real) inside = load_angles(a, token, l, at.c0, at.turns, cs, sn);
+  const bool turns = a.rot && real && inside && at.turns;
+  fetch_wait<1>();                             // the first half
+  for (int i = 0; i < each; ++i) {             // the same number of turns for all lanes
+    if (i == each / 2) fetch_wait<0>();
+    Pairs y;
+    unpack_pairs(slots[(i * 2) * NORM_THREADS + threadIdx.x], slots[(i * 2 + 1) * NORM_THREADS + threadIdx.x], y);
     if (t.w != nullptr) {
-      float w[16], ss = 0.f;
-      load_weight<D>(t.w, t.w32, at, w);
+      uint64_t ss = mul2(y[0], y[0]);
       #pragma unroll
-      for (int i = 0; i < 16; ++i) ss += y[i] * y[i];
-      const float r = rsqrtf(row_sum<LANES>(ss) * (1.f / D) + a.eps);
+      for (int k = 1; k < 8; ++k) ss = fma2(y[k], y[k], ss);
+      const uint64_t r = both(rms_factor<D>(row_sum<LANES>(pair_sum(ss)), a.eps));
       #pragma unroll
-      for (int i = 0; i < 16; ++i) y[i] *= r * w[i];
-    } else {
-      row_sum<LANES>(0.f);
+      for (int k = 0; k < 8; ++k) y[k] = mul2(mul2(y[k], r), w[k]);
     }
-    if (a.rot) {
-      const int p = table_row(a, token, l);
-      if (p < 0) {
-        #pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = 0.f;
-      } else if (at.turns) {
-        float cs[8], sn[8];
-        load8(a.cs + (long long)p * (a.rot / 2) + at.c0, cs);
-        load8(a.sn + (long long)p * (a.rot / 2) + at.c0, sn);
-        turn16(y, cs, sn, 1.f);
-      }
-    }
-    if (mine < rows) {
-      __nv_bfloat16* o = t.out + (token * t.heads + h) * D;
-      *reinterpret_cast<uint4*>(o + at.c0) = pack8(y);
-      *reinterpret_cast<uint4*>(o + at.c1) = pack8(y + 8);
+    if (turns) turn_pairs<false>(y, cs, sn);
+    if (h0 + i < h1) {
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(out + i * D + at.c0) = inside ? pack_pairs(y) : zero;
+      *reinterpret_cast<uint4*>(out + i * D + at.c1) = inside ? pack_pairs(y + 4) : zero;
     }
   }
 }
 
-// Blocks [0, q_blocks) take the queries' rows, the others the keys'; each leaves its sum of g x r in part[block][D].
+// Blocks [0, q_blocks) take the queries' rows, the others the keys'.  A warp takes `each` heads for as many tokens as rows fit a
+// warp at a time, with GRAD_DEPTH rows under way, those of its next turn among them.  Each block leaves its sum of g x r in part[block][D].
+constexpr int GRAD_DEPTH = 4;
 template <int D>
-__global__ void __launch_bounds__(256) qk_norm_bwd_kernel(const NormArgs a, int q_blocks, float* __restrict__ part) {
-  constexpr int LANES = D / 16, ROWS = 256 / LANES;
+__global__ void __launch_bounds__(NORM_THREADS, 2) qk_norm_bwd_kernel(const NormArgs a, int q_blocks, int each, float* __restrict__ part) {
+  constexpr int LANES = D / 16, TOKENS = 32 / LANES;
+  extern __shared__ uint4 slots[];             // [stage][vector][thread]
+  pdl_trigger();
   const int which = (int)blockIdx.x >= q_blocks;
   const int block = which ? blockIdx.x - q_blocks : blockIdx.x, blocks = which ? gridDim.x - q_blocks : q_blocks;
   const HeadRows& t = a.t[which];
   const int lane = threadIdx.x % LANES;
   const HeadRow<D> at(lane, a.rot);
-  const long long rows = (long long)a.B * a.L * t.heads, step = (long long)blocks * ROWS;
-  float w[16], dw[16];
+  const int units = (t.heads + each - 1) / each, tokens = a.B * a.L;
+  const long long all = ((long long)tokens + TOKENS - 1) / TOKENS * units, warps = (long long)blocks * NORM_WARPS;      // turns of the tensor, warps that take them
+  const long long mine = (long long)block * NORM_WARPS + threadIdx.x / 32;
+  const int turns = mine < all ? (int)((all - mine + warps - 1) / warps) : 0, total = turns * each;
+
+  // where a turn's rows are
+  struct Place { int token, l, h0, h1; long long x, g; };
+  auto place = [&](int turn) -> Place {
+    const long long u = mine + turn * warps, tb = u / units;
+    const long long token = tb * TOKENS + threadIdx.x % 32 / LANES;
+    Place p;
+    const bool real = token < tokens;
+    p.token = real ? (int)token : 0;
+    const int b = p.token / a.L;
+    p.l = p.token - b * a.L;
+    p.h0 = (int)(u - tb * units) * each;
+    p.h1 = real ? min(t.heads, p.h0 + each) : 0;
+    p.x = b * t.xb + p.l * t.xl + p.h0 * t.xh;
+    p.g = b * t.gb + p.l * t.gl + p.h0 * t.gh;
+    return p;
+  };
+  Place ahead;
+  int ahead_turn = -1, ahead_i = each;
+  auto fetch = [&](int j) {
+    if (j < total) {
+      if (ahead_i == each) { ahead = place(++ahead_turn); ahead_i = 0; }
+      const bool some = ahead.h0 + ahead_i < ahead.h1;
+      const __nv_bfloat16* x = t.x + (some ? ahead.x + ahead_i * t.xh : 0);
+      const __nv_bfloat16* g = t.dy + (some ? ahead.g + ahead_i * t.gh : 0);
+      uint4* to = slots + (j % GRAD_DEPTH) * 4 * NORM_THREADS + threadIdx.x;
+      fetch16(to, x + at.c0, some);
+      fetch16(to + NORM_THREADS, x + at.c1, some);
+      fetch16(to + 2 * NORM_THREADS, g + at.c0, some);
+      fetch16(to + 3 * NORM_THREADS, g + at.c1, some);
+      ++ahead_i;
+    }
+    fetch_commit();
+  };
+  #pragma unroll
+  for (int j = 0; j < GRAD_DEPTH - 1; ++j) fetch(j);
+  Pairs w, dw;
   load_weight<D>(t.w, t.w32, at, w);
   #pragma unroll
-  for (int i = 0; i < 16; ++i) dw[i] = 0.f;
-  for (long long first = (long long)block * ROWS; first < rows; first += step) {
-    const long long mine = first + threadIdx.x / LANES;
-    const bool real = mine < rows;
-    const long long row = real ? mine : rows - 1;
-    const long long token = row / t.heads;
-    const int h = (int)(row % t.heads), b = (int)(token / a.L), l = (int)(token % a.L);
-    const __nv_bfloat16* xp = t.x + b * t.xb + l * t.xl + h * t.xh;
-    const __nv_bfloat16* gp = t.dy + b * t.gb + l * t.gl + h * t.gh;
-    float x[16], g[16];
-    unpack16(*reinterpret_cast<const uint4*>(xp + at.c0), *reinterpret_cast<const uint4*>(xp + at.c1), x);
-    unpack16(*reinterpret_cast<const uint4*>(gp + at.c0), *reinterpret_cast<const uint4*>(gp + at.c1), g);
-    if (a.rot) {
-      const int p = table_row(a, token, l);
-      if (p < 0) {
+  for (int i = 0; i < 8; ++i) dw[i] = 0;
+  for (int turn = 0, j = 0; turn < turns; ++turn) {
+    const Place p = place(turn);
+    const bool real = p.h1 > 0;
+    __nv_bfloat16* out = t.out + ((long long)p.token * t.heads + p.h0) * D;
+    uint64_t cs[4], sn[4];
+    bool inside = true;
+    if (a.rot && real) inside = load_angles(a, p.token, p.l, at.c0, at.turns, cs, sn);
+    const bool rotates = a.rot && real && inside && at.turns;
+    for (int i = 0; i < each; ++i, ++j) {
+      fetch(j + GRAD_DEPTH - 1);
+      fetch_wait<GRAD_DEPTH - 1>();
+      const uint4* from = slots + (j % GRAD_DEPTH) * 4 * NORM_THREADS + threadIdx.x;
+      Pairs x, g;
+      unpack_pairs(from[0], from[NORM_THREADS], x);
+      unpack_pairs(from[2 * NORM_THREADS], from[3 * NORM_THREADS], g);
+      if (!inside) {
         #pragma unroll
-        for (int i = 0; i < 16; ++i) g[i] = 0.f;
-      } else if (at.turns) {
-        float cs[8], sn[8];
-        load8(a.cs + (long long)p * (a.rot / 2) + at.c0, cs);
-        load8(a.sn + (long long)p * (a.rot / 2) + at.c0, sn);
-        turn16(g, cs, sn, -1.f);
+        for (int k = 0; k < 8; ++k) g[k] = 0;
       }
-    }
-    if (t.w != nullptr) {
-      float ss = 0.f, hx = 0.f;
-      #pragma unroll
-      for (int i = 0; i < 16; ++i) { ss += x[i] * x[i]; hx += g[i] * w[i] * x[i]; }
-      const float r = rsqrtf(row_sum<LANES>(ss) * (1.f / D) + a.eps);
-      const float c = r * r * r * row_sum<LANES>(hx) * (1.f / D);
-      #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (real) dw[i] += g[i] * x[i] * r;
-        g[i] = r * (g[i] * w[i]) - c * x[i];
+      if (rotates) turn_pairs<true>(g, cs, sn);
+      if (t.w != nullptr) {
+        uint64_t ss = mul2(x[0], x[0]), hx = 0;
+        #pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (k) ss = fma2(x[k], x[k], ss);
+          hx = fma2(mul2(g[k], x[k]), w[k], hx);
+        }
+        float r = rms_factor<D>(row_sum<LANES>(pair_sum(ss)), a.eps);
+        if (p.h0 + i >= p.h1) r = 0.f;
+        const float c = r * r * r * row_sum<LANES>(pair_sum(hx)) * (1.f / D);
+        const uint64_t r2 = both(r), c2 = both(-c);
+        #pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          dw[k] = fma2(mul2(g[k], x[k]), r2, dw[k]);
+          g[k] = fma2(mul2(g[k], w[k]), r2, mul2(x[k], c2));
+        }
       }
-    }
-    if (real) {
-      __nv_bfloat16* o = t.out + row * D;
-      *reinterpret_cast<uint4*>(o + at.c0) = pack8(g);
-      *reinterpret_cast<uint4*>(o + at.c1) = pack8(g + 8);
+      if (p.h0 + i < p.h1) {
+        *reinterpret_cast<uint4*>(out + i * D + at.c0) = pack_pairs(g);
+        *reinterpret_cast<uint4*>(out + i * D + at.c1) = pack_pairs(g + 4);
+      }
     }
   }
   if (t.w == nullptr) return;
   __shared__ float sums[8][D];
   // the rows of a warp, then the warps one after the other: the same order at every run
   #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < 8; ++i) {
+    float lo, hi;
+    unpack2(dw[i], lo, hi);
     #pragma unroll
-    for (int o = LANES; o < 32; o <<= 1) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
-  }
-  if (threadIdx.x % 32 < LANES) {
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sums[threadIdx.x / 32][at.c0 + i] = dw[i];
-      sums[threadIdx.x / 32][at.c1 + i] = dw[8 + i];
+    for (int o = LANES; o < 32; o <<= 1) { lo += __shfl_xor_sync(0xffffffffu, lo, o); hi += __shfl_xor_sync(0xffffffffu, hi, o); }
+    if (threadIdx.x % 32 < LANES) {
+      const int c = (i < 4 ? at.c0 : at.c1 - 8) + 2 * i;
+      sums[threadIdx.x / 32][c] = lo;
+      sums[threadIdx.x / 32][c + 1] = hi;
     }
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < D; c += 256) {
+  for (int c = threadIdx.x; c < D; c += NORM_THREADS) {
     float s = 0.f;
     #pragma unroll
     for (int k = 0; k < 8; ++k) s += sums[k][c];
@@ -158,26 +219,28 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(const NormArgs a, int 
   }
 }
 
-// dw of queries (block 0) and keys (block 1) from the blocks' sums, in the blocks' order; stored, or added to what is there.
+// dw of queries (blockIdx.y 0) and keys (1) from the blocks' sums, in their order: 32 columns, 32 groups of blocks.  Stored, or added to what is there.
 struct WeightGrads { void* dst[2]; int is32[2], add[2]; };
-__global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float* __restrict__ part, int q_blocks, int blocks, int D, WeightGrads o) {
-  __shared__ float sums[1024];
-  const int which = blockIdx.x, groups = 1024 / D, c = threadIdx.x % D, g = threadIdx.x / D;
+__global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float* part, int q_blocks, int blocks, int D, WeightGrads o) {
+  __shared__ float sums[32][33];
+  const int which = blockIdx.y, c = threadIdx.x % 32, g = threadIdx.x / 32, col = blockIdx.x * 32 + c;
   if (o.dst[which] == nullptr) return;
+  pdl_wait();
   const int lo = which ? q_blocks : 0, hi = which ? blocks : q_blocks;
   float s = 0.f;
   #pragma unroll 4
-  for (int k = lo + g; k < hi; k += groups) s += part[(long long)k * D + c];
-  sums[threadIdx.x] = s;
+  for (int k = lo + g; k < hi; k += 32) s += part[(long long)k * D + col];
+  sums[g][c] = s;
   __syncthreads();
   if (g != 0) return;
   s = 0.f;
-  for (int k = 0; k < groups; ++k) s += sums[k * D + c];
+  #pragma unroll
+  for (int k = 0; k < 32; ++k) s += sums[k][c];
   if (o.is32[which]) {
-    float* p = reinterpret_cast<float*>(o.dst[which]) + c;
+    float* p = reinterpret_cast<float*>(o.dst[which]) + col;
     *p = o.add[which] ? *p + s : s;
   } else {
-    reinterpret_cast<__nv_bfloat16*>(o.dst[which])[c] = __float2bfloat16(s);
+    reinterpret_cast<__nv_bfloat16*>(o.dst[which])[col] = __float2bfloat16(s);
   }
 }
 
@@ -187,7 +250,7 @@ static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 static int norm_args(NormArgs* a, const void* q, const void* k, const void* dq, const void* dk, const long long* strides, void* qo, void* ko,
                      const void* qw, const void* kw, int qw32, int kw32, const void* cs, const void* sn, const void* positions, int pos64,
                      int B, int L, int Hq, int Hk, int D, int rot, int table_rows, float eps, int* status) {
-  if (B < 1 || L < 1 || Hq < 0 || Hk < 0 || Hq + Hk < 1 || (D != 64 && D != 128 && D != 256) || rot < 0 || rot % 16 || rot > D) return -SSM_ERR_BAD_ARG;
+  if (B < 1 || L < 1 || (long long)B * L > 0x7fffffffll || Hq < 0 || Hk < 0 || Hq + Hk < 1 || (D != 64 && D != 128 && D != 256) || rot < 0 || rot % 16 || rot > D) return -SSM_ERR_BAD_ARG;
   const void* all[] = {q, k, dq, dk, qo, ko, qw, kw, cs, sn};
   for (const void* p : all) if (!aligned16(p)) return -SSM_ERR_BAD_ARG;
   for (int i = 0; i < (dq != nullptr || dk != nullptr ? 12 : 6); ++i) if (strides[i] % 8) return -SSM_ERR_BAD_ARG;
@@ -208,9 +271,42 @@ static int norm_args(NormArgs* a, const void* q, const void* k, const void* dq, 
   return 0;
 }
 
-static unsigned norm_grid(long long rows, int D) {
-  const long long blocks = (rows + 256 / (D / 16) - 1) / (256 / (D / 16));
-  return (unsigned)(blocks < 148 * 8 ? blocks : 148 * 8);
+// Heads that a warp takes one after the other: 8, or fewer where that would leave less than three blocks per SM.
+static long long norm_turns(long long tokens, int heads, int each, int D) { return (tokens * (D / 16) + 31) / 32 * ((heads + each - 1) / each); }
+static int heads_each(long long tokens, int Hq, int Hk, int D) {
+  for (int each = EACH; each > 1; each /= 2)
+    if (norm_turns(tokens, Hq, each, D) + norm_turns(tokens, Hk, each, D) >= 148ll * 3 * NORM_WARPS) return each;
+  return 1;
+}
+struct GradPlan { int each, q_blocks, blocks; };
+static GradPlan grad_plan(long long tokens, int Hq, int Hk, int D) {
+  GradPlan p;
+  p.each = heads_each(tokens, Hq, Hk, D);
+  const long long uq = norm_turns(tokens, Hq, p.each, D), uk = norm_turns(tokens, Hk, p.each, D);
+  const long long want = (uq + uk + NORM_WARPS - 1) / NORM_WARPS, most = 148 * 2;              // what runs at once
+  const long long all = want < most ? want : most;
+  long long q = uq + uk > 0 ? (all * uq + (uq + uk) / 2) / (uq + uk) : 0;
+  if (Hq > 0 && q < 1) q = 1;
+  if (Hk > 0 && q > all - 1 && all > 1) q = all - 1;
+  const long long k = Hk == 0 ? 0 : all - q < 1 ? 1 : all - q;
+  p.q_blocks = (int)q;
+  p.blocks = (int)(q + k);
+  return p;
+}
+template <int D>
+static int norm_fwd_launch(const NormArgs& a, unsigned grid, int each, cudaStream_t st) {
+  static SmemOptIn opt;
+  if (int e = opt.ask(reinterpret_cast<const void*>(qk_norm_fwd_kernel<D>), EACH * 2 * NORM_THREADS * 16)) return e;
+  qk_norm_fwd_kernel<D><<<grid, NORM_THREADS, each * 2 * NORM_THREADS * 16, st>>>(a, each);
+  return (int)cudaGetLastError();
+}
+template <int D>
+static int norm_bwd_launch(const NormArgs& a, const GradPlan& n, float* part, cudaStream_t st) {
+  constexpr int SMEM = GRAD_DEPTH * 4 * NORM_THREADS * 16;
+  static SmemOptIn opt;
+  if (int e = opt.ask(reinterpret_cast<const void*>(qk_norm_bwd_kernel<D>), SMEM)) return e;
+  qk_norm_bwd_kernel<D><<<n.blocks, NORM_THREADS, SMEM, st>>>(a, n.q_blocks, n.each, part);
+  return (int)cudaGetLastError();
 }
 
 }  // namespace ssm
@@ -224,25 +320,16 @@ extern "C" int ssm_qk_norm_fwd(const void* q, const void* k, const long long* st
   const int bad = norm_args(&a, q, k, nullptr, nullptr, strides, qo, ko, qw, kw, qw32, kw32, cs, sn, positions, pos64, B, L, Hq, Hk, D,
                             rot, table_rows, eps, status);
   if (bad) return bad;
-  const unsigned grid = norm_grid((long long)B * L * (Hq + Hk), D);
-  if (D == 64) qk_norm_fwd_kernel<64><<<grid, 256, 0, st>>>(a);
-  else if (D == 128) qk_norm_fwd_kernel<128><<<grid, 256, 0, st>>>(a);
-  else qk_norm_fwd_kernel<256><<<grid, 256, 0, st>>>(a);
-  return (int)cudaGetLastError();
+  const int each = heads_each((long long)B * L, Hq, Hk, D);
+  const long long warps = norm_turns((long long)B * L, Hq, each, D) + norm_turns((long long)B * L, Hk, each, D);
+  const long long grid = (warps + NORM_WARPS - 1) / NORM_WARPS;
+  if (grid > 0x7fffffffll) return -SSM_ERR_BAD_ARG;
+  return D == 64 ? norm_fwd_launch<64>(a, (unsigned)grid, each, st) : D == 128 ? norm_fwd_launch<128>(a, (unsigned)grid, each, st)
+                                                                              : norm_fwd_launch<256>(a, (unsigned)grid, each, st);
 }
 
-// Blocks of the backward pass: {queries', all}; the caller's buffer of partial sums has all * D floats.
-extern "C" int ssm_qk_norm_bwd_blocks(long long tokens, int Hq, int Hk, int D, int* out2) {
-  const long long all = norm_grid(tokens * (Hq + Hk), D);
-  long long mine = (all * Hq + (Hq + Hk) / 2) / (Hq + Hk);
-  if (Hq > 0 && mine < 1) mine = 1;
-  long long theirs = all - mine;
-  if (Hk > 0 && theirs < 1) theirs = 1;
-  if (Hk == 0) theirs = 0;
-  out2[0] = (int)mine;
-  out2[1] = (int)(mine + theirs);
-  return 0;
-}
+// Blocks of the backward pass; the caller's buffer of partial sums has that many times D floats.
+extern "C" int ssm_qk_norm_bwd_blocks(long long tokens, int Hq, int Hk, int D) { return grad_plan(tokens, Hq, Hk, D).blocks; }
 
 // dwq, dwk: gradients of the weights, fp32 or bf16 (null: none wanted), stored or (fp32) added to.
 extern "C" int ssm_qk_norm_bwd(const void* q, const void* k, const void* dq, const void* dk, const long long* strides, void* dxq, void* dxk,
@@ -254,13 +341,11 @@ extern "C" int ssm_qk_norm_bwd(const void* q, const void* k, const void* dq, con
                             table_rows, eps, status);
   if (bad) return bad;
   if ((addq && !dq32) || (addk && !dk32)) return -SSM_ERR_BAD_ARG;
-  int blocks[2];
-  ssm_qk_norm_bwd_blocks((long long)B * L, Hq, Hk, D, blocks);
+  const GradPlan n = grad_plan((long long)B * L, Hq, Hk, D);
   float* p = reinterpret_cast<float*>(part);
-  if (D == 64) qk_norm_bwd_kernel<64><<<blocks[1], 256, 0, st>>>(a, blocks[0], p);
-  else if (D == 128) qk_norm_bwd_kernel<128><<<blocks[1], 256, 0, st>>>(a, blocks[0], p);
-  else qk_norm_bwd_kernel<256><<<blocks[1], 256, 0, st>>>(a, blocks[0], p);
-  if (dwq != nullptr || dwk != nullptr)
-    qk_norm_dw_kernel<<<2, 1024, 0, st>>>(p, blocks[0], blocks[1], D, WeightGrads{{dwq, dwk}, {dq32, dk32}, {addq, addk}});
-  return (int)cudaGetLastError();
+  const int e = D == 64 ? norm_bwd_launch<64>(a, n, p, st) : D == 128 ? norm_bwd_launch<128>(a, n, p, st) : norm_bwd_launch<256>(a, n, p, st);
+  if (e) return e;
+  if (dwq == nullptr && dwk == nullptr) return 0;
+  return launch_dependent(qk_norm_dw_kernel, dim3(D / 32, 2), dim3(1024), 0, st, p, n.q_blocks, n.blocks, D,
+                          WeightGrads{{dwq, dwk}, {dq32, dk32}, {addq, addk}});
 }

@@ -1447,9 +1447,7 @@ class _QKNormRotary(torch.autograd.Function):
             adds.append(0)
         if not (B and L):
             return dq, dk, *[None if t is None else t.zero_() for t in grads], None, None, None, None
-        blocks = (_c.c_int * 2)()
-        _lib().ssm_qk_norm_bwd_blocks(_ll(B * L), Hq, Hk, D, blocks)
-        part = torch.empty(blocks[1], D, dtype=torch.float32, device=dev)
+        part = torch.empty(_lib().ssm_qk_norm_bwd_blocks(_ll(B * L), Hq, Hk, D), D, dtype=torch.float32, device=dev)
         _run("ssm_qk_norm_bwd", _p(q2), _p(k2), _p(g), _p(h), _strides(*ctx.strides, gs, hs), _p(dq), _p(dk), _p(_aligned(qw)),
              _p(_aligned(kw)), _is32(qw), _is32(kw), _p(cos), _p(sin), _p(positions),
              int(positions is not None and positions.dtype == torch.int64), B, L, Hq, Hk, D, 0 if cos is None else 2 * cos.shape[1],
