@@ -2,7 +2,8 @@
 //
 // A head's row of D channels belongs to D / 16 neighbouring lanes, 16 channels each, as two vectors of 8.  The rotation pairs
 // channel i with i + R / 2 (R = rotary dim, a multiple of 16): lane j < R / 16 holds the vectors j and j + R / 16, so that both
-// halves of its pairs are in its registers; the other lanes hold two neighbouring vectors of what is not rotated.
+// halves of its pairs are in its registers; the other lanes hold such vectors of what is not rotated.  Neighbouring lanes access
+// neighbouring vectors.
 #pragma once
 #include "common.cuh"
 
@@ -16,8 +17,8 @@ struct HeadRow {
   __device__ __forceinline__ HeadRow(int lane, int rot) {
     const int pairs = rot / 16;
     turns = lane < pairs;
-    c0 = turns ? lane * 8 : rot + (lane - pairs) * 16;
-    c1 = turns ? c0 + rot / 2 : c0 + 8;
+    c0 = turns ? lane * 8 : rot + (lane - pairs) * 8;
+    c1 = c0 + (turns ? rot / 2 : (D - rot) / 2);
   }
 };
 

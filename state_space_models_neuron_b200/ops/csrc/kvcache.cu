@@ -73,23 +73,34 @@ __global__ void __launch_bounds__(KV_THREADS, 3) kv_write_kernel(const WriteArgs
   const bool exists = mine < (long long)a.B * a.L;
   const int token = exists ? (int)mine : 0;
   const int b = token / a.L, l = token - b * a.L, h0 = part * each, h1 = exists ? min(a.heads[which], h0 + each) : 0;
+  const int given = a.counts == nullptr ? a.L : a.counts[b];
+  const int count = given < 0 ? 0 : given > a.L ? a.L : given, h2 = l < count ? h1 : h0;        // padding is not read
   const __nv_bfloat16* x = a.x[which] + b * a.sb[which] + l * a.sl[which] + h0 * a.sh[which];
   for (int i = 0; i < each; ++i) {
-    const __nv_bfloat16* src = h0 + i < h1 ? x + i * a.sh[which] : x;
-    fetch16(slots + (i * 2) * KV_THREADS + threadIdx.x, src + at.c0, h0 + i < h1);
-    fetch16(slots + (i * 2 + 1) * KV_THREADS + threadIdx.x, src + at.c1, h0 + i < h1);
+    const __nv_bfloat16* src = h0 + i < h2 ? x + i * a.sh[which] : x;
+    fetch16(slots + (i * 2) * KV_THREADS + threadIdx.x, src + at.c0, h0 + i < h2);
+    fetch16(slots + (i * 2 + 1) * KV_THREADS + threadIdx.x, src + at.c1, h0 + i < h2);
     if (i == each / 2 - 1) fetch_commit();
   }
   fetch_commit();
   // where the token goes
-  const int given = a.counts == nullptr ? a.L : a.counts[b];
-  const int count = given < 0 ? 0 : given > a.L ? a.L : given;
   if (count != given) report_bad_index(a.table.status);
   const int pos = a.table.lengths[b] - count + l;
   int page = -1;
   if (l < count && pos >= 0) {
     page = page_of(a.table, b, pos);
     if (a.rot && pos >= a.table_rows) { report_bad_index(a.table.status); page = -1; }
+  }
+  if (!__any_sync(0xffffffffu, page >= 0)) {
+    // padding: only queries leave something
+    fetch_wait<0>();
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (int i = h0; which == 0 && i < h1; ++i) {
+      __nv_bfloat16* o = a.qo + ((long long)token * a.heads[0] + i) * D;
+      *reinterpret_cast<uint4*>(o + at.c0) = zero;
+      *reinterpret_cast<uint4*>(o + at.c1) = zero;
+    }
+    return;
   }
   const void* weight = which < 2 ? a.w[which] : nullptr;
   const bool turns = which < 2 && page >= 0 && at.turns;
@@ -147,33 +158,33 @@ __global__ void __launch_bounds__(KV_THREADS, 3) kv_write_kernel(const WriteArgs
   }
 }
 
-// A block takes rows (token, head) of one sequence, D / 16 lanes a row of keys and the same of values, two rows under way.
-constexpr int READ_ROWS = 2;
+// A block takes rows (token, head) of one sequence, D / 8 lanes a row of keys and the same of values, READ_ROWS rows of a thread under
+// way.  A lane has 8 channels, so that what neighbours store is contiguous (16 channels each, stored as two vectors 32 bytes
+// apart: 16 x 2048 int8 45.7 us).
+constexpr int READ_ROWS = 4;
+template <int BYTES> struct ReadVector { using Type = uint2; };
+template <> struct ReadVector<2> { using Type = uint4; };
 template <int D, int T, typename Out>
-__global__ void __launch_bounds__(KV_THREADS, 5) kv_read_kernel(const void* __restrict__ pages0, const void* __restrict__ pages1, const float* __restrict__ scale0,
-                                                                const float* __restrict__ scale1, Out* __restrict__ out0, Out* __restrict__ out1,
-                                                                PageTable table, int most, int heads) {
-  constexpr int LANES = D / 16, GROUPS = KV_THREADS / LANES, VECS = T == KV_BF16 ? 2 : 1;
+__global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const uint8_t* __restrict__ pages0, const uint8_t* __restrict__ pages1, const float* __restrict__ scale0,
+                                                             const float* __restrict__ scale1, Out* __restrict__ out0, Out* __restrict__ out1,
+                                                             PageTable table, int most, int heads) {
+  using Vector = typename ReadVector<KvType<T>::BYTES>::Type;
+  constexpr int LANES = D / 8, GROUPS = KV_THREADS / LANES;
   const int lane = threadIdx.x % LANES, b = blockIdx.y, n = table.lengths[b];
   const unsigned rows = (unsigned)most * heads, first = blockIdx.x * (GROUPS * READ_ROWS) + threadIdx.x / LANES;
-  uint4 u[READ_ROWS][2][VECS];
+  Vector u[READ_ROWS][2];
   float s[READ_ROWS][2];
   #pragma unroll
   for (int i = 0; i < READ_ROWS; ++i) {
     const unsigned row = first + i * GROUPS;
     const int p = row / heads, h = row - p * heads;
-    #pragma unroll
-    for (int k = 0; k < VECS; ++k) u[i][0][k] = u[i][1][k] = make_uint4(0, 0, 0, 0);
+    u[i][0] = u[i][1] = Vector{};
     s[i][0] = s[i][1] = 0.f;
     const int page = row < rows && p < n ? page_of(table, b, p) : -1;
     if (page < 0) continue;
     const long long slot = (((long long)page * heads + h) << table.page_shift) + (p & ((1 << table.page_shift) - 1));
-    const long long at = (slot * D + lane * 16) * KvType<T>::BYTES;
-    #pragma unroll
-    for (int k = 0; k < VECS; ++k) {
-      u[i][0][k] = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(pages0) + at)[k];
-      u[i][1][k] = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(pages1) + at)[k];
-    }
+    u[i][0] = reinterpret_cast<const Vector*>(pages0)[slot * LANES + lane];
+    u[i][1] = reinterpret_cast<const Vector*>(pages1)[slot * LANES + lane];
     if (T != KV_BF16) { s[i][0] = scale0[slot]; s[i][1] = scale1[slot]; }
   }
   #pragma unroll
@@ -182,33 +193,33 @@ __global__ void __launch_bounds__(KV_THREADS, 5) kv_read_kernel(const void* __re
     if (row >= rows) break;
     #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      Out* o = (j ? out1 : out0) + ((long long)b * rows + row) * D + lane * 16;
-      if (T == KV_BF16 && sizeof(Out) == 2) {
-        reinterpret_cast<uint4*>(o)[0] = u[i][j][0];
-        reinterpret_cast<uint4*>(o)[1] = u[i][j][VECS - 1];
-        continue;
-      }
-      Pairs y;
-      if (T == KV_BF16) {
-        unpack_pairs(u[i][j][0], u[i][j][VECS - 1], y);
-      } else {
-        const uint32_t words[4] = {u[i][j][0].x, u[i][j][0].y, u[i][j][0].z, u[i][j][0].w};
-        const uint64_t s2 = both(s[i][j]);
+      Out* o = (j ? out1 : out0) + ((long long)b * rows + row) * D + lane * 8;
+      uint32_t words[4] = {u[i][j].x, u[i][j].y, 0, 0};
+      uint64_t y[4];
+      if constexpr (T == KV_BF16) {
+        if (sizeof(Out) == 2) {
+          *reinterpret_cast<Vector*>(o) = u[i][j];
+          continue;
+        }
+        words[2] = u[i][j].z;
+        words[3] = u[i][j].w;
         #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 4; ++k) y[k] = bf16x2_pair(words[k]);
+      } else {
+        #pragma unroll
+        for (int k = 0; k < 2; ++k) {
           uint32_t lo, hi;
           widen4<T>(words[k], lo, hi);
           const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&lo)), g = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-          y[2 * k] = mul2(pack2(f.x, f.y), s2);
-          y[2 * k + 1] = mul2(pack2(g.x, g.y), s2);
+          y[2 * k] = mul2(pack2(f.x, f.y), both(s[i][j]));
+          y[2 * k + 1] = mul2(pack2(g.x, g.y), both(s[i][j]));
         }
       }
       if (sizeof(Out) == 2) {
-        reinterpret_cast<uint4*>(o)[0] = pack_pairs(y);
-        reinterpret_cast<uint4*>(o)[1] = pack_pairs(y + 4);
+        *reinterpret_cast<uint4*>(o) = pack_pairs(y);
       } else {
-        #pragma unroll
-        for (int k = 0; k < 4; ++k) reinterpret_cast<ulonglong2*>(o)[k] = make_ulonglong2(y[2 * k], y[2 * k + 1]);
+        reinterpret_cast<ulonglong2*>(o)[0] = make_ulonglong2(y[0], y[1]);
+        reinterpret_cast<ulonglong2*>(o)[1] = make_ulonglong2(y[2], y[3]);
       }
     }
   }
@@ -231,60 +242,80 @@ static int kv_write_launch(const WriteArgs& a, int Hq, int Hk, cudaStream_t st) 
   return (int)cudaGetLastError();
 }
 
+template <int D, int T, typename Out>
+static int kv_read_launch(const void* kp, const void* vp, const void* ks, const void* vs, void* ko, void* vo, const PageTable& t, dim3 grid, int most, int Hk,
+                          cudaStream_t st) {
+  kv_read_kernel<D, T, Out><<<grid, KV_THREADS, 0, st>>>(
+      reinterpret_cast<const uint8_t*>(kp), reinterpret_cast<const uint8_t*>(vp), reinterpret_cast<const float*>(ks), reinterpret_cast<const float*>(vs),
+      reinterpret_cast<Out*>(ko), reinterpret_cast<Out*>(vo), t, most, Hk);
+  return (int)cudaGetLastError();
+}
+
 }  // namespace ssm
 
 using namespace ssm;
 
-// strides: (batch, token, head) of queries, keys and values
-extern "C" int ssm_kv_write(const void* q, const void* k, const void* v, const long long* strides, void* qo, const void* qw, const void* kw,
-                            int qw32, int kw32, const void* cs, const void* sn, int rot, int table_rows, float eps, void* kp, void* vp,
-                            void* ks, void* vs, int type, int pages, int page_size, const void* table, int width, const void* lengths,
-                            const void* counts, int B, int L, int Hq, int Hk, int D, int* status, cudaStream_t st) {
+struct KvWriteCall {                           // in the order in which cuda_ops packs it
+  const void *q, *k, *v;
+  void* qo;
+  const void *qw, *kw, *cs, *sn;
+  void *kp, *vp, *ks, *vs;
+  const void *table, *lengths, *counts;
+  int* status;
+  long long strides[9];                        // (batch, token, head) of q, k, v
+  int qw32, kw32, rot, table_rows, type, pages, page_size, width, B, L, Hq, Hk, D;
+  float eps;
+};
+extern "C" int ssm_kv_write(const KvWriteCall* c, cudaStream_t st) {
   WriteArgs a;
-  if (!kv_table(&a.table, table, lengths, width, pages, page_size, status)) return -SSM_ERR_BAD_ARG;
-  if (B < 1 || L < 1 || (long long)B * L > 0x7fffffffll || Hq < 0 || Hk < 1 || rot < 0 || rot % 16 || rot > D) return -SSM_ERR_BAD_ARG;
-  const void* all[] = {q, k, v, qo, qw, kw, cs, sn, kp, vp};
+  const int D = c->D, type = c->type;
+  if (!kv_table(&a.table, c->table, c->lengths, c->width, c->pages, c->page_size, c->status)) return -SSM_ERR_BAD_ARG;
+  if (c->B < 1 || c->L < 1 || (long long)c->B * c->L > 0x7fffffffll || c->Hq < 0 || c->Hk < 1 || c->rot < 0 || c->rot % 16 || c->rot > D ||
+      (c->rot && (c->cs == nullptr || c->sn == nullptr)) || (type != KV_BF16 && (c->ks == nullptr || c->vs == nullptr)))
+    return -SSM_ERR_BAD_ARG;
+  const void* all[] = {c->q, c->k, c->v, c->qo, c->qw, c->kw, c->cs, c->sn, c->kp, c->vp};
   for (const void* p : all) if (!kv_aligned(p)) return -SSM_ERR_BAD_ARG;
-  for (int i = 0; i < 9; ++i) if (strides[i] % 8) return -SSM_ERR_BAD_ARG;
-  const void* x[3] = {q, k, v};
-  const int heads[3] = {Hq, Hk, Hk};
+  for (int i = 0; i < 9; ++i) if (c->strides[i] % 8) return -SSM_ERR_BAD_ARG;
+  const int heads[3] = {c->Hq, c->Hk, c->Hk};
   for (int i = 0; i < 3; ++i) {
-    a.x[i] = reinterpret_cast<const __nv_bfloat16*>(x[i]);
-    a.sb[i] = strides[3 * i]; a.sl[i] = strides[3 * i + 1]; a.sh[i] = strides[3 * i + 2];
+    a.x[i] = reinterpret_cast<const __nv_bfloat16*>(all[i]);
+    a.sb[i] = c->strides[3 * i]; a.sl[i] = c->strides[3 * i + 1]; a.sh[i] = c->strides[3 * i + 2];
     a.heads[i] = heads[i];
   }
-  a.w[0] = qw; a.w[1] = kw; a.w32[0] = qw32; a.w32[1] = kw32;
-  a.qo = reinterpret_cast<__nv_bfloat16*>(qo);
-  a.pages[0] = kp; a.pages[1] = vp;
-  a.scales[0] = reinterpret_cast<float*>(ks); a.scales[1] = reinterpret_cast<float*>(vs);
-  a.counts = reinterpret_cast<const int*>(counts);
-  a.cs = reinterpret_cast<const float*>(cs); a.sn = reinterpret_cast<const float*>(sn);
-  a.B = B; a.L = L; a.rot = rot; a.table_rows = table_rows; a.eps = eps;
-  #define WRITE(DD, TT) return kv_write_launch<DD, TT>(a, Hq, Hk, st)
+  a.w[0] = c->qw; a.w[1] = c->kw; a.w32[0] = c->qw32; a.w32[1] = c->kw32;
+  a.qo = reinterpret_cast<__nv_bfloat16*>(c->qo);
+  a.pages[0] = c->kp; a.pages[1] = c->vp;
+  a.scales[0] = reinterpret_cast<float*>(c->ks); a.scales[1] = reinterpret_cast<float*>(c->vs);
+  a.counts = reinterpret_cast<const int*>(c->counts);
+  a.cs = reinterpret_cast<const float*>(c->cs); a.sn = reinterpret_cast<const float*>(c->sn);
+  a.B = c->B; a.L = c->L; a.rot = c->rot; a.table_rows = c->table_rows; a.eps = c->eps;
+  #define WRITE(DD, TT) return kv_write_launch<DD, TT>(a, c->Hq, c->Hk, st)
   KV_DISPATCH(WRITE);
   #undef WRITE
   return -SSM_ERR_BAD_ARG;
 }
 
-extern "C" int ssm_kv_read(const void* kp, const void* vp, const void* ks, const void* vs, int type, int pages, int page_size, const void* table,
-                           int width, const void* lengths, void* ko, void* vo, int out32, int B, int most, int Hk, int D, int* status,
-                           cudaStream_t st) {
+struct KvReadCall {                            // in the order in which cuda_ops packs it
+  const void *kp, *vp, *ks, *vs, *table, *lengths;
+  void *ko, *vo;
+  int* status;
+  int type, pages, page_size, width, out32, B, most, Hk, D;
+};
+extern "C" int ssm_kv_read(const KvReadCall* c, cudaStream_t st) {
   PageTable t;
-  if (!kv_table(&t, table, lengths, width, pages, page_size, status)) return -SSM_ERR_BAD_ARG;
-  if (B < 1 || most < 1 || Hk < 1 || !kv_aligned(kp) || !kv_aligned(vp) || !kv_aligned(ko) || !kv_aligned(vo)) return -SSM_ERR_BAD_ARG;
-  if (B > 65535 || (long long)most * Hk > 0x7fffffffll || (D != 64 && D != 128 && D != 256)) return -SSM_ERR_BAD_ARG;
-  const long long per = KV_THREADS / (D / 16) * READ_ROWS;
-  const dim3 grid((unsigned)(((long long)most * Hk + per - 1) / per), B);
-  const float* s0 = reinterpret_cast<const float*>(ks);
-  const float* s1 = reinterpret_cast<const float*>(vs);
-  #define READ(DD, TT)                                                                                                             \
-    do {                                                                                                                           \
-      if (out32) kv_read_kernel<DD, TT, float><<<grid, KV_THREADS, 0, st>>>(kp, vp, s0, s1, reinterpret_cast<float*>(ko),                 \
-                                                                     reinterpret_cast<float*>(vo), t, most, Hk);                   \
-      else kv_read_kernel<DD, TT, __nv_bfloat16><<<grid, KV_THREADS, 0, st>>>(kp, vp, s0, s1, reinterpret_cast<__nv_bfloat16*>(ko),       \
-                                                                       reinterpret_cast<__nv_bfloat16*>(vo), t, most, Hk);         \
+  const int D = c->D, type = c->type;
+  if (!kv_table(&t, c->table, c->lengths, c->width, c->pages, c->page_size, c->status)) return -SSM_ERR_BAD_ARG;
+  if (c->B < 1 || c->B > 65535 || c->most < 1 || c->Hk < 1 || (long long)c->most * c->Hk > 0x7fffffffll || (D != 64 && D != 128 && D != 256) ||
+      !kv_aligned(c->kp) || !kv_aligned(c->vp) || !kv_aligned(c->ko) || !kv_aligned(c->vo) || (type != KV_BF16 && (c->ks == nullptr || c->vs == nullptr)))
+    return -SSM_ERR_BAD_ARG;
+  const long long per = KV_THREADS / (D / 8) * READ_ROWS;
+  const dim3 grid((unsigned)(((long long)c->most * c->Hk + per - 1) / per), c->B);
+  #define READ(DD, TT)                                                                                                                    \
+    do {                                                                                                                                  \
+      if (c->out32) return kv_read_launch<DD, TT, float>(c->kp, c->vp, c->ks, c->vs, c->ko, c->vo, t, grid, c->most, c->Hk, st);           \
+      return kv_read_launch<DD, TT, __nv_bfloat16>(c->kp, c->vp, c->ks, c->vs, c->ko, c->vo, t, grid, c->most, c->Hk, st);                 \
     } while (0)
   KV_DISPATCH(READ);
   #undef READ
-  return (int)cudaGetLastError();
+  return -SSM_ERR_BAD_ARG;
 }

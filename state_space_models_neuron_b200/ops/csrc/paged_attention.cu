@@ -773,28 +773,38 @@ extern "C" long long ssm_paged_attn_workspace(int type, int width, int page_size
   return e ? (e < 0 ? e : -e) : floats;
 }
 
-extern "C" int ssm_paged_attn(const void* q, long long qb, long long qh, void* out, const void* kp, const void* vp, const void* ks, const void* vs,
-                              int type, int pages, int page_size, const void* table, int width, const void* lengths, int B, int Hq, int Hk,
-                              int D, float scale, void* ws, long long ws_floats, int* status, cudaStream_t st) {
+struct PagedAttnCall {                         // in the order in which cuda_ops packs it
+  const void* q; void* out;
+  const void *kp, *vp, *ks, *vs, *table, *lengths;
+  void* ws;
+  int* status;
+  long long qb, qh, ws_floats;                 // strides of q; floats of ws
+  int type, pages, page_size, width, B, Hq, Hk, D;
+  float scale;
+};
+extern "C" int ssm_paged_attn(const PagedAttnCall* c, cudaStream_t st) {
   AttnArgs a;
-  if (!kv_table(&a.table, table, lengths, width, pages, page_size, status)) return -SSM_ERR_BAD_ARG;
-  if (B < 1 || Hk < 1 || Hq < Hk || Hq % Hk || qb % 8 || qh % 8 || !kv_aligned(q) || !kv_aligned(out) || !kv_aligned(kp) || !kv_aligned(vp) || !kv_aligned(ws))
+  const int D = c->D, type = c->type;
+  if (!kv_table(&a.table, c->table, c->lengths, c->width, c->pages, c->page_size, c->status)) return -SSM_ERR_BAD_ARG;
+  const void* all[] = {c->q, c->out, c->kp, c->vp, c->ks, c->vs, c->ws};
+  for (const void* p : all) if (!kv_aligned(p)) return -SSM_ERR_BAD_ARG;
+  if (c->B < 1 || c->Hk < 1 || c->Hq < c->Hk || c->Hq % c->Hk || c->qb % 8 || c->qh % 8 || c->pages < 1 ||
+      (long long)c->pages * c->Hk * c->page_size > 0x7fffffffll || (type != KV_BF16 && (c->ks == nullptr || c->vs == nullptr)))
     return -SSM_ERR_BAD_ARG;
-  if (pages < 1 || (long long)pages * Hk * page_size > 0x7fffffffll || !kv_aligned(ks) || !kv_aligned(vs)) return -SSM_ERR_BAD_ARG;
   int grid = 0;
   long long floats = 0;
-  if (int e = paged_attn_plan(type, width, page_size, B, Hq, Hk, D, &grid, &a.most_blocks, &floats)) return e;
-  if (ws_floats < floats) return -SSM_ERR_BAD_ARG;
-  a.q = reinterpret_cast<const __nv_bfloat16*>(q);
-  a.out = reinterpret_cast<__nv_bfloat16*>(out);
-  a.qb = qb; a.qh = qh;
-  a.pages[0] = reinterpret_cast<const uint8_t*>(kp); a.pages[1] = reinterpret_cast<const uint8_t*>(vp);
-  a.scales[0] = reinterpret_cast<const float*>(ks); a.scales[1] = reinterpret_cast<const float*>(vs);
-  a.B = B; a.Hq = Hq; a.Hk = Hk; a.ratio = Hq / Hk;
+  if (int e = paged_attn_plan(type, c->width, c->page_size, c->B, c->Hq, c->Hk, D, &grid, &a.most_blocks, &floats)) return e;
+  if (c->ws_floats < floats) return -SSM_ERR_BAD_ARG;
+  a.q = reinterpret_cast<const __nv_bfloat16*>(c->q);
+  a.out = reinterpret_cast<__nv_bfloat16*>(c->out);
+  a.qb = c->qb; a.qh = c->qh;
+  a.pages[0] = reinterpret_cast<const uint8_t*>(c->kp); a.pages[1] = reinterpret_cast<const uint8_t*>(c->vp);
+  a.scales[0] = reinterpret_cast<const float*>(c->ks); a.scales[1] = reinterpret_cast<const float*>(c->vs);
+  a.B = c->B; a.Hq = c->Hq; a.Hk = c->Hk; a.ratio = c->Hq / c->Hk;
   const bool two = two_tiles(a.ratio, D);
   a.groups = (a.ratio + (two ? 15 : 7)) / (two ? 16 : 8);
-  a.scale = scale * 1.4426950408889634f;
-  a.ws = reinterpret_cast<float*>(ws);
+  a.scale = c->scale * 1.4426950408889634f;
+  a.ws = reinterpret_cast<float*>(c->ws);
   using Pool = ScratchPool<SCRATCH_ATTENTION>;
   Pool& pool = Pool::get();
   std::lock_guard<std::mutex> hold(pool.lock);

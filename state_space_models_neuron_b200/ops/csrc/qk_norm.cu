@@ -246,28 +246,35 @@ __global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float* part, int
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// strides: q's (batch, token, head), k's, then for the backward pass dq's and dk's
-static int norm_args(NormArgs* a, const void* q, const void* k, const void* dq, const void* dk, const long long* strides, void* qo, void* ko,
-                     const void* qw, const void* kw, int qw32, int kw32, const void* cs, const void* sn, const void* positions, int pos64,
-                     int B, int L, int Hq, int Hk, int D, int rot, int table_rows, float eps, int* status) {
-  if (B < 1 || L < 1 || (long long)B * L > 0x7fffffffll || Hq < 0 || Hk < 0 || Hq + Hk < 1 || (D != 64 && D != 128 && D != 256) || rot < 0 || rot % 16 || rot > D) return -SSM_ERR_BAD_ARG;
-  const void* all[] = {q, k, dq, dk, qo, ko, qw, kw, cs, sn};
+struct NormCall {                              // in the order in which cuda_ops packs it
+  const void *q, *k, *dq, *dk;                 // dq, dk: gradients of the results, backward pass only
+  void *qo, *ko;                               // results, or gradients of q and k
+  const void *qw, *kw, *cs, *sn, *positions;
+  int* status;
+  void *part, *dwq, *dwk;                      // dwq, dwk: gradients of the weights, fp32 or bf16 (null: none wanted), stored or (fp32) added to
+  long long strides[12];                       // (batch, token, head) of q, k, dq, dk
+  int qw32, kw32, pos64, B, L, Hq, Hk, D, rot, table_rows, dq32, dk32, addq, addk;
+  float eps;
+};
+static int norm_args(NormArgs* a, const NormCall& c, bool grads) {
+  if (c.B < 1 || c.L < 1 || (long long)c.B * c.L > 0x7fffffffll || c.Hq < 1 || c.Hk < 1 || (c.D != 64 && c.D != 128 && c.D != 256) || c.rot < 0 || c.rot % 16 ||
+      c.rot > c.D || (c.rot && (c.cs == nullptr || c.sn == nullptr)))
+    return -SSM_ERR_BAD_ARG;
+  const void* all[] = {c.q, c.k, c.qo, c.ko, c.qw, c.kw, c.cs, c.sn, grads ? c.dq : nullptr, grads ? c.dk : nullptr};
   for (const void* p : all) if (!aligned16(p)) return -SSM_ERR_BAD_ARG;
-  for (int i = 0; i < (dq != nullptr || dk != nullptr ? 12 : 6); ++i) if (strides[i] % 8) return -SSM_ERR_BAD_ARG;
+  for (int i = 0; i < (grads ? 12 : 6); ++i) if (c.strides[i] % 8) return -SSM_ERR_BAD_ARG;
   auto in = [](const void* p) { return reinterpret_cast<const __nv_bfloat16*>(p); };
   auto out = [](void* p) { return reinterpret_cast<__nv_bfloat16*>(p); };
-  const bool grads = dq != nullptr || dk != nullptr;
-  const long long none[6] = {0, 0, 0, 0, 0, 0};
-  const long long* g = grads ? strides + 6 : none;
-  a->t[0] = HeadRows{in(q), in(dq), out(qo), qw, strides[0], strides[1], strides[2], g[0], g[1], g[2], Hq, qw32};
-  a->t[1] = HeadRows{in(k), in(dk), out(ko), kw, strides[3], strides[4], strides[5], g[3], g[4], g[5], Hk, kw32};
-  a->cs = reinterpret_cast<const float*>(cs);
-  a->sn = reinterpret_cast<const float*>(sn);
-  a->positions = positions;
-  a->pos64 = pos64;
-  a->B = B; a->L = L; a->rot = rot; a->table_rows = table_rows;
-  a->eps = eps;
-  a->status = status;
+  const long long* g = c.strides;
+  a->t[0] = HeadRows{in(c.q), in(c.dq), out(c.qo), c.qw, g[0], g[1], g[2], g[6], g[7], g[8], c.Hq, c.qw32};
+  a->t[1] = HeadRows{in(c.k), in(c.dk), out(c.ko), c.kw, g[3], g[4], g[5], g[9], g[10], g[11], c.Hk, c.kw32};
+  a->cs = reinterpret_cast<const float*>(c.cs);
+  a->sn = reinterpret_cast<const float*>(c.sn);
+  a->positions = c.positions;
+  a->pos64 = c.pos64;
+  a->B = c.B; a->L = c.L; a->rot = c.rot; a->table_rows = c.table_rows;
+  a->eps = c.eps;
+  a->status = c.status;
   return 0;
 }
 
@@ -285,10 +292,10 @@ static GradPlan grad_plan(long long tokens, int Hq, int Hk, int D) {
   const long long uq = norm_turns(tokens, Hq, p.each, D), uk = norm_turns(tokens, Hk, p.each, D);
   const long long want = (uq + uk + NORM_WARPS - 1) / NORM_WARPS, most = 148 * 2;              // what runs at once
   const long long all = want < most ? want : most;
-  long long q = uq + uk > 0 ? (all * uq + (uq + uk) / 2) / (uq + uk) : 0;
-  if (Hq > 0 && q < 1) q = 1;
-  if (Hk > 0 && q > all - 1 && all > 1) q = all - 1;
-  const long long k = Hk == 0 ? 0 : all - q < 1 ? 1 : all - q;
+  long long q = (all * uq + (uq + uk) / 2) / (uq + uk);
+  if (q < 1) q = 1;
+  if (q > all - 1 && all > 1) q = all - 1;
+  const long long k = all - q < 1 ? 1 : all - q;
   p.q_blocks = (int)q;
   p.blocks = (int)(q + k);
   return p;
@@ -313,39 +320,28 @@ static int norm_bwd_launch(const NormArgs& a, const GradPlan& n, float* part, cu
 
 using namespace ssm;
 
-extern "C" int ssm_qk_norm_fwd(const void* q, const void* k, const long long* strides, void* qo, void* ko, const void* qw, const void* kw,
-                               int qw32, int kw32, const void* cs, const void* sn, const void* positions, int pos64, int B, int L,
-                               int Hq, int Hk, int D, int rot, int table_rows, float eps, int* status, cudaStream_t st) {
+extern "C" int ssm_qk_norm_fwd(const NormCall* c, cudaStream_t st) {
   NormArgs a;
-  const int bad = norm_args(&a, q, k, nullptr, nullptr, strides, qo, ko, qw, kw, qw32, kw32, cs, sn, positions, pos64, B, L, Hq, Hk, D,
-                            rot, table_rows, eps, status);
-  if (bad) return bad;
-  const int each = heads_each((long long)B * L, Hq, Hk, D);
-  const long long warps = norm_turns((long long)B * L, Hq, each, D) + norm_turns((long long)B * L, Hk, each, D);
-  const long long grid = (warps + NORM_WARPS - 1) / NORM_WARPS;
+  if (int bad = norm_args(&a, *c, false)) return bad;
+  const long long tokens = (long long)c->B * c->L;
+  const int each = heads_each(tokens, c->Hq, c->Hk, c->D);
+  const long long grid = (norm_turns(tokens, c->Hq, each, c->D) + norm_turns(tokens, c->Hk, each, c->D) + NORM_WARPS - 1) / NORM_WARPS;
   if (grid > 0x7fffffffll) return -SSM_ERR_BAD_ARG;
-  return D == 64 ? norm_fwd_launch<64>(a, (unsigned)grid, each, st) : D == 128 ? norm_fwd_launch<128>(a, (unsigned)grid, each, st)
-                                                                              : norm_fwd_launch<256>(a, (unsigned)grid, each, st);
+  return c->D == 64 ? norm_fwd_launch<64>(a, (unsigned)grid, each, st) : c->D == 128 ? norm_fwd_launch<128>(a, (unsigned)grid, each, st)
+                                                                                    : norm_fwd_launch<256>(a, (unsigned)grid, each, st);
 }
 
-// Blocks of the backward pass; the caller's buffer of partial sums has that many times D floats.
+// Blocks of the backward pass; `part` has that many times D floats.
 extern "C" int ssm_qk_norm_bwd_blocks(long long tokens, int Hq, int Hk, int D) { return grad_plan(tokens, Hq, Hk, D).blocks; }
 
-// dwq, dwk: gradients of the weights, fp32 or bf16 (null: none wanted), stored or (fp32) added to.
-extern "C" int ssm_qk_norm_bwd(const void* q, const void* k, const void* dq, const void* dk, const long long* strides, void* dxq, void* dxk,
-                               const void* qw, const void* kw, int qw32, int kw32, const void* cs, const void* sn, const void* positions,
-                               int pos64, int B, int L, int Hq, int Hk, int D, int rot, int table_rows, float eps, int* status,
-                               void* part, void* dwq, void* dwk, int dq32, int dk32, int addq, int addk, cudaStream_t st) {
+extern "C" int ssm_qk_norm_bwd(const NormCall* c, cudaStream_t st) {
   NormArgs a;
-  const int bad = norm_args(&a, q, k, dq, dk, strides, dxq, dxk, qw, kw, qw32, kw32, cs, sn, positions, pos64, B, L, Hq, Hk, D, rot,
-                            table_rows, eps, status);
-  if (bad) return bad;
-  if ((addq && !dq32) || (addk && !dk32)) return -SSM_ERR_BAD_ARG;
-  const GradPlan n = grad_plan((long long)B * L, Hq, Hk, D);
-  float* p = reinterpret_cast<float*>(part);
-  const int e = D == 64 ? norm_bwd_launch<64>(a, n, p, st) : D == 128 ? norm_bwd_launch<128>(a, n, p, st) : norm_bwd_launch<256>(a, n, p, st);
-  if (e) return e;
-  if (dwq == nullptr && dwk == nullptr) return 0;
-  return launch_dependent(qk_norm_dw_kernel, dim3(D / 32, 2), dim3(1024), 0, st, p, n.q_blocks, n.blocks, D,
-                          WeightGrads{{dwq, dwk}, {dq32, dk32}, {addq, addk}});
+  if (int bad = norm_args(&a, *c, true)) return bad;
+  if ((c->addq && !c->dq32) || (c->addk && !c->dk32)) return -SSM_ERR_BAD_ARG;
+  const GradPlan n = grad_plan((long long)c->B * c->L, c->Hq, c->Hk, c->D);
+  float* p = reinterpret_cast<float*>(c->part);
+  const int e = c->D == 64 ? norm_bwd_launch<64>(a, n, p, st) : c->D == 128 ? norm_bwd_launch<128>(a, n, p, st) : norm_bwd_launch<256>(a, n, p, st);
+  if (e || (c->dwq == nullptr && c->dwk == nullptr)) return e;
+  return launch_dependent(qk_norm_dw_kernel, dim3(c->D / 32, 2), dim3(1024), 0, st, p, n.q_blocks, n.blocks, c->D,
+                          WeightGrads{{c->dwq, c->dwk}, {c->dq32, c->dk32}, {c->addq, c->addk}});
 }

@@ -1351,51 +1351,59 @@ def attention(q, k, v, causal=True):
 # norms of queries and keys with rotation, paged key-value cache, attention of one new token
 # ======================================================================================
 _KV_TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1, torch.int8: 2}
+_NORM_CALL = struct.Struct("=15Q12q14if")
+_KV_WRITE_CALL = struct.Struct("=16Q9q13if")
+_KV_READ_CALL = struct.Struct("=9Q9i")
+_PAGED_ATTN_CALL = struct.Struct("=10Q3q8if")
+_NO_STRIDES = (0, 0, 0)
 
 
 def _head_view(t: torch.Tensor):
-    """t [B, L, H, Dh] with unit channel stride, other strides multiples of 8 and a 16-byte base, and its strides (a copy only
-    where it must be).  The stride of a dimension of one element says nothing and counts as 0."""
-    sb, sl, sh = [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
-    if t.stride(3) != 1 or (sb | sl | sh) & 7 or t.data_ptr() & 15:
-        t = t.contiguous()
-        if t.data_ptr() & 15:
-            t = t.clone()
-        _, L, H, D = t.shape
-        sb, sl, sh = L * H * D, H * D, D
-    return t, (sb, sl, sh)
-
-
-def _strides(*each):
-    flat = [s for strides in each for s in strides]
-    return (_c.c_longlong * len(flat))(*flat)
+    """(t, its address, strides of batch, token and head): t [B, L, H, Dh] with unit channel stride, the others multiples of 8, and a
+    16-byte base (a copy only where it must be).  The stride of a dimension of one element says nothing and counts as 0."""
+    (B, L, H, D), (sb, sl, sh, sd) = t.shape, t.stride()
+    sb, sl, sh, at = sb if B > 1 else 0, sl if L > 1 else 0, sh if H > 1 else 0, t.data_ptr()
+    if sd != 1 or (sb | sl | sh) & 7 or at & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        return t, t.data_ptr(), (L * H * D, H * D, D)
+    return t, at, (sb, sl, sh)
 
 
 def _aligned(t: Optional[torch.Tensor]):
-    """t contiguous on a 16-byte base."""
-    if t is None or (t.is_contiguous() and not t.data_ptr() & 15):
-        return t
-    return t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+    """(t, its address), contiguous on a 16-byte base; (None, 0) for None."""
+    if t is None:
+        return None, 0
+    at = t.data_ptr()
+    if at & 15 or not t.is_contiguous():
+        t = t.clone(memory_format=torch.contiguous_format)
+        at = t.data_ptr()
+    return t, at
+
+
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _is32(t) -> int:
+    return int(t is not None and t.dtype is torch.float32)
 
 
 def _require_head_dim(dim: int, rotary: int) -> None:
     if dim not in HEAD_DIMS:
         raise ValueError(f"the kernels are written for heads of {HEAD_DIMS} channels, got {dim}")
-    if rotary % 16:
+    if rotary & 15:
         raise ValueError(f"the kernels rotate a multiple of 16 channels, got {rotary}")
 
 
 def _require_norm_weight(w) -> None:
-    if w is not None and w.dtype not in (torch.bfloat16, torch.float32):
+    if w is not None and w.dtype is not torch.bfloat16 and w.dtype is not torch.float32:
         raise TypeError(f"norm weights are bfloat16 or float32, got {w.dtype}")
 
 
-def _require_one_device(*ts) -> torch.device:
-    dev = ts[0].device
+def _require_device(dev: int, *ts) -> None:
     for t in ts:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    return dev
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"the tensors of a call are on one device: cuda:{dev}, got one on {t.device}")
 
 
 def _on_device(op):
@@ -1412,52 +1420,56 @@ def _on_device(op):
 class _QKNormRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, qw, kw, eps, cos, sin, positions):
-        (B, L, Hq, D), Hk = q.shape, k.shape[2]
-        (q2, qs), (k2, ks) = _head_view(q), _head_view(k)
-        qw2, kw2 = _aligned(qw), _aligned(kw)
-        qo = torch.empty(B, L, Hq, D, dtype=torch.bfloat16, device=q.device)
-        ko = torch.empty(B, L, Hk, D, dtype=torch.bfloat16, device=q.device)
+        (B, L, Hq, D), Hk, dev = q.shape, k.shape[2], q.device
+        (q2, q_at, qs), (k2, k_at, ks) = _head_view(q), _head_view(k)
+        (w1, qw_at), (w2, kw_at) = _aligned(qw), _aligned(kw)
+        qo = torch.empty((B, L, Hq, D), dtype=torch.bfloat16, device=dev)
+        ko = torch.empty((B, L, Hk, D), dtype=torch.bfloat16, device=dev)
+        rotary, rows = (0, 0) if cos is None else (2 * cos.shape[1], cos.shape[0])
+        # of the call: what the backward pass packs again
+        ctx.call = (_is32(qw), _is32(kw), int(positions is not None and positions.dtype is torch.int64), B, L, Hq, Hk, D, rotary, rows)
         if B and L:
-            _run("ssm_qk_norm_fwd", _p(q2), _p(k2), _strides(qs, ks), _p(qo), _p(ko), _p(qw2), _p(kw2), _is32(qw), _is32(kw), _p(cos),
-                 _p(sin), _p(positions), int(positions is not None and positions.dtype == torch.int64), B, L, Hq, Hk, D,
-                 0 if cos is None else 2 * cos.shape[1], 0 if cos is None else cos.shape[0], _c.c_float(eps),
-                 _p(status_tensor(q.device)), _st())
+            _run("ssm_qk_norm_fwd", _NORM_CALL.pack(q_at, k_at, 0, 0, qo.data_ptr(), ko.data_ptr(), qw_at, kw_at, _at(cos), _at(sin),
+                                                    _at(positions), status_tensor(dev).data_ptr(), 0, 0, 0, *qs, *ks, *_NO_STRIDES,
+                                                    *_NO_STRIDES, *ctx.call, 0, 0, 0, 0, eps), _st())
         ctx.save_for_backward(q2, k2, qw, kw, cos, sin, positions)
-        ctx.eps, ctx.strides = eps, (qs, ks)
+        ctx.eps, ctx.strides = eps, (*qs, *ks)
         return qo, ko
 
     @staticmethod
     def backward(ctx, dqo, dko):
-        q2, k2, qw, kw, cos, sin, positions = ctx.saved_tensors
-        (B, L, Hq, D), Hk, dev = q2.shape, k2.shape[2], q2.device
-        (g, gs), (h, hs) = _head_view(dqo), _head_view(dko)
-        dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q2, k2))
-        grads, targets, adds = [], [], []
-        for w, need in ((qw, ctx.needs_input_grad[2]), (kw, ctx.needs_input_grad[3])):
-            mg = getattr(w, "main_grad", None) if need and w.is_leaf else None
-            if mg is not None and mg.dtype == torch.float32 and B and L:
-                # the optimizer's fp32 gradient: stored by the first contribution of a step, added to by the others
-                targets.append(mg)
-                adds.append(int(not getattr(w, "grad_stale", False)))
-                w.grad_stale = False
-                grads.append(None)
+        q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
+        _, _, _, B, L, Hq, Hk, D, _, _ = ctx.call
+        dev, need = q.device, ctx.needs_input_grad
+        (g, g_at, gs), (h, h_at, hs) = _head_view(dqo), _head_view(dko)
+        dq = torch.empty((B, L, Hq, D), dtype=torch.bfloat16, device=dev)
+        dk = torch.empty((B, L, Hk, D), dtype=torch.bfloat16, device=dev)
+        grads, targets, adds = [None, None], [None, None], [0, 0]
+        for i, w in enumerate((qw, kw)):
+            if not need[2 + i]:
                 continue
-            grads.append(torch.empty(D, dtype=w.dtype, device=dev) if need else None)
-            targets.append(grads[-1])
-            adds.append(0)
+            mg = getattr(w, "main_grad", None) if w.is_leaf else None
+            if mg is None or mg.dtype is not torch.float32 or not (B and L):
+                grads[i] = targets[i] = torch.empty((D,), dtype=w.dtype, device=dev)
+                continue
+            # the optimizer's fp32 gradient: stored by the first contribution of a step, added to by the others
+            targets[i], adds[i] = mg, int(not getattr(w, "grad_stale", False))
+            w.grad_stale = False
         if not (B and L):
             return dq, dk, *[None if t is None else t.zero_() for t in grads], None, None, None, None
-        part = torch.empty(_lib().ssm_qk_norm_bwd_blocks(_ll(B * L), Hq, Hk, D), D, dtype=torch.float32, device=dev)
-        _run("ssm_qk_norm_bwd", _p(q2), _p(k2), _p(g), _p(h), _strides(*ctx.strides, gs, hs), _p(dq), _p(dk), _p(_aligned(qw)),
-             _p(_aligned(kw)), _is32(qw), _is32(kw), _p(cos), _p(sin), _p(positions),
-             int(positions is not None and positions.dtype == torch.int64), B, L, Hq, Hk, D, 0 if cos is None else 2 * cos.shape[1],
-             0 if cos is None else cos.shape[0], _c.c_float(ctx.eps), _p(status_tensor(dev)), _p(part), _p(targets[0]), _p(targets[1]),
-             _is32(targets[0]), _is32(targets[1]), *adds, _st())
+        part = torch.empty((_norm_grad_blocks(B * L, Hq, Hk, D) * D,), dtype=torch.float32, device=dev)
+        (w1, qw_at), (w2, kw_at) = _aligned(qw), _aligned(kw)
+        _run("ssm_qk_norm_bwd", _NORM_CALL.pack(_at(q), _at(k), g_at, h_at, dq.data_ptr(), dk.data_ptr(), qw_at, kw_at, _at(cos), _at(sin),
+                                                _at(positions), status_tensor(dev).data_ptr(), part.data_ptr(), _at(targets[0]),
+                                                _at(targets[1]), *ctx.strides, *gs, *hs, *ctx.call, _is32(targets[0]), _is32(targets[1]),
+                                                *adds, ctx.eps), _st())
         return dq, dk, *grads, None, None, None, None
 
 
-def _is32(t) -> int:
-    return int(t is not None and t.dtype == torch.float32)
+@functools.lru_cache(maxsize=1024)
+def _norm_grad_blocks(*sizes) -> int:
+    tokens, Hq, Hk, D = sizes
+    return _lib().ssm_qk_norm_bwd_blocks(_ll(tokens), Hq, Hk, D)
 
 
 @_on_device
@@ -1465,20 +1477,23 @@ def qk_norm_rotary(q, k, q_weight, k_weight, eps, cos, sin, positions):
     _require_bf16(q, k)
     _require_norm_weight(q_weight)
     _require_norm_weight(k_weight)
-    _require_one_device(q, k, q_weight, k_weight, cos, sin, positions)
+    _require_device(q.get_device(), k, q_weight, k_weight, cos, sin, positions)
     _require_head_dim(q.shape[3], 0 if cos is None else 2 * cos.shape[1])
-    if positions is not None:
+    if positions is not None and not positions.is_contiguous():
         positions = positions.contiguous()
-    return _apply(_QKNormRotary, q, k, q_weight, k_weight, float(eps), _aligned(cos), _aligned(sin), positions)
+    return _apply(_QKNormRotary, q, k, q_weight, k_weight, float(eps), _aligned(cos)[0], _aligned(sin)[0], positions)
 
 
 def _page_args(pages):
-    t = _KV_TYPES.get(pages.k.dtype)
+    """Addresses of the pages and scales, type, pages and page size."""
+    k, v, ks, vs = pages
+    t = _KV_TYPES.get(k.dtype)
     if t is None:
-        raise TypeError(f"GPU pages hold bfloat16, float8_e4m3fn or int8, got {pages.k.dtype}")
-    if (pages.k.data_ptr() | pages.v.data_ptr()) & 15:
-        raise ValueError("pages begin on 16 bytes")
-    return (_p(pages.k), _p(pages.v), _p(pages.k_scale), _p(pages.v_scale), t, pages.k.shape[0], pages.k.shape[2])
+        raise TypeError(f"GPU pages hold bfloat16, float8_e4m3fn or int8, got {k.dtype}")
+    at = (k.data_ptr(), v.data_ptr(), _at(ks), _at(vs))
+    if (at[0] | at[1] | at[2] | at[3]) & 15:
+        raise ValueError("pages and scales begin on 16 bytes")
+    return at, (t, k.shape[0], k.shape[2])
 
 
 @_on_device
@@ -1486,20 +1501,26 @@ def kv_cache_write(k, v, pages, block_table, lengths, counts, q, q_weight, k_wei
     _require_bf16(k, v, q)
     _require_norm_weight(q_weight)
     _require_norm_weight(k_weight)
-    dev = _require_one_device(k, v, pages.k, q, q_weight, k_weight, cos, sin)
-    B, L, Hk, D = k.shape
+    _require_device(k.get_device(), v, pages.k, q, q_weight, k_weight, cos, sin)
+    (B, L, Hk, D), dev = k.shape, k.device
     rotary, rows = (0, 0) if cos is None else (2 * cos.shape[1], cos.shape[0])
     _require_head_dim(D, rotary)
-    held = _page_args(pages)
-    (k, ks), (v, vs) = _head_view(k), _head_view(v)
-    q, qs = (None, (0, 0, 0)) if q is None else _head_view(q)
-    Hq = 0 if q is None else q.shape[2]
-    out = None if q is None else torch.empty(B, L, Hq, D, dtype=torch.bfloat16, device=dev)
+    held, sizes = _page_args(pages)
+    (k, k_at, ks), (v, v_at, vs) = _head_view(k), _head_view(v)
+    Hq, out, q_at, out_at, qs = 0, None, 0, 0, _NO_STRIDES
+    if q is not None:
+        Hq = q.shape[2]
+        q, q_at, qs = _head_view(q)
+        out = torch.empty((B, L, Hq, D), dtype=torch.bfloat16, device=dev)
+        out_at = out.data_ptr()
+    (w1, qw_at), (w2, kw_at), (c1, cos_at), (c2, sin_at) = _aligned(q_weight), _aligned(k_weight), _aligned(cos), _aligned(sin)
     if B and L:
-        _run("ssm_kv_write", _p(q), _p(k), _p(v), _strides(qs, ks, vs), _p(out), _p(_aligned(q_weight)), _p(_aligned(k_weight)),
-             _is32(q_weight), _is32(k_weight), _p(_aligned(cos)), _p(_aligned(sin)), rotary, rows, _c.c_float(eps), *held,
-             _p(block_table), block_table.shape[1], _p(lengths), _p(counts), B, L, Hq, Hk, D, _p(status_tensor(dev)), _st())
-        torch.autograd.graph.increment_version([t for t in pages if t is not None])
+        _run("ssm_kv_write", _KV_WRITE_CALL.pack(q_at, k_at, v_at, out_at, qw_at, kw_at, cos_at, sin_at, *held, block_table.data_ptr(),
+                                                 lengths.data_ptr(), _at(counts), status_tensor(dev).data_ptr(), *qs, *ks, *vs,
+                                                 _is32(q_weight), _is32(k_weight), rotary, rows, *sizes, block_table.shape[1], B, L, Hq,
+                                                 Hk, D, eps), _st())
+        # written through their addresses: autograd learns of it here
+        torch.autograd.graph.increment_version(pages[:2] if pages.k_scale is None else pages)
     return out
 
 
@@ -1509,20 +1530,23 @@ def kv_cache_read(pages, block_table, lengths, max_length, dtype):
 
 @_on_device
 def _kv_cache_read(first, pages, block_table, lengths, max_length, dtype):
-    if dtype not in (torch.bfloat16, torch.float32):
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise TypeError(f"cached values are read as bfloat16 or float32, got {dtype}")
-    _, Hk, _, D = first.shape
+    Hk, D, B, dev = first.shape[1], first.shape[3], block_table.shape[0], first.device
     _require_head_dim(D, 0)
-    held = _page_args(pages)
-    B = block_table.shape[0]
-    k, v = (torch.empty(B, max_length, Hk, D, dtype=dtype, device=first.device) for _ in range(2))
+    held, sizes = _page_args(pages)
+    if B > 65535:
+        raise ValueError(f"the kernel reads at most 65535 sequences at once, got {B}")
+    k = torch.empty((B, max_length, Hk, D), dtype=dtype, device=dev)
+    v = torch.empty((B, max_length, Hk, D), dtype=dtype, device=dev)
     if B and max_length:
-        _run("ssm_kv_read", *held, _p(block_table), block_table.shape[1], _p(lengths), _p(k), _p(v), int(dtype == torch.float32), B,
-             max_length, Hk, D, _p(status_tensor(first.device)), _st())
+        _run("ssm_kv_read", _KV_READ_CALL.pack(*held, block_table.data_ptr(), lengths.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                               status_tensor(dev).data_ptr(), *sizes, block_table.shape[1], int(dtype is torch.float32),
+                                               B, max_length, Hk, D), _st())
     return k, v
 
 
-@functools.lru_cache(maxsize=256)
+@functools.lru_cache(maxsize=1024)
 def _paged_workspace(device: int, *sizes) -> int:
     """Floats of the attention's workspace for (type, width, page, B, Hq, Hkv, D) on the current device."""
     fn = _lib().ssm_paged_attn_workspace
@@ -1536,17 +1560,20 @@ def _paged_workspace(device: int, *sizes) -> int:
 @_on_device
 def paged_attention(q, pages, block_table, lengths, scale):
     _require_bf16(q)
-    dev = _require_one_device(q, pages.k)
-    B, _, Hq, D = q.shape
+    index, dev, first = q.get_device(), q.device, pages.k
+    _require_device(index, first)
+    (B, _, Hq, D), (n, Hk, page, _), width = q.shape, first.shape, block_table.shape[1]
     _require_head_dim(D, 0)
-    held = _page_args(pages)
-    q, (qb, _, qh) = _head_view(q)
-    out = torch.empty(B, 1, Hq, D, dtype=torch.bfloat16, device=dev)
-    if B:
-        Hk, width = pages.k.shape[1], block_table.shape[1]
-        if pages.k.numel() // D >= 2 ** 31:
-            raise ValueError("the attention kernel reads pools of less than 2^31 rows (pages x key heads x page size)")
-        ws = torch.empty(_paged_workspace(dev.index, held[4], width, held[6], B, Hq, Hk, D), dtype=torch.float32, device=dev)
-        _run("ssm_paged_attn", _p(q), _ll(qb), _ll(qh), _p(out), *held, _p(block_table), width, _p(lengths), B, Hq, Hk, D,
-             _c.c_float(1.0 / D ** 0.5 if scale is None else scale), _p(ws), _ll(ws.numel()), _p(status_tensor(dev)), _st())
-    return out
+    held, sizes = _page_args(pages)
+    if n * Hk * page >= 2 ** 31:
+        raise ValueError("the attention kernel reads pools of less than 2^31 rows (pages x key heads x page size)")
+    q, q_at, (qb, _, qh) = _head_view(q)
+    out = torch.empty((B, 1, Hq, D), dtype=torch.bfloat16, device=dev)
+    if B and n and width:
+        floats = _paged_workspace(index, sizes[0], width, page, B, Hq, Hk, D)
+        ws = torch.empty((floats,), dtype=torch.float32, device=dev)
+        _run("ssm_paged_attn", _PAGED_ATTN_CALL.pack(q_at, out.data_ptr(), *held, block_table.data_ptr(), lengths.data_ptr(),
+                                                     ws.data_ptr(), status_tensor(dev).data_ptr(), qb, qh, floats, *sizes, width, B, Hq,
+                                                     Hk, D, D ** -0.5 if scale is None else scale), _st())
+        return out
+    return out.zero_()

@@ -74,7 +74,7 @@ def qk_norm_rotary(q, k, q_weight, k_weight, eps: float, cos=None, sin=None, pos
     or None (no rotation).  Token l has the tables' row l, or row positions[b, l] (int32 or int64 [B, L]; packed sequences).
     q and k may be strided views of one projection.  On the GPU: bf16 activations, bf16 or fp32 weights, Dh 64, 128 or 256, rotary
     dim a multiple of 16; a position outside the tables gives a zero row (gradient zero) and status 3 (`check_status`)."""
-    check_heads(q, k, (cos, sin), positions)
+    check_heads(q, k, cos, sin, positions, True)
     check_norm_weight("q_weight", q_weight, q.shape[3])
     check_norm_weight("k_weight", k_weight, q.shape[3])
     if _native(q):
@@ -220,7 +220,6 @@ def attention(q, k, v, causal: bool = True):
 
 
 # ---- paged key-value cache ------------------------------------------------------------------
-@torch.no_grad()
 def kv_cache_write(k, v, pages: KVPages, block_table, lengths, counts=None, q=None, q_weight=None, k_weight=None,
                    eps: float = 1e-6, cos=None, sin=None):
     """Puts the new tokens' k and v [B, L, Hkv, Dh] into `pages`, 8-bit pages quantised per token and head; with k_weight
@@ -233,17 +232,18 @@ def kv_cache_write(k, v, pages: KVPages, block_table, lengths, counts=None, q=No
     are not written, their queries are zero.  Two tokens never share a position: pages that sequences share are not written.
     A position without a page or outside the tables raises on the CPU; on the GPU such a token is skipped in the same way
     and leaves status 3 (`check_status`).  No gradients."""
-    check_heads(q, k, (cos, sin), None if cos is None else lengths[:, None].expand(k.shape[:2]))
+    check_heads(q, k, cos, sin, None, False)
     check_pages(pages, block_table, lengths, k.shape[0], counts)
     if v.shape != k.shape or v.dtype != k.dtype or pages.k.shape[1] != k.shape[2] or pages.k.shape[3] != k.shape[3]:
         raise ValueError(f"keys {tuple(k.shape)}, values {tuple(v.shape)} and pages {tuple(pages.k.shape)} do not fit together")
     check_norm_weight("q_weight", q_weight, k.shape[3])
     check_norm_weight("k_weight", k_weight, k.shape[3])
-    op = _cuda().kv_cache_write if _native(k) else oracle.kv_cache_write
-    return op(k, v, pages, block_table, lengths, counts, q, q_weight, k_weight, eps, cos, sin)
+    if _native(k):
+        return _cuda().kv_cache_write(k, v, pages, block_table, lengths, counts, q, q_weight, k_weight, eps, cos, sin)
+    with torch.no_grad():
+        return oracle.kv_cache_write(k, v, pages, block_table, lengths, counts, q, q_weight, k_weight, eps, cos, sin)
 
 
-@torch.no_grad()
 def kv_cache_read(pages: KVPages, block_table, lengths, max_length: int, dtype=torch.bfloat16):
     """The cached keys and values of every sequence as the values they stand for: two tensors [B, max_length, Hkv, Dh] of
     `dtype` (GPU: bfloat16 or float32), zeros from lengths[b] on.  A position without a page raises on the CPU; on the GPU
@@ -251,11 +251,12 @@ def kv_cache_read(pages: KVPages, block_table, lengths, max_length: int, dtype=t
     check_pages(pages, block_table, lengths, block_table.shape[0])
     if max_length < 0:
         raise ValueError("max_length is not negative")
-    op = _cuda().kv_cache_read if _native(pages.k) else oracle.kv_cache_read
-    return op(pages, block_table, lengths, max_length, dtype)
+    if _native(pages.k):
+        return _cuda().kv_cache_read(pages, block_table, lengths, max_length, dtype)
+    with torch.no_grad():
+        return oracle.kv_cache_read(pages, block_table, lengths, max_length, dtype)
 
 
-@torch.no_grad()
 def paged_attention(q, pages: KVPages, block_table, lengths, scale: Optional[float] = None):
     """Attention of one new token per sequence over its cached tokens: q [B, 1, Hq, Dh] -> [B, 1, Hq, Dh].  Query head h reads
     key head h // (Hq / Hkv); scale None: 1 / sqrt(Dh).  lengths [B] int32 counts the tokens of each sequence, the new one
@@ -266,8 +267,10 @@ def paged_attention(q, pages: KVPages, block_table, lengths, scale: Optional[flo
         raise ValueError(f"queries are [batch, 1, heads, head_dim], heads a multiple of the pages' key heads; got {tuple(q.shape)} "
                          f"for pages {tuple(pages.k.shape)}")
     check_pages(pages, block_table, lengths, q.shape[0])
-    op = _cuda().paged_attention if _native(q) else oracle.paged_attention
-    return op(q, pages, block_table, lengths, scale)
+    if _native(q):
+        return _cuda().paged_attention(q, pages, block_table, lengths, scale)
+    with torch.no_grad():
+        return oracle.paged_attention(q, pages, block_table, lengths, scale)
 
 
 def gelu(x):

@@ -41,53 +41,58 @@ def kv_pages(num_pages: int, kv_heads: int, page_size: int, head_dim: int, dtype
 
 
 def check_pages(pages, block_table, lengths, batch: int, counts=None) -> None:
-    """What holds for every operation on a cache; raises TypeError or ValueError."""
+    """What holds for every operation on a cache; raises ValueError.  (One expression: a call costs the host as much as its launch.)"""
     k, v, ks, vs = pages
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+    shape, dtype, dev, i32, f32 = k.shape, k.dtype, k.get_device(), torch.int32, torch.float32
+    page = shape[2] if len(shape) == 4 else 0
+    if (page >= 16 and not page & (page - 1) and v.shape == shape and v.dtype is dtype and k.is_contiguous() and v.is_contiguous()
+            and v.get_device() == dev and block_table.dtype is i32 and block_table.dim() == 2 and block_table.shape[0] == batch
+            and block_table.is_contiguous() and block_table.get_device() == dev and lengths.dtype is i32 and lengths.shape == (batch,)
+            and lengths.is_contiguous() and lengths.get_device() == dev
+            and (counts is None or (counts.dtype is i32 and counts.shape == (batch,) and counts.is_contiguous()
+                                    and counts.get_device() == dev))
+            and (ks is None and vs is None if dtype not in QUANT_MAX else
+                 ks is not None and vs is not None and ks.dtype is f32 and vs.dtype is f32 and ks.shape == shape[:3]
+                 and vs.shape == shape[:3] and ks.is_contiguous() and vs.is_contiguous() and ks.get_device() == dev
+                 and vs.get_device() == dev)):
+        return
+    if len(shape) != 4 or v.shape != shape or v.dtype != dtype:
         raise ValueError("k and v pages are [pages, kv_heads, page_size, head_dim] of one shape and type, got "
-                         f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
-    page = k.shape[2]
+                         f"{tuple(shape)} {dtype} and {tuple(v.shape)} {v.dtype}")
     if page < 16 or page & (page - 1):
         raise ValueError(f"a page holds a power of two of at least 16 tokens, got {page}")
-    if (ks is None) != (vs is None) or (ks is not None) != (k.dtype in QUANT_MAX):
+    if (ks is None) != (vs is None) or (ks is not None) != (dtype in QUANT_MAX):
         raise ValueError("8-bit pages come with scales for keys and values, other pages with none")
     for s in (ks, vs):
-        if s is not None and (s.shape != k.shape[:3] or s.dtype != torch.float32):
-            raise ValueError(f"scales are fp32 of shape {tuple(k.shape[:3])}, got {s.dtype} {tuple(s.shape)}")
-    if any(t is not None and not t.is_contiguous() for t in pages):
-        raise ValueError("pages and scales are contiguous")
-    for name, t, shape in (("block_table", block_table, (batch, block_table.shape[-1])), ("lengths", lengths, (batch,)),
-                           ("counts", counts, (batch,))):
-        if t is None:
-            continue
-        if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
-            raise ValueError(f"{name} is a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
-    for t in (v, ks, vs, block_table, lengths, counts):
-        if t is not None and t.device != k.device:
-            raise ValueError(f"pages, block table and lengths are on one device, got {k.device} and {t.device}")
+        if s is not None and (s.shape != shape[:3] or s.dtype != f32):
+            raise ValueError(f"scales are fp32 of shape {tuple(shape[:3])}, got {s.dtype} {tuple(s.shape)}")
+    for name, t, wanted in (("block_table", block_table, (batch, block_table.shape[-1])), ("lengths", lengths, (batch,)),
+                            ("counts", counts, (batch,))):
+        if t is not None and (t.dtype != i32 or tuple(t.shape) != wanted or not t.is_contiguous()):
+            raise ValueError(f"{name} is a contiguous int32 tensor of shape {wanted}, got {t.dtype} {tuple(t.shape)}")
+    raise ValueError("pages and scales are contiguous and on one device with the block table, lengths and counts")
 
 
-def check_heads(q, k, tables, positions=None) -> None:
-    """Shapes of queries and keys (either may be None) and of the rotation's tables."""
-    x = k if q is None else q
-    if x.dim() != 4 or (q is not None and k is not None and (
-            k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3])):
+def check_heads(q, k, cos, sin, positions, from_zero: bool) -> None:
+    """Shapes of queries and keys (q may be None) and of the rotation's tables; from_zero: without positions, token l has row l."""
+    shape = k.shape
+    if len(shape) != 4 or (q is not None and (q.dim() != 4 or q.shape[:2] != shape[:2] or q.shape[3] != shape[3])):
         raise ValueError("queries and keys are [batch, tokens, heads, head_dim] with the same batch, tokens and head_dim")
-    cos, sin = tables
-    if (cos is None) != (sin is None):
+    if cos is None and sin is None:
+        if positions is not None:
+            raise ValueError("positions without cos and sin")
+        return
+    if cos is None or sin is None:
         raise ValueError("cos and sin come together")
-    if cos is not None:
-        if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape
-                or cos.shape[1] * 2 > x.shape[3] or cos.shape[1] < 1):
-            raise ValueError("cos and sin are fp32 [positions, rotary_dim / 2] with rotary_dim <= head_dim")
-        if positions is not None and (positions.dtype not in (torch.int32, torch.int64) or positions.shape != x.shape[:2]):
-            raise ValueError("positions are int32 or int64 [batch, tokens]")
-        if positions is None and cos.shape[0] < x.shape[1]:
-            raise ValueError(f"tables of {cos.shape[0]} positions are too short for {x.shape[1]} tokens")
-    elif positions is not None:
-        raise ValueError("positions without cos and sin")
+    if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.dim() != 2 or cos.shape != sin.shape
+            or not 2 <= cos.shape[1] * 2 <= shape[3]):
+        raise ValueError("cos and sin are fp32 [positions, rotary_dim / 2] with rotary_dim <= head_dim")
+    if positions is not None and (positions.dtype not in (torch.int32, torch.int64) or positions.shape != shape[:2]):
+        raise ValueError("positions are int32 or int64 [batch, tokens]")
+    if positions is None and from_zero and cos.shape[0] < shape[1]:
+        raise ValueError(f"tables of {cos.shape[0]} positions are too short for {shape[1]} tokens")
 
 
 def check_norm_weight(name: str, weight, head_dim: int) -> None:
-    if weight is not None and tuple(weight.shape) != (head_dim,):
+    if weight is not None and weight.shape != (head_dim,):
         raise ValueError(f"{name} has one value per channel of a head, [{head_dim}], got {tuple(weight.shape)}")
