@@ -15,7 +15,7 @@ import sys
 import torch
 import torch.distributed as dist
 
-from state_space_models_neuron_b200.models import Mamba2Cache, Mamba2ForCausalLM, get_config
+from state_space_models_neuron_b200.models import Mamba2ForCausalLM, Mamba2HybridConfig, Mamba2HybridForCausalLM, get_config
 from state_space_models_neuron_b200.parallel import state as ps
 from state_space_models_neuron_b200.parallel.cross_entropy import parallel_argmax
 from state_space_models_neuron_b200.parallel.layers import set_init_seed
@@ -51,12 +51,24 @@ def build(args, device):
     dtype = torch.float32 if args.dtype == "float32" else torch.bfloat16
     config = get_config(args.model, args.vocab_size, n_groups=args.n_groups, dtype=dtype, head_dim=args.head_dim,
                         rmsnorm_within_groups=not args.rmsnorm_across_groups)
+    cls = Mamba2ForCausalLM
+    if isinstance(config, Mamba2HybridConfig):
+        cls = Mamba2HybridForCausalLM
+        config.qk_norm, config.rotary_emb_dim = args.qk_norm, args.rotary_emb_dim
     set_init_seed(args.seed)
     if args.checkpoint_path:
-        model = Mamba2ForCausalLM.from_pretrained(args.checkpoint_path, dtype=dtype)
+        model = cls.from_pretrained(args.checkpoint_path, dtype=dtype)
     else:
-        model = Mamba2ForCausalLM(config, device=device).to(dtype)
+        model = cls(config, device=device).to(dtype)
     return model.to(device).eval(), dtype
+
+
+def new_cache(args, model, tokens):
+    """An empty cache with room for `tokens` of each sequence."""
+    if not isinstance(model, Mamba2HybridForCausalLM):
+        return model.new_cache(args.batch)
+    kv = {"model": None, "bfloat16": torch.bfloat16, "float8_e4m3fn": torch.float8_e4m3fn, "int8": torch.int8}[args.kv_cache_dtype]
+    return model.new_cache(args.batch, tokens, kv_dtype=kv, page_size=args.page_size)
 
 
 @torch.no_grad()
@@ -68,14 +80,14 @@ def check(args, device) -> bool:
     if torch.isnan(full).any() or torch.isinf(full).any():
         print("NaN/Inf in full-forward logits")
         return False
-    cache = Mamba2Cache(model.config, args.batch, dtype=dtype, device=device)
+    cache = new_cache(args, model, args.seq_len)
     steps = [model.step(ids[:, i:i + 1], cache) for i in range(args.seq_len)]
     step_logits = torch.cat(steps, dim=1)
     lp = dtype != torch.float32
     ok = print_stats("step-by-step vs forward", step_logits, full, low_precision=lp)
     half = (args.seq_len // 2) // 128 * 128
     if half >= 128:
-        _, cache2 = model.prefill(ids[:, :half])
+        _, cache2 = model.prefill(ids[:, :half], new_cache(args, model, args.seq_len))
         tail = torch.cat([model.step(ids[:, i:i + 1], cache2) for i in range(half, args.seq_len)], dim=1)
         ok = print_stats("prefill+decode vs forward", tail, full[:, half:], low_precision=lp) and ok
     return ok
@@ -86,7 +98,7 @@ def bench(args, device) -> dict:
     model, dtype = build(args, device)
     g = torch.Generator().manual_seed(args.seed)
     prompt = torch.randint(0, args.vocab_size, (args.batch, args.seq_len), generator=g).to(device)
-    logits, cache = model.prefill(prompt)
+    logits, cache = model.prefill(prompt, new_cache(args, model, args.seq_len + args.warmup + args.decode_tokens))
     tok = parallel_argmax(logits[:, -1]).unsqueeze(-1)
     cuda = device.type == "cuda"
     graphed = None
@@ -146,6 +158,11 @@ def main(argv=None):
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--rmsnorm_across_groups", action="store_true")
     ap.add_argument("--checkpoint_path", default=None)
+    ap.add_argument("--kv_cache_dtype", default="model", choices=["model", "bfloat16", "float8_e4m3fn", "int8"],
+                    help="hybrid models: type of the cached keys and values (model: that of the weights)")
+    ap.add_argument("--page_size", type=int, default=64, help="hybrid models: tokens per page of the key-value cache")
+    ap.add_argument("--qk_norm", action="store_true", help="hybrid models without a checkpoint: norms of queries and keys")
+    ap.add_argument("--rotary_emb_dim", type=int, default=None, help="hybrid models without a checkpoint: rotated channels")
     ap.add_argument("--device", default=None)
     ap.add_argument("--no_graph", action="store_true", help="decode with eager launches instead of a CUDA graph")
     args = ap.parse_args(argv)

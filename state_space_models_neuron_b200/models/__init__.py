@@ -1,4 +1,4 @@
-from .cache import Mamba2Cache  # noqa: F401
+from .cache import Mamba2Cache, Mamba2HybridCache  # noqa: F401
 from .configuration_mamba2 import Mamba2Config  # noqa: F401
 from .configuration_mamba2hybrid import Mamba2HybridConfig  # noqa: F401
 from .layer_allocation import allocate_layers  # noqa: F401

@@ -1,9 +1,11 @@
-"""Decode cache: per layer a rolling conv window and the SSM state.
+"""Decode caches: per Mamba layer a rolling conv window and the SSM state, per attention layer of a hybrid model pages of keys
+and values.
 
 Field names and shapes follow the `Mamba2Cache` of transformers 4.46 that the reference imports
 (mamba2/mamba2_mixer.py:23) and the layouts its decode kernel uses
 (mamba2/mamba2_kernel_inference.py:36-43): `conv_states[layer]` is `[B, conv_dim, K]` (oldest token
-first), `ssm_states[layer]` is `[B, H, P, N]`; sizes are per tensor-parallel rank.
+first), `ssm_states[layer]` is `[B, H, P, N]`; sizes are per tensor-parallel rank.  The reference's hybrid has no cache
+(mamba2hybrid/mamba2hybrid_attn.py:379); the pages are those of `ops.kv_pages`.
 """
 from __future__ import annotations
 
@@ -12,6 +14,7 @@ from typing import Optional
 
 import torch
 
+from .. import ops
 from ..parallel import state as ps
 
 
@@ -59,3 +62,59 @@ class Mamba2Cache:
         self.seqlen_offset = 0
         for t in list(self.conv_states.values()) + list(self.ssm_states.values()):
             t.zero_()
+
+    def step_state(self):
+        """The tensors that a decoding step changes and the next one reads."""
+        return list(self.conv_states.values()) + list(self.ssm_states.values())
+
+    def require_room(self, tokens: int) -> None:
+        """Raises where the cache cannot take more tokens; the states of Mamba layers always can."""
+
+
+class Mamba2HybridCache(Mamba2Cache):
+    """Cache of a hybrid model: the Mamba layers' states, and for each attention layer a pool of pages (`pages[layer]`,
+    `ops.KVPages`) with room for `max_length` tokens of every sequence.  `block_table` [B, pages per sequence] and `lengths` [B]
+    (int32, tokens of each sequence) serve all layers.  `kv_dtype`: bfloat16, float8_e4m3fn or int8 (None: `dtype`)."""
+
+    def __init__(self, config, batch_size: int, max_length: int, dtype: torch.dtype = torch.bfloat16,
+                 device: Optional[torch.device] = None, ssm_dtype: torch.dtype = torch.float32, kv_dtype: Optional[torch.dtype] = None,
+                 page_size: int = 64):
+        from .layer_allocation import ATTENTION, MAMBA, allocate_layers
+        kinds = allocate_layers(config.num_hidden_layers, config.hybrid_attention_ratio, config.hybrid_mlp_ratio,
+                                config.hybrid_override_pattern)
+        super().__init__(config, batch_size, dtype, device, ssm_dtype, [i for i, k in enumerate(kinds) if k == MAMBA])
+        mult = int(getattr(config, "kv_shared_group_size", 1)) if getattr(config, "qkv_linear", False) else 1
+        heads = config.attn_key_value_heads * mult // ps.get_tensor_model_parallel_size()
+        per = -(-max_length // page_size)
+        self.max_length = max_length
+        self.pages = {i: ops.kv_pages(batch_size * per, heads, page_size, config.attn_head_dim, kv_dtype or dtype, device)
+                      for i, k in enumerate(kinds) if k == ATTENTION}
+        self.block_table = torch.arange(batch_size * per, dtype=torch.int32, device=device).view(batch_size, per)
+        self.lengths = torch.zeros(batch_size, dtype=torch.int32, device=device)
+        self._tables = {}
+
+    def rotary_tables(self, dim: int, theta: float):
+        """cos / sin of every position that the cache has room for."""
+        if (dim, theta) not in self._tables:
+            self._tables[dim, theta] = ops.rotary_tables(self.max_length, dim, theta, device=self.lengths.device)
+        return self._tables[dim, theta]
+
+    def require_room(self, tokens: int) -> None:
+        if self.seqlen_offset + tokens > self.max_length:
+            raise ValueError(f"the cache has room for {self.max_length} tokens, holds {self.seqlen_offset} and was given {tokens} more")
+
+    def take(self, tokens: int) -> None:
+        """Counts new tokens of every sequence; the attention layers put them behind the others."""
+        self.require_room(tokens)
+        self.lengths.add_(tokens)
+
+    def keys_values(self, layer_idx: int, dtype: torch.dtype = torch.bfloat16):
+        """Cached keys and values of an attention layer as the values they stand for, [B, tokens, kv heads, head_dim] each."""
+        return ops.kv_cache_read(self.pages[layer_idx], self.block_table, self.lengths, self.seqlen_offset, dtype)
+
+    def step_state(self):
+        return super().step_state() + [self.lengths]
+
+    def reset(self) -> None:
+        super().reset()
+        self.lengths.zero_()

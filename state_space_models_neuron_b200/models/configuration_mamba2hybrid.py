@@ -4,7 +4,8 @@ Defaults follow the reference (mamba2hybrid/configuration_mamba2hybrid.py:130-23
 cover variants the reference's hybrid never turns on but whose code it carries
 (mamba2hybrid/mamba2hybrid_attn.py:500-503, mamba2hybrid/mamba2hybrid_mlp.py:155-165):
 `rotary_emb_dim`/`rope_theta` (rotary position embedding in attention; None = off) and
-`gated_linear_unit` (SwiGLU-style gated MLP; False = plain GELU MLP).
+`gated_linear_unit` (SwiGLU-style gated MLP; False = plain GELU MLP).  `qk_norm` (an addition, off by
+default) gives the attention layers an RMS norm of every query and key head in front of the rotation.
 """
 from __future__ import annotations
 
@@ -39,6 +40,7 @@ class Mamba2HybridConfig(Mamba2Config):
         gated_linear_unit: bool = False,
         rotary_emb_dim=None,
         rope_theta: float = 10000.0,
+        qk_norm: bool = False,
         max_position_embeddings: int = 8192,
         dtype=torch.bfloat16,
         **kwargs,
@@ -56,6 +58,7 @@ class Mamba2HybridConfig(Mamba2Config):
         self.gated_linear_unit = gated_linear_unit
         self.rotary_emb_dim = rotary_emb_dim
         self.rope_theta = rope_theta
+        self.qk_norm = qk_norm
         self.max_position_embeddings = max_position_embeddings
         super().__init__(
             vocab_size=vocab_size,

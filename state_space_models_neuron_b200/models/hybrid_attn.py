@@ -6,7 +6,8 @@ dropout, per-rank heads = attn_num_heads/TP and kv heads = attn_key_value_heads/
 all-gather, K/V heads are never replicated in memory (the kernel indexes kv head = q head // ratio,
 where the reference materialises `repeat_kv`, mamba2hybrid_attn.py:440-447), and rotary embedding (its own
 kernel, forward and backward, with cached tables) is an option that is off by default as in the reference
-hybrid (mamba2hybrid_attn.py:500-503).
+hybrid (mamba2hybrid_attn.py:500-503).  With `qk_norm` queries and keys are normed per head and rotated in one pass.
+A prompt leaves its keys and values in the pages of a `Mamba2HybridCache`; `step` decodes one token over them.
 """
 from __future__ import annotations
 
@@ -17,6 +18,17 @@ from .. import ops
 from ..parallel import mappings as mp
 from ..parallel import state as ps
 from ..parallel.layers import ColumnParallelLinear, GQAQKVColumnParallelLinear, RowParallelLinear, normal_init
+
+
+class HeadRMSNorm(nn.Module):
+    """Weight of an RMS norm over the channels of a head, shared by the heads; the attention applies it.  Each tensor-parallel rank
+    sees its own heads, so the gradient is summed over the group as that of a norm under sequence parallelism is."""
+
+    def __init__(self, head_dim: int, dtype=torch.float32, device=None):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(head_dim, dtype=dtype, device=device))
+        if ps.get_tensor_model_parallel_size() > 1:
+            self.weight.sequence_parallel_enabled = True
 
 
 class Mamba2HybridAttention(nn.Module):
@@ -38,6 +50,10 @@ class Mamba2HybridAttention(nn.Module):
         self.rotary_emb_dim = getattr(config, "rotary_emb_dim", None)
         self.rope_theta = getattr(config, "rope_theta", 10000.0)
         dtype = config.dtype or torch.float32
+        self.norm_eps = config.layer_norm_epsilon
+        qk_norm = bool(getattr(config, "qk_norm", False))
+        self.q_norm = HeadRMSNorm(self.head_dim, dtype, device) if qk_norm else None
+        self.k_norm = HeadRMSNorm(self.head_dim, dtype, device) if qk_norm else None
         init = normal_init(config.initializer_range)
         kw = dict(bias=False, init_method=init, dtype=dtype, device=device,
                   sequence_parallel_enabled=config.sequence_parallel_enabled)
@@ -54,7 +70,8 @@ class Mamba2HybridAttention(nn.Module):
                                         init_method=init, dtype=dtype, device=device,
                                         sequence_parallel_enabled=config.sequence_parallel_enabled)
 
-    def forward(self, hidden_states: torch.Tensor, cache_params=None) -> torch.Tensor:
+    def _queries_keys_values(self, hidden_states):
+        """[B, L, heads, head_dim] each, of the whole sequence."""
         qkv = None
         if self.qkv_linear:
             qkv = self.qkv_proj(hidden_states)
@@ -74,9 +91,43 @@ class Mamba2HybridAttention(nn.Module):
         q = qkv[0].view(B, L, self.num_heads, self.head_dim)
         k = qkv[1].view(B, L, self.num_kv_heads, self.head_dim)
         v = qkv[2].view(B, L, self.num_kv_heads, self.head_dim)
+        return q, k, v
+
+    def forward(self, hidden_states: torch.Tensor, cache_params=None) -> torch.Tensor:
+        """Whole sequences.  With `cache_params` (a `Mamba2HybridCache` that has counted these tokens) their keys and values go
+        into the layer's pages, ready for `step`."""
+        q, k, v = self._queries_keys_values(hidden_states)
+        B, L = q.shape[:2]
+        cos = sin = None
         if self.rotary_emb_dim is not None:
             cos, sin = ops.rotary_tables(L, self.rotary_emb_dim, self.rope_theta, device=q.device)
+        if self.q_norm is not None:
+            q, k = ops.qk_norm_rotary(q, k, self.q_norm.weight, self.k_norm.weight, self.norm_eps, cos, sin)
+        elif cos is not None:
             q = ops.apply_rotary(q, cos, sin)
             k = ops.apply_rotary(k, cos, sin)
+        if cache_params is not None:
+            ops.kv_cache_write(k, v, cache_params.pages[self.layer_idx], cache_params.block_table, cache_params.lengths)
         o = ops.attention(q, k, v, causal=True)
         return self.o_proj(o.reshape(B, L, self.num_heads * self.head_dim))
+
+    @torch.no_grad()
+    def step(self, hidden_states: torch.Tensor, cache_params) -> torch.Tensor:
+        """Single-token decode over the cached keys and values; hidden_states [B, 1, D].  Norm, rotation and the write into the
+        pages are one kernel, the attention another."""
+        assert hidden_states.shape[1] == 1, "step() takes one token at a time"
+        if self.sequence_parallel_enabled:
+            raise RuntimeError("decode runs without sequence parallelism; build the model with it disabled")
+        q, k, v = self._queries_keys_values(hidden_states)
+        pages, table, lengths = cache_params.pages[self.layer_idx], cache_params.block_table, cache_params.lengths
+        cos = sin = None
+        if self.rotary_emb_dim is not None:
+            cos, sin = cache_params.rotary_tables(self.rotary_emb_dim, self.rope_theta)
+        if self.q_norm is None and cos is None:
+            ops.kv_cache_write(k, v, pages, table, lengths)
+        else:
+            weights = (None, None) if self.q_norm is None else (self.q_norm.weight, self.k_norm.weight)
+            q = ops.kv_cache_write(k, v, pages, table, lengths, q=q, q_weight=weights[0], k_weight=weights[1], eps=self.norm_eps,
+                                   cos=cos, sin=sin)
+        o = ops.paged_attention(q, pages, table, lengths)
+        return self.o_proj(o.reshape(o.shape[0], 1, self.num_heads * self.head_dim))

@@ -330,12 +330,16 @@ class Mamba2ForCausalLM(Mamba2PreTrainedModel, GenerationMixin):
         logits, stats = self.lm_head(hidden, ce_labels=shifted)
         return _mean_loss(logits, shifted, stats)
 
+    def new_cache(self, batch_size: int, max_length: int = 0) -> Mamba2Cache:
+        """An empty cache; its size does not depend on the number of tokens."""
+        p = next(self.parameters())
+        return Mamba2Cache(self.config, batch_size, dtype=p.dtype, device=p.device)
+
     @torch.no_grad()
     def prefill(self, input_ids, cache_params: Optional[Mamba2Cache] = None):
         """Run the chunked scan over a prompt, fill the cache, return last-token logits."""
         if cache_params is None:
-            p = next(self.parameters())
-            cache_params = Mamba2Cache(self.config, input_ids.shape[0], dtype=p.dtype, device=p.device)
+            cache_params = self.new_cache(input_ids.shape[0])
         out = self.backbone(input_ids=input_ids, cache_params=cache_params, use_cache=True)
         return ops.widen(self.lm_head(out.last_hidden_state[:, -1:, :])), cache_params
 
@@ -371,8 +375,7 @@ class Mamba2ForCausalLM(Mamba2PreTrainedModel, GenerationMixin):
         temperature 0 = greedy.  Returns [B, L + new] token ids.  (HuggingFace's `generate()` plumbing is kept for
         API compatibility, but like in the reference it does not drive this cache.)"""
         B, L = input_ids.shape
-        p = next(self.parameters())
-        cache = Mamba2Cache(self.config, B, dtype=p.dtype, device=p.device)
+        cache = self.new_cache(B, L + max_new_tokens)
         chunk = 128
         Lp = (L // chunk) * chunk
         logits = None

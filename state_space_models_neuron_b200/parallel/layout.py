@@ -9,7 +9,7 @@ from that tool's hard-coded 7B / TP=8 / head_dim=128 / one-group-per-rank case t
     conv1d.weight/bias  rows   x | B | C            same
     out_proj / o_proj / down_proj weight            split on columns (dim 1)
     A_log, D, dt_bias, mixer norm.weight, embeddings, lm_head, q/k/v, gate_up (per gate/up block)   dim 0
-    layer norms, norm_f                              replicated
+    layer norms, norm_f, q_norm, k_norm              replicated
 """
 from __future__ import annotations
 
@@ -50,7 +50,7 @@ def partition_rule(key: str, config) -> Rule:
         return 0, None
     if re.search(r"qkv_proj\.(weight|bias)_[qkv]$", key):      # kv_size_multiplier 1 only (no replicated heads)
         return 0, None
-    return None, None  # block norms, norm_f: replicated
+    return None, None  # block norms, norm_f, norms of queries and keys: replicated
 
 
 def shard_state_dict(full: Dict[str, torch.Tensor], config, tp_size: int, tp_rank: int) -> Dict[str, torch.Tensor]:
