@@ -64,6 +64,8 @@ __global__ void __launch_bounds__(KV_THREADS, 3) kv_write_kernel(const WriteArgs
   extern __shared__ uint4 slots[];             // [row][vector][thread]
   const int lane = threadIdx.x % LANES;
   const HeadRow<D> at(lane, a.rot);
+  pdl_trigger();
+  pdl_wait();
   const int qu = (a.heads[0] + each - 1) / each, ku = (a.heads[1] + each - 1) / each, units = qu + 2 * ku;
   const long long warp = (long long)blockIdx.x * KV_WARPS + threadIdx.x / 32, block = warp / units;
   int part = (int)(warp - block * units);
@@ -238,8 +240,7 @@ static int kv_write_launch(const WriteArgs& a, int Hq, int Hk, cudaStream_t st) 
   if (grid > 0x7fffffffll) return -SSM_ERR_BAD_ARG;
   static SmemOptIn opt;
   if (int e = opt.ask(reinterpret_cast<const void*>(kv_write_kernel<D, T>), EACH * 2 * KV_THREADS * 16)) return e;
-  kv_write_kernel<D, T><<<(unsigned)grid, KV_THREADS, each * 2 * KV_THREADS * 16, st>>>(a, each);
-  return (int)cudaGetLastError();
+  return launch_dependent(kv_write_kernel<D, T>, dim3((unsigned)grid), dim3(KV_THREADS), each * 2 * KV_THREADS * 16, st, a, each);
 }
 
 template <int D, int T, typename Out>

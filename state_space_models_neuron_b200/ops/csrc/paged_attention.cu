@@ -25,7 +25,7 @@
 namespace ssm {
 
 constexpr int PA_WARPS = 4, PA_BOX = 16, PA_COUNTERS = 768;      // PA_BOX: tokens of a box
-constexpr int PA_MIN_SHARE = 2 * PA_WARPS;     // steps: two per warp
+constexpr int PA_MIN_SHARE = 4 * PA_WARPS;     // steps: four per warp (two: 200 tokens 8.3 us instead of 7.0, a join that saves nothing; eight: 2048 tokens 12.5 instead of 10.2)
 constexpr int FEW_ITEMS = 8;                   // blocks per item, see the kernel
 // A running maximum moves when scores pass it by 2^8: bf16 and fp16 hold larger shares as well.
 constexpr float PA_GROWTH = 8.f, PA_SHARE = 256.f;
@@ -51,7 +51,9 @@ struct PagedAttn {
   static constexpr int BOX = PA_BOX * ROW;                     // bytes of a box's keys, or values
   static constexpr int STAGE = SUB * 2 * BOX;                  // of one warp: keys and values of each box
   static constexpr int LOADED = 2 * BOX + (T == KV_BF16 ? 0 : 2 * PA_BOX * 4); // of one box, with the scales
-  static constexpr int STAGES = 3;
+  // Two stages of 128-channel int8 leave room for three blocks, whose instructions hide each other (64 x 8192 199 -> 180 us; e4m3,
+  // which takes fewer, loses more by what is no longer under way: 176 -> 181); four of the smallest for as many bytes under way.
+  static constexpr int STAGES = T == KV_INT8 && ROW == 128 ? 2 : STAGE <= 4096 ? 4 : 3;
   static constexpr int RING = PA_WARPS * STAGES * STAGE;
   static constexpr int SMEM = RING + 1024;                     // boxes begin on 1024 bytes
   // per SM: as many as 96 KB, or more than one, of loads under way ask for, and registers leave
@@ -424,8 +426,12 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
     #pragma unroll
     for (int i = 0; i < C::STAGES; ++i) mbar_init(&full[warp][i], 1);
     mbar_fence_init();
+    tma_prefetch_desc(&kmap);
+    tma_prefetch_desc(&vmap);
   }
   __syncwarp();
+  pdl_trigger();
+  pdl_wait();
 
   // Where this block's share begins.  The steps of all sequences and heads stand in a row, each sequence's heads one behind the other;
   // sequences in the order lane, lane + 32, ... of the lanes that look at them (every warp finds the same).
@@ -448,16 +454,21 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
     }
   }
   const bool few = (long long)filled * items * FEW_ITEMS <= a.most_blocks;
-  const int blocks = few ? a.most_blocks - filled * items : gridDim.x;         // few: at most most_blocks shares in all
-  const int share = max(PA_MIN_SHARE, ((total + blocks - 1) / blocks + PA_WARPS - 1) / PA_WARPS * PA_WARPS);
+  const int blocks = few ? a.most_blocks : gridDim.x;
+  int share = max(PA_MIN_SHARE, ((total + blocks - 1) / blocks + PA_WARPS - 1) / PA_WARPS * PA_WARPS);
   if (few) {
-    // counted in shares from here on
-    mine = (first_steps + share - 1) / share * items;
-    for (int b = lane + 32; b < a.B; b += 32) mine += (steps_of(b) + share - 1) / share * items;
+    // The smallest share of which there are at most most_blocks; the last guess always fits.  Counted in shares from here on.
+    const int fits = max(PA_MIN_SHARE, ((total + blocks - filled * items - 1) / (blocks - filled * items) + PA_WARPS - 1) / PA_WARPS * PA_WARPS);
+    for (int guess = 0;; ++guess, share += PA_WARPS) {
+      if (guess == 3 || share > fits) share = fits;
+      mine = (first_steps + share - 1) / share * items;
+      for (int b = lane + 32; b < a.B; b += 32) mine += (steps_of(b) + share - 1) / share * items;
+      total = __reduce_add_sync(0xffffffffu, mine);
+      if (total <= blocks || share == fits) break;
+    }
     upto = mine;
     #pragma unroll
     for (int d = 1; d < 32; d <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += v; }
-    total = __shfl_sync(0xffffffffu, upto, 31);
   }
   const int unit = few ? 1 : share;            // of the row, per block
   if ((long long)unit * blockIdx.x >= total) return;
@@ -720,8 +731,7 @@ static int paged_attn_launch(const AttnArgs& a, int grid, cudaStream_t st) {
     if (make_tmap_2d(&map[i], C::BYTES == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, C::BYTES, a.pages[i], D, rows, C::ROW,
                      C::TILE / C::BYTES, PA_BOX, C::TILE == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
       return -SSM_ERR_BAD_ARG;
-  paged_attn_kernel<D, T, NT><<<grid, PA_WARPS * 32, C::SMEM, st>>>(a, map[0], map[1]);
-  return (int)cudaGetLastError();
+  return launch_dependent(paged_attn_kernel<D, T, NT>, dim3(grid), dim3(PA_WARPS * 32), C::SMEM, st, a, map[0], map[1]);
 }
 
 // Two column tiles for more than 8 query heads per key head; 256 channels leave registers for one.
