@@ -44,20 +44,21 @@ struct AttnArgs {
 template <int D, int T, int NT>
 struct PagedAttn {
   static constexpr int BYTES = KvType<T>::BYTES, ROW = D * BYTES, HEADS = 8 * NT;
-  static constexpr int SUB = ROW <= 128 ? 2 : 1, STEP = PA_BOX * SUB;         // boxes and tokens of a warp's step: 4 KB of keys and values or more
+  static constexpr int SUB = ROW == 64 ? 4 : ROW == 128 ? 2 : 1, STEP = PA_BOX * SUB;        // boxes and tokens of a warp's step: 8 KB of keys and values
   static constexpr int TILE = ROW >= 128 ? 128 : 64, TILES = ROW / TILE;      // bytes of a box's rows (and of its swizzle), boxes of a row
   static constexpr int KCH = ROW / 64;                         // 16-byte pieces of a key row per lane (four lanes share a row)
   static constexpr int VB = TILE / 8, VEL = VB / BYTES;        // bytes and values of a lane's piece of a value row's tile (eight lanes share it)
   static constexpr int BOX = PA_BOX * ROW;                     // bytes of a box's keys, or values
   static constexpr int STAGE = SUB * 2 * BOX;                  // of one warp: keys and values of each box
   static constexpr int LOADED = 2 * BOX + (T == KV_BF16 ? 0 : 2 * PA_BOX * 4); // of one box, with the scales
-  // Two stages of 128-channel int8 leave room for three blocks, whose instructions hide each other (64 x 8192 199 -> 180 us; e4m3,
-  // which takes fewer, loses more by what is no longer under way: 176 -> 181); four of the smallest for as many bytes under way.
-  static constexpr int STAGES = T == KV_INT8 && ROW == 128 ? 2 : STAGE <= 4096 ? 4 : 3;
+  static constexpr int STAGES = 2;
   static constexpr int RING = PA_WARPS * STAGES * STAGE;
   static constexpr int SMEM = RING + 1024;                     // boxes begin on 1024 bytes
-  // per SM: as many as 96 KB, or more than one, of loads under way ask for, and registers leave
-  static constexpr int BLOCKS = SMEM > 113 * 1024 ? 1 : SMEM > 73 * 1024 || NT == 2 ? 2 : 3;
+  // Blocks per SM.  64 KB of loads under way per SM are enough, and more of them cost bandwidth (bf16, two blocks of two stages / of three /
+  // three blocks of two, us: 64 x 8192 320 / 331 / 327, one of 131072 88 / 95 / 99; 256 of 200 tokens 53.5 / 51.0 / 48.6).  Where the
+  // instructions bound it, 8-bit values of 64 channels and int8, a third block hides them (two / three: 64 channels e4m3 65 / 58, 64 x 8192 int8
+  // 195 / 181, but e4m3 of 128 channels 176 / 181 and one of 131072 54 / 62).
+  static constexpr int BLOCKS = SMEM > 113 * 1024 ? 1 : NT == 1 && (ROW == 64 || (ROW == 128 && T == KV_INT8)) ? 3 : 2;
   static constexpr int SLOT = HEADS * D + 3 * HEADS;           // floats of a part: o [channel][head], m, sum, M
   static constexpr int MEET = D * HEADS + D / VEL * 8;         // floats of a warp's o where the warps meet, see leave()
   static_assert(PA_WARPS * MEET * 4 <= RING && PA_COUNTERS * HEADS * 4 <= RING, "the warps' results meet in the ring");
@@ -184,9 +185,9 @@ struct AttnWarp {
     for (int t = 0; t < D / 16; ++t) { o[nt][t][j] *= f; o[nt][t][j + 2] *= f; }
   }
 
-  // The boxes of a stage of this warp's ring; the first `valid & 255` tokens of the first box count, and so on for the second.
+  // The boxes of a stage of this warp's ring; of the first box the first `valid & 255` tokens count, of the next as the next byte says.
   __device__ __forceinline__ void step(const uint8_t* stage, const float* scales, int valid) {
-    constexpr int SUB = C::SUB, FULL = SUB == 2 ? PA_BOX | PA_BOX << 8 : PA_BOX;
+    constexpr int SUB = C::SUB, FULL = SUB == 4 ? 0x10101010 : SUB == 2 ? 0x1010 : 0x10;
     const int g = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3, tok = sigma<C::TILE>(g);
     float s[SUB][NT][4];
     #pragma unroll
@@ -220,7 +221,6 @@ struct AttnWarp {
     }
     // lane (g, c): tokens tok and tok + 8 of each box, heads 2c and 2c + 1 of each tile: s' - m
     float vs[SUB][2];                           // scales of the values
-    bool grows = false;
     #pragma unroll
     for (int u = 0; u < SUB; ++u) {
       float ks[2] = {1.f, 1.f};
@@ -249,15 +249,13 @@ struct AttnWarp {
         }
       }
     }
+    float most = s[0][0][0];
     #pragma unroll
     for (int u = 0; u < SUB; ++u) {
       #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) grows |= s[u][nt][i] > PA_GROWTH;
-      }
+      for (int nt = 0; nt < NT; ++nt) most = fmaxf(fmaxf(most, fmaxf(s[u][nt][0], s[u][nt][1])), fmaxf(s[u][nt][2], s[u][nt][3]));
     }
-    const bool moves = __any_sync(0xffffffffu, grows) || fresh;
+    const bool moves = __any_sync(0xffffffffu, most > PA_GROWTH) || fresh;
     if (moves) {
       #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -279,22 +277,24 @@ struct AttnWarp {
       }
     }
     uint32_t p[SUB][NT][2];
-    bool large = false;
+    most = 0.f;
     #pragma unroll
     for (int u = 0; u < SUB; ++u) {
       #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        float w[4];
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float e = exp2f(s[u][nt][i]);
           l[nt][i & 1] += e;
           s[u][nt][i] = e;
-          if (F16) large |= e * (vs[u][i >> 1] * G[nt][i & 1]) > PA_SHARE;
+          w[i] = e * (vs[u][i >> 1] * G[nt][i & 1]);
         }
+        if (F16) most = fmaxf(fmaxf(most, fmaxf(w[0], w[1])), fmaxf(w[2], w[3]));
       }
     }
     if (F16) {
-      if (__any_sync(0xffffffffu, large) || moves) {
+      if (__any_sync(0xffffffffu, most > PA_SHARE) || moves) {
         #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           #pragma unroll
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
     const int count = to - from > warp ? (to - from - warp + PA_WARPS - 1) / PA_WARPS : 0;      // steps of this warp: from + warp + 4 j
     const int* ids = a.table.ids + (long long)b * a.table.width;
     int id = -1, valid[C::STAGES - 1];
-    // starts the copies of step j; the tokens of its boxes (8 bits each), 0 where there is no page
+    // Starts the copies of step j, a lane for each box; the tokens of its boxes (8 bits each), 0 where there is no page.
     auto issue = [&](int j) -> int {
       if (j >= count) return 0;
       if (j % PER == 0) {
@@ -525,38 +525,29 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
           if (id < 0 || id >= a.table.pages) { report_bad_index(a.table.status); id = -1; }
         }
       }
-      int real_tokens = 0, boxes = 0, page[SUB];
-      const int t0 = (from + warp + PA_WARPS * j) * C::STEP;
-      #pragma unroll
-      for (int i = 0; i < SUB; ++i) {
-        page[i] = __shfl_sync(0xffffffffu, id, j % PER * SUB + i);
-        if (page[i] < 0) continue;
-        ++boxes;
-        real_tokens |= min(PA_BOX, n - t0 - i * PA_BOX) << (8 * i);
-      }
-      if (boxes == 0 || !alive) return 0;
-      if (lane == 0) {
-        uint64_t* bar = &full[warp][put];
-        mbar_expect_tx(bar, boxes * C::LOADED);
+      const int page = __shfl_sync(0xffffffffu, id, j % PER * SUB + lane % SUB), t0 = (from + warp + PA_WARPS * j) * C::STEP + lane * PA_BOX;
+      const bool mine = lane < SUB && page >= 0 && alive;
+      const unsigned boxes = __ballot_sync(0xffffffffu, mine);
+      if (boxes == 0) return 0;
+      uint64_t* bar = &full[warp][put];
+      if (lane == 0) mbar_expect_tx(bar, __popc(boxes) * C::LOADED);
+      __syncwarp();
+      if (mine) {
+        const int slot = ((page * a.Hk + hk) << a.table.page_shift) + (t0 & page_mask);      // below 2^31: the host sees to it
+        uint8_t* dst = my_ring + put * C::STAGE + lane * 2 * C::BOX;
         #pragma unroll
-        for (int i = 0; i < SUB; ++i) {
-          if (page[i] < 0) continue;
-          const int slot = ((page[i] * a.Hk + hk) << a.table.page_shift) + ((t0 + i * PA_BOX) & page_mask);      // below 2^31: the host sees to it
-          uint8_t* dst = my_ring + put * C::STAGE + i * 2 * C::BOX;
-          #pragma unroll
-          for (int k = 0; k < C::TILES; ++k) {
-            tma_load_2d(dst + k * PA_BOX * C::TILE, &kmap, k * C::TILE / C::BYTES, slot, bar);
-            tma_load_2d(dst + C::BOX + k * PA_BOX * C::TILE, &vmap, k * C::TILE / C::BYTES, slot, bar);
-          }
-          if (T != KV_BF16) {
-            float* sc = scales[warp * C::STAGES + put] + i * 2 * PA_BOX;
-            bulk_load(sc, a.scales[0] + slot, PA_BOX * 4, bar);
-            bulk_load(sc + PA_BOX, a.scales[1] + slot, PA_BOX * 4, bar);
-          }
+        for (int k = 0; k < C::TILES; ++k) {
+          tma_load_2d(dst + k * PA_BOX * C::TILE, &kmap, k * C::TILE / C::BYTES, slot, bar);
+          tma_load_2d(dst + C::BOX + k * PA_BOX * C::TILE, &vmap, k * C::TILE / C::BYTES, slot, bar);
+        }
+        if (T != KV_BF16) {
+          float* sc = scales[warp * C::STAGES + put] + lane * 2 * PA_BOX;
+          bulk_load(sc, a.scales[0] + slot, PA_BOX * 4, bar);
+          bulk_load(sc + PA_BOX, a.scales[1] + slot, PA_BOX * 4, bar);
         }
       }
       put = put + 1 == C::STAGES ? 0 : put + 1;
-      return real_tokens;
+      return (int)__reduce_or_sync(0xffffffffu, mine ? (unsigned)min(PA_BOX, n - t0) << (8 * lane) : 0u);
     };
     #pragma unroll
     for (int j = 0; j < C::STAGES - 1; ++j) valid[j] = issue(j);
