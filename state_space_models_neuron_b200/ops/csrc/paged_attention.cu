@@ -637,6 +637,23 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
         constexpr int LOOK = THREADS / HEADS;
         auto part = [&](int k) -> const float* { return a.ws + ((long long)(c0 + k) * 2 + (k == 0)) * C::SLOT; };
         float* factors = os;                   // [part][head]
+        // Up to 32 loads of a thread under way: of each of its channels from some parts.  The first come while the factors are found.
+        constexpr int MANY = D * HEADS / 4 / THREADS, AT_ONCE = MANY > 2 || C::BLOCKS > 2 ? 8 : 16;
+        const int d0 = threadIdx.x / fours, dd = THREADS / fours;
+        float4 acc[MANY], v[AT_ONCE][MANY];
+        auto load = [&](int k0) {
+          #pragma unroll
+          for (int k = 0; k < AT_ONCE; ++k) {
+            #pragma unroll
+            for (int i = 0; i < MANY; ++i) {
+              v[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (k0 + k < parts && d0 + i * dd < D) v[k][i] = *reinterpret_cast<const float4*>(part(k0 + k) + (d0 + i * dd) * HEADS + h);
+            }
+          }
+        };
+        load(0);
+        #pragma unroll
+        for (int i = 0; i < MANY; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         const int head = threadIdx.x % HEADS;
         float mm = -INFINITY, MM = -INFINITY, sum = 0.f;
         #pragma unroll 4
@@ -671,22 +688,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
           stats[0][head] = out_factor(mm, MM, sum);
         }
         __syncthreads();
-        // up to 32 loads of a thread under way: of each of its channels from some parts
-        constexpr int MANY = D * HEADS / 4 / THREADS, AT_ONCE = MANY > 2 ? 8 : 16;
-        float4 acc[MANY];
-        #pragma unroll
-        for (int i = 0; i < MANY; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        const int d0 = threadIdx.x / fours, dd = THREADS / fours;
-        for (int k0 = 0; k0 < parts; k0 += AT_ONCE) {
-          float4 v[AT_ONCE][MANY];
-          #pragma unroll
-          for (int k = 0; k < AT_ONCE; ++k) {
-            #pragma unroll
-            for (int i = 0; i < MANY; ++i) {
-              v[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (k0 + k < parts && d0 + i * dd < D) v[k][i] = *reinterpret_cast<const float4*>(part(k0 + k) + (d0 + i * dd) * HEADS + h);
-            }
-          }
+        for (int k0 = 0;;) {
           #pragma unroll
           for (int k = 0; k < AT_ONCE; ++k) {
             if (k0 + k >= parts) break;
@@ -694,6 +696,9 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
             #pragma unroll
             for (int i = 0; i < MANY; ++i) { acc[i].x += f.x * v[k][i].x; acc[i].y += f.y * v[k][i].y; acc[i].z += f.z * v[k][i].z; acc[i].w += f.w * v[k][i].w; }
           }
+          k0 += AT_ONCE;
+          if (k0 >= parts) break;
+          load(k0);
         }
         #pragma unroll
         for (int i = 0; i < MANY; ++i) {

@@ -148,8 +148,11 @@ def test_training_step_in_a_graph():
     from state_space_models_neuron_b200.parallel.graph import GraphedTrainStep
     ids = tokens(2, 128)
 
+    weights = build().state_dict()                                 # every construction draws others
+
     def start():
         model = build().train()
+        model.load_state_dict(weights)
         cfg = nxd.parallel_config(1, {"zero_one_enabled": True})
         return model, nxd.initialize_parallel_optimizer(cfg, nxd.AdamW_FP32OptimParams, [{"params": list(model.parameters())}], lr=1e-3)
 
