@@ -99,8 +99,12 @@ template <int N>
 __device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 constexpr int EACH = 8;                        // most heads that a group of lanes takes one after the other
 
-// 1 / sqrt(mean + eps), correctly rounded: an error here moves whole rows
+// 1 / sqrt(mean + eps) to about a rounding: an error here moves whole rows.  One Newton step on the approximation, except where that is
+// zero or infinite.
 template <int D>
-__device__ __forceinline__ float rms_factor(float sum_of_squares, float eps) { return __frsqrt_rn(sum_of_squares * (1.f / D) + eps); }
+__device__ __forceinline__ float rms_factor(float sum_of_squares, float eps) {
+  const float a = fmaf(sum_of_squares, 1.f / D, eps), r = rsqrtf(a);
+  return a > 0.f && a < INFINITY ? fmaf(0.5f * r, fmaf(-a * r, r, 1.f), r) : r;
+}
 
 }  // namespace ssm

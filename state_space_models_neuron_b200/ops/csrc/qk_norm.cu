@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(NORM_THREADS, 2) qk_norm_bwd_kernel(const Norm
   const int turns = mine < all ? (int)((all - mine + warps - 1) / warps) : 0, total = turns * each;
 
   // where a turn's rows are
-  struct Place { int token, l, h0, h1; long long x, g; };
+  struct Place { int token, l, h0, h1; const __nv_bfloat16 *x, *g; };
   auto place = [&](int turn) -> Place {
     const long long u = mine + turn * warps, tb = u / units;
     const long long token = tb * TOKENS + threadIdx.x % 32 / LANES;
@@ -125,8 +125,8 @@ __global__ void __launch_bounds__(NORM_THREADS, 2) qk_norm_bwd_kernel(const Norm
     p.l = p.token - b * a.L;
     p.h0 = (int)(u - tb * units) * each;
     p.h1 = real ? min(t.heads, p.h0 + each) : 0;
-    p.x = b * t.xb + p.l * t.xl + p.h0 * t.xh;
-    p.g = b * t.gb + p.l * t.gl + p.h0 * t.gh;
+    p.x = t.x + b * t.xb + p.l * t.xl + p.h0 * t.xh;
+    p.g = t.dy + b * t.gb + p.l * t.gl + p.h0 * t.gh;
     return p;
   };
   Place ahead;
@@ -134,14 +134,14 @@ __global__ void __launch_bounds__(NORM_THREADS, 2) qk_norm_bwd_kernel(const Norm
   auto fetch = [&](int j) {
     if (j < total) {
       if (ahead_i == each) { ahead = place(++ahead_turn); ahead_i = 0; }
-      const bool some = ahead.h0 + ahead_i < ahead.h1;
-      const __nv_bfloat16* x = t.x + (some ? ahead.x + ahead_i * t.xh : 0);
-      const __nv_bfloat16* g = t.dy + (some ? ahead.g + ahead_i * t.gh : 0);
+      const bool some = ahead.h0 + ahead_i < ahead.h1;          // the address of a row that does not exist is not read
       uint4* to = slots + (j % GRAD_DEPTH) * 4 * NORM_THREADS + threadIdx.x;
-      fetch16(to, x + at.c0, some);
-      fetch16(to + NORM_THREADS, x + at.c1, some);
-      fetch16(to + 2 * NORM_THREADS, g + at.c0, some);
-      fetch16(to + 3 * NORM_THREADS, g + at.c1, some);
+      fetch16(to, ahead.x + at.c0, some);
+      fetch16(to + NORM_THREADS, ahead.x + at.c1, some);
+      fetch16(to + 2 * NORM_THREADS, ahead.g + at.c0, some);
+      fetch16(to + 3 * NORM_THREADS, ahead.g + at.c1, some);
+      ahead.x += t.xh;
+      ahead.g += t.gh;
       ++ahead_i;
     }
     fetch_commit();
