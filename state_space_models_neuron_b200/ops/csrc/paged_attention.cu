@@ -24,9 +24,11 @@
 
 namespace ssm {
 
-constexpr int PA_WARPS = 4, PA_BOX = 16, PA_COUNTERS = 768;      // PA_BOX: tokens of a box
-constexpr int PA_MIN_SHARE = 4 * PA_WARPS;     // steps: four per warp (two: 200 tokens 8.3 us instead of 7.0, a join that saves nothing; eight: 2048 tokens 12.5 instead of 10.2)
-constexpr int FEW_ITEMS = 8;                   // blocks per item, see the kernel
+constexpr int PA_WARPS = 4, PA_BOX = 16, PA_COUNTERS = 2048;     // PA_BOX: tokens of a box
+// Steps of a block (few items) and of a warp that make a share.  Blocks: four steps per warp (two: 200 tokens 8.3 us instead of 7.0, a join that saves
+// nothing; eight: 2048 tokens 12.5 instead of 10.2).
+constexpr int PA_BLOCK_SHARE = 4 * PA_WARPS, PA_WARP_SHARE = 4;
+constexpr int FEW_ITEMS = 8, LONG_ITEM = 48;   // blocks per item and steps of an item, see the kernel
 // A running maximum moves when scores pass it by 2^8: bf16 and fp16 hold larger shares as well.
 constexpr float PA_GROWTH = 8.f, PA_SHARE = 256.f;
 
@@ -61,7 +63,7 @@ struct PagedAttn {
   static constexpr int BLOCKS = SMEM > 113 * 1024 ? 1 : NT == 1 && (ROW == 64 || (ROW == 128 && T == KV_INT8)) ? 3 : 2;
   static constexpr int SLOT = HEADS * D + 3 * HEADS;           // floats of a part: o [channel][head], m, sum, M
   static constexpr int MEET = D * HEADS + D / VEL * 8;         // floats of a warp's o where the warps meet, see leave()
-  static_assert(PA_WARPS * MEET * 4 <= RING && PA_COUNTERS * HEADS * 4 <= RING, "the warps' results meet in the ring");
+  static_assert(PA_WARPS * MEET * 4 <= RING && PA_COUNTERS / PA_WARPS * HEADS * 4 <= RING, "the warps' results meet in the ring");
 };
 
 // Token of row g of S^T (and of row g + 8, eight further), and 16-byte piece of a 128-byte row of V that lane group g takes: 0 4 1 5
@@ -290,7 +292,7 @@ struct AttnWarp {
           s[u][nt][i] = e;
           w[i] = e * (vs[u][i >> 1] * G[nt][i & 1]);
         }
-        if (F16) most = fmaxf(fmaxf(most, fmaxf(w[0], w[1])), fmaxf(w[2], w[3]));
+        if (F16) most = fmaxf(fmaxf(most, fmaxf(fabsf(w[0]), fabsf(w[1]))), fmaxf(fabsf(w[2]), fabsf(w[3])));
       }
     }
     if (F16) {
@@ -380,6 +382,101 @@ struct AttnWarp {
     }
   }
 
+  __device__ __forceinline__ void add_sums() {
+    #pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      #pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        #pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], d);
+      }
+    }
+  }
+  // the result, for sums over the whole warp
+  __device__ __forceinline__ void store(__nv_bfloat16* out, int real) {
+    const int g = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3;
+    #pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      #pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int head = nt * 8 + 2 * c + j;
+        if (head >= real) continue;
+        const float f = out_factor(m[nt][j], F16 ? M[nt][j] : m[nt][j], l[nt][j]);
+        #pragma unroll
+        for (int k = 0; k < C::TILES; ++k) {
+          uint32_t w[C::VEL / 2];
+          #pragma unroll
+          for (int e = 0; e < C::VEL / 2; ++e) {
+            const int t = k * (C::VEL / 2) + e;
+            w[e] = pack_bf16(o[nt][t][j] * f, o[nt][t][j + 2] * f);
+          }
+          uint4* at = reinterpret_cast<uint4*>(out + head * D + (k * 8 + sigma<C::TILE>(g)) * C::VEL);
+          #pragma unroll
+          for (int e = 0; e < C::VEL / 8; ++e) at[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        }
+      }
+    }
+  }
+  // A part of an item: what the lanes hold, [register][lane], and (m, sum, M) of the heads.
+  __device__ __forceinline__ void leave_part(float* slot) {
+    const int lane = threadIdx.x & 31, c = lane & 3;
+    #pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      #pragma unroll
+      for (int t = 0; t < D / 16; ++t)
+        reinterpret_cast<float4*>(slot)[(nt * (D / 16) + t) * 32 + lane] = make_float4(o[nt][t][0], o[nt][t][1], o[nt][t][2], o[nt][t][3]);
+      if (lane >= 4) continue;
+      #pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float* st = slot + C::HEADS * D + nt * 8 + 2 * c + j;
+        st[0] = fresh ? -INFINITY : m[nt][j];
+        st[C::HEADS] = l[nt][j];
+        st[2 * C::HEADS] = fresh ? -INFINITY : F16 ? M[nt][j] : m[nt][j];
+      }
+    }
+  }
+  // the parts of an item, in their order
+  template <typename Part>
+  __device__ __forceinline__ void join(int parts, Part part) {
+    const int lane = threadIdx.x & 31, c = lane & 3;
+    reset();
+    #pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      #pragma unroll
+      for (int j = 0; j < 2; ++j) m[nt][j] = M[nt][j] = -INFINITY;
+    }
+    #pragma unroll 4
+    for (int k = 0; k < parts; ++k) {
+      #pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        #pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float* st = part(k) + C::HEADS * D + nt * 8 + 2 * c + j;
+          m[nt][j] = fmaxf(m[nt][j], st[0]);
+          M[nt][j] = fmaxf(M[nt][j], st[2 * C::HEADS]);
+        }
+      }
+    }
+    for (int k = 0; k < parts; ++k) {
+      const float* p = part(k);
+      #pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float f[2];
+        #pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float* st = p + C::HEADS * D + nt * 8 + 2 * c + j;
+          l[nt][j] += st[C::HEADS] * part_factor(st[0], m[nt][j]);
+          f[j] = part_factor(st[2 * C::HEADS], M[nt][j]);
+        }
+        #pragma unroll
+        for (int t = 0; t < D / 16; ++t) {
+          const float4 v = reinterpret_cast<const float4*>(p)[(nt * (D / 16) + t) * 32 + lane];
+          o[nt][t][0] += f[0] * v.x; o[nt][t][1] += f[1] * v.y; o[nt][t][2] += f[0] * v.z; o[nt][t][3] += f[1] * v.w;
+        }
+      }
+    }
+  }
+
   // o into `to`, [channel][head] with 8 floats between the pieces of neighbouring lane groups (their banks would be the same);
   // lanes with g == 0 put (m, sum, M) of their heads into `stats`
   __device__ __forceinline__ void leave(float* to, float* stats) {
@@ -396,12 +493,9 @@ struct AttnWarp {
       }
       #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float sum = l[nt][j];
-        #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (g == 0) {
           stats[head + j] = fresh ? -INFINITY : m[nt][j];
-          stats[C::HEADS + head + j] = sum;
+          stats[C::HEADS + head + j] = l[nt][j];
           stats[2 * C::HEADS + head + j] = fresh ? -INFINITY : F16 ? M[nt][j] : m[nt][j];
         }
       }
@@ -433,10 +527,13 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
   pdl_trigger();
   pdl_wait();
 
-  // Where this block's share begins.  The steps of all sequences and heads stand in a row, each sequence's heads one behind the other;
+  // Where this worker's share begins.  The steps of all sequences and heads stand in a row, each sequence's heads one behind the other;
   // sequences in the order lane, lane + 32, ... of the lanes that look at them (every warp finds the same).
-  // Many of them (items): blocks cut the row at equal distances, wherever that is.  Few: every item is cut by itself, so that no
-  // block has parts of two, at the price of up to one shorter share per item.
+  // Workers cut the row at equal distances, wherever that is.  Only where there are few items is every item cut by itself, so that no worker
+  // has parts of two, at the price of up to one shorter share per item.
+  // Workers are blocks, whose warps take every fourth step and meet at the end of a piece, or, where items are short, warps, which never
+  // wait for each other (256 of 200 tokens, bf16 and e4m3, us: blocks 52.5 and 51.7, warps 44.6 and 33.8).  Blocks read longer stretches of
+  // memory at a time (64 x 8192 bf16 319, warps 328; 64 x 2048 87 and 91, e4m3 55.0 and 55.5).
   auto steps_of = [&](int b) -> int { return (tokens_of(a, b) + C::STEP - 1) / C::STEP; };
   const int first_steps = lane < a.B ? steps_of(lane) : 0;
   int mine = first_steps * items, some = first_steps > 0;
@@ -454,25 +551,27 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
     }
   }
   const bool few = (long long)filled * items * FEW_ITEMS <= a.most_blocks;
-  const int blocks = few ? a.most_blocks : gridDim.x;
-  int share = max(PA_MIN_SHARE, ((total + blocks - 1) / blocks + PA_WARPS - 1) / PA_WARPS * PA_WARPS);
+  const bool team = few || total >= (long long)filled * items * LONG_ITEM;
+  const int workers = few ? a.most_blocks : team ? gridDim.x : gridDim.x * PA_WARPS, me = team ? blockIdx.x : blockIdx.x * PA_WARPS + warp;
+  int share = (total + workers - 1) / workers;
+  share = team ? max(PA_BLOCK_SHARE, (share + PA_WARPS - 1) / PA_WARPS * PA_WARPS) : max(PA_WARP_SHARE, share);
   if (few) {
     // The smallest share of which there are at most most_blocks; the last guess always fits.  Counted in shares from here on.
-    const int fits = max(PA_MIN_SHARE, ((total + blocks - filled * items - 1) / (blocks - filled * items) + PA_WARPS - 1) / PA_WARPS * PA_WARPS);
+    const int rest = workers - filled * items, fits = max(PA_BLOCK_SHARE, ((total + rest - 1) / rest + PA_WARPS - 1) / PA_WARPS * PA_WARPS);
     for (int guess = 0;; ++guess, share += PA_WARPS) {
       if (guess == 3 || share > fits) share = fits;
       mine = (first_steps + share - 1) / share * items;
       for (int b = lane + 32; b < a.B; b += 32) mine += (steps_of(b) + share - 1) / share * items;
       total = __reduce_add_sync(0xffffffffu, mine);
-      if (total <= blocks || share == fits) break;
+      if (total <= workers || share == fits) break;
     }
     upto = mine;
     #pragma unroll
     for (int d = 1; d < 32; d <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += v; }
   }
-  const int unit = few ? 1 : share;            // of the row, per block
-  if ((long long)unit * blockIdx.x >= total) return;
-  int u = unit * blockIdx.x;
+  const int unit = few ? 1 : share;            // of the row, per worker
+  if ((long long)unit * me >= total) return;
+  int u = unit * me;
   const int end = total - u < unit ? total : u + unit;
   int b = lane, seq0 = upto - mine;            // first step (share) of sequence b in the row
   const bool here = seq0 <= u && u < upto;
@@ -495,37 +594,48 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
   uint32_t parity = 0;                         // of the next to read
   bool alive = true;                           // no wait of this warp has run out
 
-  while (u < end) {
-    const int n = tokens_of(a, b), steps = (n + C::STEP - 1) / C::STEP, row = few ? (steps + share - 1) / share : steps;   // row: of an item
-    if (u >= seq0 + row * items) {
-      seq0 += row * items;
-      b += 32;
-      if (b >= a.B) b = (b & 31) + 1;
-      continue;
+  // A piece of the share: steps of one item.
+  struct Piece { int b, n, from, to, c0, parts, hk, head0, real; };
+  auto take = [&](Piece& p) -> bool {
+    while (u < end) {
+      const int n = tokens_of(a, b), steps = (n + C::STEP - 1) / C::STEP, row = few ? (steps + share - 1) / share : steps;   // row: of an item
+      if (u >= seq0 + row * items) {
+        seq0 += row * items;
+        b += 32;
+        if (b >= a.B) b = (b & 31) + 1;
+        continue;
+      }
+      const int item = (u - seq0) / row, at = (u - seq0) % row, item0 = seq0 + item * row, first = item % a.groups * HEADS;
+      p.b = b;
+      p.n = n;
+      p.from = few ? at * share : at;
+      p.to = min(steps, p.from + (few ? share : end - u));
+      p.c0 = item0 / unit;
+      p.parts = (item0 + row - 1) / unit - p.c0 + 1;             // workers that share the item
+      p.hk = item / a.groups;
+      p.head0 = p.hk * a.ratio + first;
+      p.real = min(HEADS, a.ratio - first);
+      u += few ? 1 : p.to - p.from;
+      return true;
     }
-    const int item = (u - seq0) / row, at = (u - seq0) % row;
-    const int from = few ? at * share : at, to = min(steps, from + (few ? share : end - u));
-    const int item0 = seq0 + item * row;
-    const int c0 = item0 / unit, parts = (item0 + row - 1) / unit - c0 + 1;    // blocks that share the item
-    const int hk = item / a.groups, first = (item % a.groups) * HEADS, real = min(HEADS, a.ratio - first);
-    const int head0 = hk * a.ratio + first;
-
-    const int count = to - from > warp ? (to - from - warp + PA_WARPS - 1) / PA_WARPS : 0;      // steps of this warp: from + warp + 4 j
-    const int* ids = a.table.ids + (long long)b * a.table.width;
-    int id = -1, valid[C::STAGES - 1];
+    return false;
+  };
+  Piece cur = {};
+  const int stride = team ? PA_WARPS : 1, offset = team ? warp : 0;              // steps of this warp: from + offset + stride j
+  int count = 0, id = -1, valid[C::STAGES - 1];
     // Starts the copies of step j, a lane for each box; the tokens of its boxes (8 bits each), 0 where there is no page.
     auto issue = [&](int j) -> int {
       if (j >= count) return 0;
       if (j % PER == 0) {
         // the pages of the boxes of this warp's next steps, one per lane
-        const int k = j + lane / SUB, t = (from + warp + PA_WARPS * k) * C::STEP + lane % SUB * PA_BOX;
+        const int k = j + lane / SUB, t = (cur.from + offset + stride * k) * C::STEP + lane % SUB * PA_BOX;
         id = -1;
-        if (k < count && t < n) {
-          id = ids[t >> a.table.page_shift];
+        if (k < count && t < cur.n) {
+          id = a.table.ids[(long long)cur.b * a.table.width + (t >> a.table.page_shift)];
           if (id < 0 || id >= a.table.pages) { report_bad_index(a.table.status); id = -1; }
         }
       }
-      const int page = __shfl_sync(0xffffffffu, id, j % PER * SUB + lane % SUB), t0 = (from + warp + PA_WARPS * j) * C::STEP + lane * PA_BOX;
+      const int page = __shfl_sync(0xffffffffu, id, j % PER * SUB + lane % SUB), t0 = (cur.from + offset + stride * j) * C::STEP + lane * PA_BOX;
       const bool mine = lane < SUB && page >= 0 && alive;
       const unsigned boxes = __ballot_sync(0xffffffffu, mine);
       if (boxes == 0) return 0;
@@ -533,7 +643,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
       if (lane == 0) mbar_expect_tx(bar, __popc(boxes) * C::LOADED);
       __syncwarp();
       if (mine) {
-        const int slot = ((page * a.Hk + hk) << a.table.page_shift) + (t0 & page_mask);      // below 2^31: the host sees to it
+        const int slot = ((page * a.Hk + cur.hk) << a.table.page_shift) + (t0 & page_mask);      // below 2^31: the host sees to it
         uint8_t* dst = my_ring + put * C::STAGE + lane * 2 * C::BOX;
         #pragma unroll
         for (int k = 0; k < C::TILES; ++k) {
@@ -547,11 +657,18 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
         }
       }
       put = put + 1 == C::STAGES ? 0 : put + 1;
-      return (int)__reduce_or_sync(0xffffffffu, mine ? (unsigned)min(PA_BOX, n - t0) << (8 * lane) : 0u);
+      return (int)__reduce_or_sync(0xffffffffu, mine ? (unsigned)min(PA_BOX, cur.n - t0) << (8 * lane) : 0u);
     };
+  // takes the next piece and starts its first copies
+  auto begin = [&]() -> bool {
+    if (!take(cur)) return false;
+    count = max(0, (cur.to - cur.from - offset + stride - 1) / stride);
     #pragma unroll
     for (int j = 0; j < C::STAGES - 1; ++j) valid[j] = issue(j);
-    x.load_queries(a, a.q + b * a.qb + head0 * a.qh, real);
+    return true;
+  };
+  for (bool more = begin(); more;) {
+    x.load_queries(a, a.q + cur.b * a.qb + cur.head0 * a.qh, cur.real);
     x.reset();
     for (int j = 0; j < count; ++j) {
       const int now = valid[0];
@@ -571,16 +688,38 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
       __syncwarp();                            // before the next copies into this stage
     }
 
-    // the warps meet
+    const Piece p = cur;
+    const int real = p.real, parts = p.parts, c0 = p.c0;
+    const bool whole = parts == 1;
+    float* slot = whole ? nullptr : a.ws + ((long long)me * 2 + (c0 == me)) * C::SLOT;
+    auto part = [&](int k) -> const float* { return a.ws + ((long long)(c0 + k) * 2 + (k == 0)) * C::SLOT; };     // the first worker's is its second
+    __nv_bfloat16* out = a.out + ((long long)p.b * a.Hq + p.head0) * D;
+    x.add_sums();
+    if (!team) {
+      more = begin();                          // under way while this one is brought to its end
+      if (!whole) {
+        x.leave_part(slot);
+        __syncwarp();
+        int before = 0;
+        if (lane == 0) {
+          before = arrive(a.counters + c0);
+          if (before == parts - 1) a.counters[c0] = 0;
+        }
+        if (__shfl_sync(0xffffffffu, before, 0) != parts - 1) continue;
+        __syncwarp();                          // what lane 0 has seen, all have
+        x.join(parts, part);                   // all parts are there
+      }
+      x.store(out, real);
+      continue;
+    }
+
+    // the warps of a block meet
     float* os = reinterpret_cast<float*>(ring);
     __syncthreads();
     x.leave(os + warp * C::MEET, stats[warp]);
     __syncthreads();
-    const bool whole = parts == 1;
     // threads take a channel of four heads at a time, always the same heads
     const int fours = real <= 4 ? 1 : real <= 8 ? 2 : 4, h = threadIdx.x % fours * 4;
-    float* slot = whole ? nullptr : a.ws + ((long long)blockIdx.x * 2 + (c0 == (int)blockIdx.x)) * C::SLOT;
-    __nv_bfloat16* out = a.out + ((long long)b * a.Hq + head0) * D;
     {
       float f[PA_WARPS][4], mm[4], MM[4], sum[4];
       #pragma unroll
@@ -632,10 +771,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
       }
       __syncthreads();
       if (arrived == parts - 1) {
-        // All parts are there: joined in the order of the blocks (the first one holds its part in its second slot).  A thread looks at
-        // one head of every LOOK-th part for the largest m and M, then leaves the parts' factors in the ring.
+        // All parts are there: joined in the order of the blocks.  A thread looks at one head of every LOOK-th part for the largest m and M, then leaves the parts' factors in the ring.
         constexpr int LOOK = THREADS / HEADS;
-        auto part = [&](int k) -> const float* { return a.ws + ((long long)(c0 + k) * 2 + (k == 0)) * C::SLOT; };
         float* factors = os;                   // [part][head]
         // Up to 32 loads of a thread under way: of each of its channels from some parts.  The first come while the factors are found.
         constexpr int MANY = D * HEADS / 4 / THREADS, AT_ONCE = MANY > 2 || C::BLOCKS > 2 ? 8 : 16;
@@ -710,9 +847,9 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
         }
       }
     }
-    u += few ? 1 : to - from;
     fence_proxy_async_smem();
     __syncthreads();                           // the ring, for TMA to write, and the statistics are free again
+    more = begin();
   }
 }
 
@@ -756,13 +893,13 @@ static int paged_attn_plan(int type, int width, int page_size, int B, int Hq, in
   // no more blocks than there can be shares
   const long long items = (long long)B * Hk * ((ratio + group - 1) / group), most = items * (((long long)width * page_size + step - 1) / step);
   if (most > 0x7fffffffll - (1 << 20)) return -SSM_ERR_BAD_ARG;                // counted in 32 bits
-  const long long shares = (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE + items;
+  const long long shares = (most + PA_BLOCK_SHARE - 1) / PA_BLOCK_SHARE + items;
   long long n = (long long)sms * blocks;
-  if (n > PA_COUNTERS) n = PA_COUNTERS;
+  if (n > PA_COUNTERS / PA_WARPS) n = PA_COUNTERS / PA_WARPS;
   *most_blocks = (int)n;
   if (n > shares) n = shares;
   *grid = n < 1 ? 1 : (int)n;
-  *floats = (long long)*grid * 2 * slot;
+  *floats = (long long)*grid * PA_WARPS * 2 * slot;
   return 0;
 }
 

@@ -1444,13 +1444,16 @@ class _QKNormRotary(torch.autograd.Function):
         (g, g_at, gs), (h, h_at, hs) = _head_view(dqo), _head_view(dko)
         dq = torch.empty((B, L, Hq, D), dtype=torch.bfloat16, device=dev)
         dk = torch.empty((B, L, Hk, D), dtype=torch.bfloat16, device=dev)
-        grads, targets, adds = [None, None], [None, None], [0, 0]
+        grads, targets, adds, second = [None, None], [None, None], [0, 0], None
         for i, w in enumerate((qw, kw)):
             if not need[2 + i]:
                 continue
             mg = getattr(w, "main_grad", None) if w.is_leaf else None
             if mg is None or mg.dtype is not torch.float32 or not (B and L):
                 grads[i] = targets[i] = torch.empty((D,), dtype=w.dtype, device=dev)
+                continue
+            if mg is targets[0]:               # one weight of both: the kernel adds to it once
+                second, targets[i] = mg, torch.empty_like(mg)
                 continue
             # the optimizer's fp32 gradient: stored by the first contribution of a step, added to by the others
             targets[i], adds[i] = mg, int(not getattr(w, "grad_stale", False))
@@ -1463,6 +1466,8 @@ class _QKNormRotary(torch.autograd.Function):
                                                 _at(positions), status_tensor(dev).data_ptr(), part.data_ptr(), _at(targets[0]),
                                                 _at(targets[1]), *ctx.strides, *gs, *hs, *ctx.call, _is32(targets[0]), _is32(targets[1]),
                                                 *adds, ctx.eps), _st())
+        if second is not None:
+            second.add_(targets[1])
         return dq, dk, *grads, None, None, None, None
 
 

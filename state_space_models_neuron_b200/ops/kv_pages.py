@@ -6,7 +6,7 @@ A page holds `page_size` tokens of every key/value head, a head's tokens one beh
 the token so that the attention kernel reads a head's page as one piece of page_size * head_dim values.
 
 Values are bfloat16, or 8-bit (float8_e4m3fn, int8) with one fp32 scale per token and head in `k_scale` / `v_scale`
-[pages, kv_heads, page_size]; a stored value stands for value * scale.
+[pages, kv_heads, page_size], not negative; a stored value stands for value * scale.
 """
 from __future__ import annotations
 
@@ -78,6 +78,8 @@ def check_heads(q, k, cos, sin, positions, from_zero: bool) -> None:
     shape = k.shape
     if len(shape) != 4 or (q is not None and (q.dim() != 4 or q.shape[:2] != shape[:2] or q.shape[3] != shape[3])):
         raise ValueError("queries and keys are [batch, tokens, heads, head_dim] with the same batch, tokens and head_dim")
+    if shape[2] < 1 or (q is not None and q.shape[2] < 1):
+        raise ValueError("queries and keys have at least one head")
     if cos is None and sin is None:
         if positions is not None:
             raise ValueError("positions without cos and sin")

@@ -191,7 +191,7 @@ def test_attention(dtype, Hq, Hk, D, page):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("lengths", [(1,), (20000,), (3, 12345), (4096, 4095, 4097), (777,) * 70, (1,) * 300, (9000,) + (1,) * 40])
+@pytest.mark.parametrize("lengths", [(1,), (20000,), (3, 12345), (4096, 4095, 4097), (777,) * 70, (1,) * 300, (3000, 100) * 30, (9000,) + (1,) * 40])
 def test_attention_over_lengths_and_batches(dtype, lengths):
     pages, table = filled(len(lengths), lengths, 2, 128, 64, TYPES[dtype], 11)
     q = draw((len(lengths), 1, 8, 128), 6, 1.5)
@@ -260,10 +260,10 @@ def test_query_layouts():
     assert torch.equal(shared[0], good[0]) and torch.equal(shared[1], good[0])
 
 
-def test_runs_give_the_same_bits():
-    lengths = (5000, 1, 777, 20000)
-    pages, table = filled(4, lengths, 2, 128, 64, torch.bfloat16, 29)
-    q = draw((4, 1, 8, 128), 12)
+@pytest.mark.parametrize("lengths", [(5000, 1, 777, 20000), (200, 37) * 60, (2000, 2500) * 20])
+def test_runs_give_the_same_bits(lengths):
+    pages, table = filled(len(lengths), lengths, 2, 128, 64, torch.bfloat16, 29)
+    q = draw((len(lengths), 1, 8, 128), 12)
     first = ops.paged_attention(q, pages, table, ints(*lengths))
     for _ in range(20):
         assert torch.equal(ops.paged_attention(q, pages, table, ints(*lengths)), first)

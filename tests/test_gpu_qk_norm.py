@@ -141,6 +141,21 @@ def test_gradients_go_to_the_optimizer_buffer():
         assert torch.equal(t.main_grad, f + f)
 
 
+def test_one_weight_of_both_goes_to_the_optimizer_buffer():
+    q, k, dq, dk, qw, _ = inputs(2, 700, 4, 2, 128, True, 23)
+    w = qw.clone().requires_grad_()
+    torch.autograd.backward(ops.qk_norm_rotary(q, k, w, w, EPS), (dq, dk))
+    for stale in (True, False):
+        t = qw.clone().requires_grad_()
+        t.main_grad = torch.full((128,), 3.0, device="cuda")
+        t.grad_stale = stale
+        torch.autograd.backward(ops.qk_norm_rotary(q, k, t, t, EPS), (dq, dk))
+        want = w.grad + (0.0 if stale else 3.0)
+        assert t.grad is None and not t.grad_stale
+        # one fp32 addition more, in another order
+        assert ((t.main_grad - want).abs() <= 2 ** -22 * (want.abs() + 3.0 + w.grad.abs().max())).all()
+
+
 def test_runs_give_the_same_bits():
     q, k, dq, dk, qw, kw = inputs(2, 1500, 8, 2, 128, True, 15)
     cos, sin = tables(1500, 128)
