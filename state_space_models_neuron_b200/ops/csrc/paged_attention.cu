@@ -278,7 +278,9 @@ struct AttnWarp {
         }
       }
     }
-    uint32_t p[SUB][NT][2];
+    // 16-bit probabilities beside bf16 values come in two pieces, which have 16 bits of mantissa between them: their rounding to one would
+    // add as much to the error as that of the result does (2.3e-3 instead of 1.7e-3), and the products have time (1 %).  fp16 has 11 bits.
+    uint32_t p[SUB][NT][2], rest[SUB][NT][2];
     most = 0.f;
     #pragma unroll
     for (int u = 0; u < SUB; ++u) {
@@ -325,8 +327,18 @@ struct AttnWarp {
         float w[4];
         #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = F16 ? s[u][nt][i] * (vs[u][i >> 1] * G[nt][i & 1]) : s[u][nt][i];
-        p[u][nt][0] = transpose8x8(F16 ? pack_f16(w[0], w[1]) : pack_bf16(w[0], w[1]));
-        p[u][nt][1] = transpose8x8(F16 ? pack_f16(w[2], w[3]) : pack_bf16(w[2], w[3]));
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float a = w[2 * i], b = w[2 * i + 1];
+          if (F16) {
+            p[u][nt][i] = transpose8x8(pack_f16(a, b));
+          } else {
+            // the upper piece is cut off, and the lower is never 0 or below: an infinite value stays one
+            const uint32_t top = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+            p[u][nt][i] = transpose8x8(top);
+            rest[u][nt][i] = transpose8x8(pack_bf16(fmaxf(a - bf16_lo(top), 0x1p-126f), fmaxf(b - bf16_hi(top), 0x1p-126f)));
+          }
+        }
       }
     }
     fresh = false;
@@ -364,7 +376,10 @@ struct AttnWarp {
             const uint32_t a0 = __byte_perm(x[0][t], x[1][t], 0x5410), a1 = __byte_perm(x[0][t], x[1][t], 0x7632);
             const uint32_t a2 = __byte_perm(x[2][t], x[3][t], 0x5410), a3 = __byte_perm(x[2][t], x[3][t], 0x7632);
             #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[nt][k * (C::VEL / 2) + t], a0, a1, a2, a3, p[u][nt][0], p[u][nt][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<false>(o[nt][k * (C::VEL / 2) + t], a0, a1, a2, a3, p[u][nt][0], p[u][nt][1]);
+              mma16816<false>(o[nt][k * (C::VEL / 2) + t], a0, a1, a2, a3, rest[u][nt][0], rest[u][nt][1]);
+            }
           } else {
             uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
             widen4<T>(__byte_perm(x[0][t], x[1][t], 0x5140), a0, a1);
