@@ -5,6 +5,7 @@ against logits produced token by token with `model.step` from an empty cache, pl
 hand-off; prints error statistics and exits non-zero if `allclose(atol 1e-3, rtol 3e-2)` fails.
 Mode `bench`: prefill a prompt through the chunked scan, decode N tokens with cached conv/SSM states,
 report decode tokens/s and p50 per-token latency (device-timed).  Works with TP > 1 under torchrun.
+Both modes take the hybrid presets too, whose attention layers decode over a paged key-value cache.
 """
 from __future__ import annotations
 

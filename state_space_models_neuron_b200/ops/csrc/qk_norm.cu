@@ -4,6 +4,10 @@
 //   backward: g = dy turned by -a,  h = g w,  dx = r h - x r^3 mean(h x),  dw = sum over rows of g x r
 // r is computed again in the backward pass: x is read there anyway.
 // Sums and the rotation are fp32; each result is rounded once.
+// Bound by memory: 4 bytes per value forward, 6 backward, where the rows are many (us, 32 + 8 heads of 128 channels, forward and backward:
+// 4 x 8192 tokens 108 and 183, floors 103 and 154; 2 x 4096 34 and 50, floors 26 and 38), by latency below (1 x 257 tokens 8.5 both).
+// What it took: rows on their way in shared memory instead of registers (rows of both tensors in registers, two blocks per SM:
+// backward 2 x 4096 69 us), arithmetic in pairs, a token's cosines and sines in registers for all its heads.
 #include "head_norm.cuh"
 
 namespace ssm {

@@ -1466,6 +1466,7 @@ class _QKNormRotary(torch.autograd.Function):
                                                 _at(positions), status_tensor(dev).data_ptr(), part.data_ptr(), _at(targets[0]),
                                                 _at(targets[1]), *ctx.strides, *gs, *hs, *ctx.call, _is32(targets[0]), _is32(targets[1]),
                                                 *adds, ctx.eps), _st())
+        _launches[0] += targets[0] is not None or targets[1] is not None
         if second is not None:
             second.add_(targets[1])
         return dq, dk, *grads, None, None, None, None
