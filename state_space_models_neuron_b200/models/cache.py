@@ -103,6 +103,11 @@ class Mamba2HybridCache(Mamba2Cache):
         if self.seqlen_offset + tokens > self.max_length:
             raise ValueError(f"the cache has room for {self.max_length} tokens, holds {self.seqlen_offset} and was given {tokens} more")
 
+    def begin(self, tokens: int) -> None:
+        """Counts a prompt's tokens in an empty cache (whatever a prompt that failed has left)."""
+        self.require_room(tokens)
+        self.lengths.fill_(tokens)
+
     def take(self, tokens: int) -> None:
         """Counts new tokens of every sequence; the attention layers put them behind the others."""
         self.require_room(tokens)

@@ -86,9 +86,9 @@ class Mamba2HybridModel(Mamba2HybridPreTrainedModel):
     def set_input_embeddings(self, new_embeddings):
         self.embeddings = new_embeddings
 
-    def forward(self, input_ids=None, inputs_embeds=None, cache_params: Optional[Mamba2HybridCache] = None,
-                use_cache: Optional[bool] = None, output_hidden_states: Optional[bool] = None,
-                return_dict: Optional[bool] = None, **kwargs):
+    def forward(self, input_ids=None, inputs_embeds=None, output_hidden_states: Optional[bool] = None,
+                return_dict: Optional[bool] = None, cache_params: Optional[Mamba2HybridCache] = None,
+                use_cache: Optional[bool] = None, **kwargs):
         if (input_ids is None) == (inputs_embeds is None):
             raise ValueError("pass exactly one of input_ids and inputs_embeds")
         sp = self.sequence_parallel_enabled
@@ -106,7 +106,7 @@ class Mamba2HybridModel(Mamba2HybridPreTrainedModel):
                     raise ValueError("a prompt fills an empty cache; further tokens go through step(), one at a time")
                 with torch.no_grad():
                     return Mamba2Output(last_hidden_state=self._step(hidden, cache_params), cache_params=cache_params)
-            cache_params.take(tokens)
+            cache_params.begin(tokens)
         all_hidden = () if output_hidden_states else None
         residual = None
         for block in self.layers:

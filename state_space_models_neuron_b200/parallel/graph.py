@@ -175,7 +175,7 @@ class GraphedDecodeStep:
     """One autoregressive decode step (all layers, LM head, greedy argmax) captured as a CUDA graph.
 
     The caches (conv and SSM states; pages and lengths of a hybrid model) are updated in place by the kernels, so replaying the
-    graph advances them; the token buffer is static.  Warm-up and capture run on a copy of the cache contents which is restored afterwards, so
+    graph advances them; the token buffer is static.  Warm-up and capture run on the cache, whose contents are restored afterwards, so
     constructing the object does not disturb the decoding state."""
 
     def __init__(self, model, cache, batch_size: int, warmup: int = 2):

@@ -83,6 +83,11 @@ def test_use_cache_in_the_forward_pass_and_generate():
     assert out.cache_params.max_length == 8192 and (out.logits - full[:, :128]).abs().max() < 1e-4
     out = model(input_ids=ids[:, 128:129], use_cache=True, cache_params=out.cache_params)
     assert (out.logits[:, 0] - full[:, 128]).abs().max() < 1e-4
+    again = model.new_cache(2, 256)
+    with pytest.raises(ValueError, match="multiple of"):
+        model.prefill(ids[:, :100], again)                         # leaves an empty cache behind
+    assert (model.prefill(ids[:, :128], again)[0][:, 0] - full[:, 127]).abs().max() < 1e-4 and again.lengths.tolist() == [128, 128]
+    assert (model.step(ids[:, 128:129], again)[:, 0] - full[:, 128]).abs().max() < 1e-4
     with pytest.raises(ValueError, match="empty cache"):
         model(input_ids=ids[:, :128], use_cache=True, cache_params=out.cache_params)
     new = model.generate(ids[:, :130], max_new_tokens=6, do_sample=False)
