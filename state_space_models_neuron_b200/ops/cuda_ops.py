@@ -15,7 +15,7 @@ import torch
 from torch.autograd import forward_ad as _forward_ad
 
 from . import native
-from .kv_pages import HEAD_DIMS
+from .paged import HEAD_DIMS
 
 _c = ctypes
 _status = {}

@@ -13,7 +13,7 @@ import torch
 import torch.nn.functional as F
 
 from . import oracle
-from .kv_pages import KVPages, check_heads, check_norm_weight, check_pages, kv_pages  # noqa: F401
+from .paged import KVPages, check_heads, check_norm_weight, check_pages, kv_pages  # noqa: F401
 
 
 # Measurement switch used only by `baseline/nccl_cublas.py`: run the PyTorch/cuBLAS restatement on GPU tensors.

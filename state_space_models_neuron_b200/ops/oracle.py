@@ -19,7 +19,7 @@ from typing import Optional, Tuple
 import torch
 import torch.nn.functional as F
 
-from .kv_pages import QUANT_MAX, QUANT_TINY
+from .paged import QUANT_MAX, QUANT_TINY
 
 
 def softplus(x: torch.Tensor, threshold: float = 20.0) -> torch.Tensor:
