@@ -893,6 +893,14 @@ static void paged_attn_shape(int* blocks, int* slot, int* step) {
   *slot = PagedAttn<D, T, NT>::SLOT;
   *step = PagedAttn<D, T, NT>::STEP;
 }
+static int sm_count(int dev) {
+  static std::atomic<int> known[64];
+  if (dev < 64 && known[dev].load(std::memory_order_relaxed) > 0) return known[dev].load(std::memory_order_relaxed);
+  int n = 0;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
 // blocks of the launch, and floats of its workspace
 static int paged_attn_plan(int type, int width, int page_size, int B, int Hq, int Hk, int D, int* grid, int* most_blocks, long long* floats) {
   int blocks = 0, slot = 0, step = 1, sms = 0, dev = 0;
@@ -905,7 +913,7 @@ static int paged_attn_plan(int type, int width, int page_size, int B, int Hq, in
     } while (0)
   KV_DISPATCH(SHAPE);
   #undef SHAPE
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return (int)cudaGetLastError();
+  if (cudaGetDevice(&dev) != cudaSuccess || (sms = sm_count(dev)) < 1) return (int)cudaGetLastError();
   const int group = two ? 16 : 8;
   // no more blocks than there can be shares
   const long long items = (long long)B * Hk * ((ratio + group - 1) / group), most = items * (((long long)width * page_size + step - 1) / step);

@@ -1380,6 +1380,11 @@ def _aligned(t: Optional[torch.Tensor]):
     return t, at
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """Uninitialised and contiguous (half of the time of `torch.empty` with a shape)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _at(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -1423,8 +1428,7 @@ class _QKNormRotary(torch.autograd.Function):
         (B, L, Hq, D), Hk, dev = q.shape, k.shape[2], q.device
         (q2, q_at, qs), (k2, k_at, ks) = _head_view(q), _head_view(k)
         (w1, qw_at), (w2, kw_at) = _aligned(qw), _aligned(kw)
-        qo = torch.empty((B, L, Hq, D), dtype=torch.bfloat16, device=dev)
-        ko = torch.empty((B, L, Hk, D), dtype=torch.bfloat16, device=dev)
+        qo, ko = _like(q), _like(k)
         rotary, rows = (0, 0) if cos is None else (2 * cos.shape[1], cos.shape[0])
         # of the call: what the backward pass packs again
         ctx.call = (_is32(qw), _is32(kw), int(positions is not None and positions.dtype is torch.int64), B, L, Hq, Hk, D, rotary, rows)
@@ -1442,15 +1446,14 @@ class _QKNormRotary(torch.autograd.Function):
         _, _, _, B, L, Hq, Hk, D, _, _ = ctx.call
         dev, need = q.device, ctx.needs_input_grad
         (g, g_at, gs), (h, h_at, hs) = _head_view(dqo), _head_view(dko)
-        dq = torch.empty((B, L, Hq, D), dtype=torch.bfloat16, device=dev)
-        dk = torch.empty((B, L, Hk, D), dtype=torch.bfloat16, device=dev)
+        dq, dk = _like(q), _like(k)
         grads, targets, adds, second = [None, None], [None, None], [0, 0], None
         for i, w in enumerate((qw, kw)):
             if not need[2 + i]:
                 continue
             mg = getattr(w, "main_grad", None) if w.is_leaf else None
             if mg is None or mg.dtype is not torch.float32 or not (B and L):
-                grads[i] = targets[i] = torch.empty((D,), dtype=w.dtype, device=dev)
+                grads[i] = targets[i] = torch.empty_like(w)
                 continue
             if mg is targets[0]:               # one weight of both: the kernel adds to it once
                 second, targets[i] = mg, torch.empty_like(mg)
@@ -1460,7 +1463,7 @@ class _QKNormRotary(torch.autograd.Function):
             w.grad_stale = False
         if not (B and L):
             return dq, dk, *[None if t is None else t.zero_() for t in grads], None, None, None, None
-        part = torch.empty((_norm_grad_blocks(B * L, Hq, Hk, D) * D,), dtype=torch.float32, device=dev)
+        part = torch.empty(_norm_grad_blocks(B * L, Hq, Hk, D) * D, dtype=torch.float32, device=dev)
         (w1, qw_at), (w2, kw_at) = _aligned(qw), _aligned(kw)
         _run("ssm_qk_norm_bwd", _NORM_CALL.pack(_at(q), _at(k), g_at, h_at, dq.data_ptr(), dk.data_ptr(), qw_at, kw_at, _at(cos), _at(sin),
                                                 _at(positions), status_tensor(dev).data_ptr(), part.data_ptr(), _at(targets[0]),
@@ -1517,7 +1520,7 @@ def kv_cache_write(k, v, pages, block_table, lengths, counts, q, q_weight, k_wei
     if q is not None:
         Hq = q.shape[2]
         q, q_at, qs = _head_view(q)
-        out = torch.empty((B, L, Hq, D), dtype=torch.bfloat16, device=dev)
+        out = _like(q)
         out_at = out.data_ptr()
     (w1, qw_at), (w2, kw_at), (c1, cos_at), (c2, sin_at) = _aligned(q_weight), _aligned(k_weight), _aligned(cos), _aligned(sin)
     if B and L:
@@ -1543,8 +1546,8 @@ def _kv_cache_read(first, pages, block_table, lengths, max_length, dtype):
     held, sizes = _page_args(pages)
     if B > 65535:
         raise ValueError(f"the kernel reads at most 65535 sequences at once, got {B}")
-    k = torch.empty((B, max_length, Hk, D), dtype=dtype, device=dev)
-    v = torch.empty((B, max_length, Hk, D), dtype=dtype, device=dev)
+    k = torch.empty(B, max_length, Hk, D, dtype=dtype, device=dev)
+    v = _like(k)
     if B and max_length:
         _run("ssm_kv_read", _KV_READ_CALL.pack(*held, block_table.data_ptr(), lengths.data_ptr(), k.data_ptr(), v.data_ptr(),
                                                status_tensor(dev).data_ptr(), *sizes, block_table.shape[1], int(dtype is torch.float32),
@@ -1574,10 +1577,10 @@ def paged_attention(q, pages, block_table, lengths, scale):
     if n * Hk * page >= 2 ** 31:
         raise ValueError("the attention kernel reads pools of less than 2^31 rows (pages x key heads x page size)")
     q, q_at, (qb, _, qh) = _head_view(q)
-    out = torch.empty((B, 1, Hq, D), dtype=torch.bfloat16, device=dev)
+    out = _like(q)
     if B and n and width:
         floats = _paged_workspace(index, sizes[0], width, page, B, Hq, Hk, D)
-        ws = torch.empty((floats,), dtype=torch.float32, device=dev)
+        ws = torch.empty(floats, dtype=torch.float32, device=dev)
         _run("ssm_paged_attn", _PAGED_ATTN_CALL.pack(q_at, out.data_ptr(), *held, block_table.data_ptr(), lengths.data_ptr(),
                                                      ws.data_ptr(), status_tensor(dev).data_ptr(), qb, qh, floats, *sizes, width, B, Hq,
                                                      Hk, D, D ** -0.5 if scale is None else scale), _st())
