@@ -229,7 +229,8 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const uint8_t* __re
   }
 }
 
-// Heads that a warp takes one after the other: 8, or fewer where that would leave less than three blocks per SM.
+// Heads that a warp takes one after the other: 8, or fewer where that would leave less than three blocks per SM (128 tokens written and read
+// 6.2 us, with eight heads 9.0; 8 x 1000 written with eight, four, two heads 32.6, 31.7, 40.1).
 static long long write_warps(long long tokens, int Hq, int Hk, int each, int D) {
   return (tokens * (D / 16) + 31) / 32 * ((Hq + each - 1) / each + 2 * ((Hk + each - 1) / each));
 }

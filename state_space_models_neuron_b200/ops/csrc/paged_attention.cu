@@ -28,9 +28,10 @@ namespace ssm {
 
 constexpr int PA_WARPS = 4, PA_BOX = 16, PA_COUNTERS = 2048;     // PA_BOX: tokens of a box
 // Steps of a block (few items) and of a warp that make a share.  Blocks: four steps per warp (two: 200 tokens 8.3 us instead of 7.0, a join that saves
-// nothing; eight: 2048 tokens 12.5 instead of 10.2).
+// nothing; eight: 2048 tokens 12.5 instead of 10.2).  Warps: four (one / four / twelve, us: 100 of 50 tokens bf16 12.1 / 8.4 / 17.3, 300 of 1 11.2 / 12.9 /
+// 29.6, 40 of 300 int8 13.5 / 18.0 / 33.6).
 constexpr int PA_BLOCK_SHARE = 4 * PA_WARPS, PA_WARP_SHARE = 4;
-constexpr int FEW_ITEMS = 8, LONG_ITEM = 48;   // blocks per item and steps of an item, see the kernel
+constexpr int FEW_ITEMS = 2, LONG_ITEM = 48;   // blocks per item and steps of an item, see the kernel
 // A running maximum moves when scores pass it by 2^8: bf16 and fp16 hold larger shares as well.
 constexpr float PA_GROWTH = 8.f, PA_SHARE = 256.f;
 
@@ -547,7 +548,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
   // Where this worker's share begins.  The steps of all sequences and heads stand in a row, each sequence's heads one behind the other;
   // sequences in the order lane, lane + 32, ... of the lanes that look at them (every warp finds the same).
   // Workers cut the row at equal distances, wherever that is.  Only where there are few items is every item cut by itself, so that no worker
-  // has parts of two, at the price of up to one shorter share per item.
+  // has parts of two, at the price of up to one shorter share per item (itself / row, us, bf16: 64 items of 2048 tokens 15.4 / 16.9, of 8192 47.6 /
+  // 51.5, 50 of up to 4000 e4m3 14.5 / 22.8; 144 of 8192 96.9 / 95.8, of up to 8192 58 / 62).
   // Workers are blocks, whose warps take every fourth step and meet at the end of a piece, or, where items are short, warps, which never
   // wait for each other (256 of 200 tokens, bf16 and e4m3, us: blocks 52.5 and 51.7, warps 44.6 and 33.8).  Blocks read longer stretches of
   // memory at a time (64 x 8192 bf16 319, warps 328; 64 x 2048 87 and 91, e4m3 55.0 and 55.5).
@@ -575,8 +577,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
   if (few) {
     // The smallest share of which there are at most most_blocks; the last guess always fits.  Counted in shares from here on.
     const int rest = workers - filled * items, fits = max(PA_BLOCK_SHARE, ((total + rest - 1) / rest + PA_WARPS - 1) / PA_WARPS * PA_WARPS);
-    for (int guess = 0;; ++guess, share += PA_WARPS) {
-      if (guess == 3 || share > fits) share = fits;
+    for (int guess = 0;; ++guess, share += (share / 8 + PA_WARPS - 1) / PA_WARPS * PA_WARPS) {
+      if (guess == 6 || share > fits) share = fits;
       mine = (first_steps + share - 1) / share * items;
       for (int b = lane + 32; b < a.B; b += 32) mine += (steps_of(b) + share - 1) / share * items;
       total = __reduce_add_sync(0xffffffffu, mine);
@@ -884,7 +886,8 @@ static int paged_attn_launch(const AttnArgs& a, int grid, cudaStream_t st) {
   return launch_dependent(paged_attn_kernel<D, T, NT>, dim3(grid), dim3(PA_WARPS * 32), C::SMEM, st, a, map[0], map[1]);
 }
 
-// Two column tiles for more than 8 query heads per key head; 256 channels leave registers for one.
+// Two column tiles for more than 8 query heads per key head, which would else be read twice (32 x 8192 tokens, 16 heads on one, two tiles / one,
+// us: bf16 32 / 48, int8 25.7 / 33); 256 channels leave registers for one.
 static bool two_tiles(int ratio, int D) { return ratio > 8 && D <= 128; }
 
 template <int D, int T, int NT>

@@ -282,7 +282,8 @@ static int norm_args(NormArgs* a, const NormCall& c, bool grads) {
   return 0;
 }
 
-// Heads that a warp takes one after the other: 8, or fewer where that would leave less than three blocks per SM.
+// Heads that a warp takes one after the other: 8, or fewer where that would leave less than three blocks per SM (257 tokens with gradients
+// 8.4 us, with eight heads 18; 2 x 4096 forward with eight, four, two heads 33.6, 33.2, 38.9).
 static long long norm_turns(long long tokens, int heads, int each, int D) { return (tokens * (D / 16) + 31) / 32 * ((heads + each - 1) / each); }
 static int heads_each(long long tokens, int Hq, int Hk, int D) {
   for (int each = EACH; each > 1; each /= 2)
