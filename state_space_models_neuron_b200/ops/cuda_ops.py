@@ -1483,7 +1483,8 @@ def _norm_grad_blocks(*sizes) -> int:
 
 @_on_device
 def qk_norm_rotary(q, k, q_weight, k_weight, eps, cos, sin, positions):
-    _require_bf16(q, k)
+    if q.dtype is not torch.bfloat16 or k.dtype is not torch.bfloat16:
+        _require_bf16(q, k)
     _require_norm_weight(q_weight)
     _require_norm_weight(k_weight)
     _require_device(q.get_device(), k, q_weight, k_weight, cos, sin, positions)
@@ -1507,12 +1508,16 @@ def _page_args(pages):
 
 @_on_device
 def kv_cache_write(k, v, pages, block_table, lengths, counts, q, q_weight, k_weight, eps, cos, sin):
-    _require_bf16(k, v, q)
+    if k.dtype is not torch.bfloat16 or (q is not None and q.dtype is not torch.bfloat16):      # v has the type of k
+        _require_bf16(k, v, q)
     _require_norm_weight(q_weight)
     _require_norm_weight(k_weight)
     _require_device(k.get_device(), v, pages.k, q, q_weight, k_weight, cos, sin)
     (B, L, Hk, D), dev = k.shape, k.device
-    rotary, rows = (0, 0) if cos is None else (2 * cos.shape[1], cos.shape[0])
+    rotary, rows = 0, 0
+    if cos is not None:
+        rows, rotary = cos.shape
+        rotary *= 2
     _require_head_dim(D, rotary)
     held, sizes = _page_args(pages)
     (k, k_at, ks), (v, v_at, vs) = _head_view(k), _head_view(v)
@@ -1556,33 +1561,35 @@ def _kv_cache_read(first, pages, block_table, lengths, max_length, dtype):
 
 
 @functools.lru_cache(maxsize=1024)
-def _paged_workspace(device: int, *sizes) -> int:
-    """Floats of the attention's workspace for (type, width, page, B, Hq, Hkv, D) on the current device."""
+def _paged_workspace(device: int, *sizes):
+    """Floats of the attention's workspace for (type, width, page, B, Hq, Hkv, D) on the current device, and a template of that
+    size without memory of its own (`_like` of it takes the host less than `torch.empty`)."""
     fn = _lib().ssm_paged_attn_workspace
     fn.restype = _c.c_longlong
     n = int(fn(*sizes))
     if n < 0:
         raise RuntimeError(f"ssm_paged_attn_workspace failed with code {n}")
-    return n
+    return n, status_tensor(torch.device("cuda", device)).view(torch.float32).expand(n)
 
 
 @_on_device
 def paged_attention(q, pages, block_table, lengths, scale):
-    _require_bf16(q)
-    index, dev, first = q.get_device(), q.device, pages.k
-    _require_device(index, first)
+    index, first = q.get_device(), pages.k
     (B, _, Hq, D), (n, Hk, page, _), width = q.shape, first.shape, block_table.shape[1]
-    _require_head_dim(D, 0)
+    if q.dtype is not torch.bfloat16 or first.get_device() != index or D not in HEAD_DIMS:
+        _require_bf16(q)
+        _require_device(index, first)
+        _require_head_dim(D, 0)
     held, sizes = _page_args(pages)
     if n * Hk * page >= 2 ** 31:
         raise ValueError("the attention kernel reads pools of less than 2^31 rows (pages x key heads x page size)")
     q, q_at, (qb, _, qh) = _head_view(q)
     out = _like(q)
     if B and n and width:
-        floats = _paged_workspace(index, sizes[0], width, page, B, Hq, Hk, D)
-        ws = torch.empty(floats, dtype=torch.float32, device=dev)
+        floats, template = _paged_workspace(index, sizes[0], width, page, B, Hq, Hk, D)
+        ws = _like(template)
         _run("ssm_paged_attn", _PAGED_ATTN_CALL.pack(q_at, out.data_ptr(), *held, block_table.data_ptr(), lengths.data_ptr(),
-                                                     ws.data_ptr(), status_tensor(dev).data_ptr(), qb, qh, floats, *sizes, width, B, Hq,
+                                                     ws.data_ptr(), status_tensor(q.device).data_ptr(), qb, qh, floats, *sizes, width, B, Hq,
                                                      Hk, D, D ** -0.5 if scale is None else scale), _st())
         return out
     return out.zero_()

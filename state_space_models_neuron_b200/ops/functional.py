@@ -233,11 +233,12 @@ def kv_cache_write(k, v, pages: KVPages, block_table, lengths, counts=None, q=No
     A position without a page or outside the tables raises on the CPU; on the GPU such a token is skipped in the same way
     and leaves status 3 (`check_status`).  No gradients."""
     check_heads(q, k, cos, sin, None, False)
-    check_pages(pages, block_table, lengths, k.shape[0], counts)
-    if v.shape != k.shape or v.dtype != k.dtype or pages.k.shape[1] != k.shape[2] or pages.k.shape[3] != k.shape[3]:
-        raise ValueError(f"keys {tuple(k.shape)}, values {tuple(v.shape)} and pages {tuple(pages.k.shape)} do not fit together")
-    check_norm_weight("q_weight", q_weight, k.shape[3])
-    check_norm_weight("k_weight", k_weight, k.shape[3])
+    shape, held = k.shape, pages[0].shape
+    check_pages(pages, block_table, lengths, shape[0], counts)
+    if v.shape != shape or v.dtype is not k.dtype or held[1] != shape[2] or held[3] != shape[3]:
+        raise ValueError(f"keys {tuple(shape)}, values {tuple(v.shape)} and pages {tuple(held)} do not fit together")
+    check_norm_weight("q_weight", q_weight, shape[3])
+    check_norm_weight("k_weight", k_weight, shape[3])
     if _native(k):
         return _cuda().kv_cache_write(k, v, pages, block_table, lengths, counts, q, q_weight, k_weight, eps, cos, sin)
     with torch.no_grad():
@@ -263,10 +264,11 @@ def paged_attention(q, pages: KVPages, block_table, lengths, scale: Optional[flo
     included (`kv_cache_write` comes first); a sequence without tokens gets zeros.  What lies behind a length is never used.
     A position without a page raises on the CPU; on the GPU it is left out and leaves status 3 (`check_status`).
     No gradients."""
-    if q.dim() != 4 or q.shape[1] != 1 or q.shape[3] != pages.k.shape[3] or q.shape[2] % pages.k.shape[1]:
-        raise ValueError(f"queries are [batch, 1, heads, head_dim], heads a multiple of the pages' key heads; got {tuple(q.shape)} "
-                         f"for pages {tuple(pages.k.shape)}")
-    check_pages(pages, block_table, lengths, q.shape[0])
+    shape, held = q.shape, pages[0].shape
+    if len(shape) != 4 or len(held) != 4 or shape[1] != 1 or shape[3] != held[3] or held[1] < 1 or shape[2] < 1 or shape[2] % held[1]:
+        raise ValueError(f"queries are [batch, 1, heads, head_dim], heads a multiple of the pages' key heads; got {tuple(shape)} "
+                         f"for pages {tuple(held)}")
+    check_pages(pages, block_table, lengths, shape[0])
     if _native(q):
         return _cuda().paged_attention(q, pages, block_table, lengths, scale)
     with torch.no_grad():

@@ -75,10 +75,10 @@ def check_pages(pages, block_table, lengths, batch: int, counts=None) -> None:
 
 def check_heads(q, k, cos, sin, positions, from_zero: bool) -> None:
     """Shapes of queries and keys (q may be None) and of the rotation's tables; from_zero: without positions, token l has row l."""
-    shape = k.shape
-    if len(shape) != 4 or (q is not None and (q.dim() != 4 or q.shape[:2] != shape[:2] or q.shape[3] != shape[3])):
+    shape, like = k.shape, k.shape if q is None else q.shape
+    if len(shape) != 4 or len(like) != 4 or like[0] != shape[0] or like[1] != shape[1] or like[3] != shape[3]:
         raise ValueError("queries and keys are [batch, tokens, heads, head_dim] with the same batch, tokens and head_dim")
-    if shape[2] < 1 or (q is not None and q.shape[2] < 1):
+    if shape[2] < 1 or like[2] < 1:
         raise ValueError("queries and keys have at least one head")
     if cos is None and sin is None:
         if positions is not None:
@@ -86,13 +86,14 @@ def check_heads(q, k, cos, sin, positions, from_zero: bool) -> None:
         return
     if cos is None or sin is None:
         raise ValueError("cos and sin come together")
-    if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.dim() != 2 or cos.shape != sin.shape
-            or not 2 <= cos.shape[1] * 2 <= shape[3]):
+    table = cos.shape
+    if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or len(table) != 2 or sin.shape != table
+            or not 2 <= table[1] * 2 <= shape[3]):
         raise ValueError("cos and sin are fp32 [positions, rotary_dim / 2] with rotary_dim <= head_dim")
     if positions is not None and (positions.dtype not in (torch.int32, torch.int64) or positions.shape != shape[:2]):
         raise ValueError("positions are int32 or int64 [batch, tokens]")
-    if positions is None and from_zero and cos.shape[0] < shape[1]:
-        raise ValueError(f"tables of {cos.shape[0]} positions are too short for {shape[1]} tokens")
+    if positions is None and from_zero and table[0] < shape[1]:
+        raise ValueError(f"tables of {table[0]} positions are too short for {shape[1]} tokens")
 
 
 def check_norm_weight(name: str, weight, head_dim: int) -> None:
