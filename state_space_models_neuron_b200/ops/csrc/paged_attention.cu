@@ -549,7 +549,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
   // sequences in the order lane, lane + 32, ... of the lanes that look at them (every warp finds the same).
   // Workers cut the row at equal distances, wherever that is.  Only where there are few items is every item cut by itself, so that no worker
   // has parts of two, at the price of up to one shorter share per item (itself / row, us, bf16: 64 items of 2048 tokens 15.4 / 16.9, of 8192 47.6 /
-  // 51.5, 50 of up to 4000 e4m3 14.5 / 22.8; 144 of 8192 96.9 / 95.8, of up to 8192 58 / 62).
+  // 51.5, 50 of up to 4000 e4m3 14.5 / 22.8; 144 of 8192 96.9 / 95.8, of up to 8192 58 / 62;
+  // 128 of 8192 with 256 channels e4m3 100.8 / 93.2, of up to 8192 56 / 65).
   // Workers are blocks, whose warps take every fourth step and meet at the end of a piece, or, where items are short, warps, which never
   // wait for each other (256 of 200 tokens, bf16 and e4m3, us: blocks 52.5 and 51.7, warps 44.6 and 33.8).  Blocks read longer stretches of
   // memory at a time (64 x 8192 bf16 319, warps 328; 64 x 2048 87 and 91, e4m3 55.0 and 55.5).
