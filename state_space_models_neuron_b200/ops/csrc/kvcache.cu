@@ -1,20 +1,27 @@
 // Paged key-value cache: writing new tokens (keys normed and rotated, 8-bit values quantised in the same pass) and reading sequences
 // back.  8-bit values have one fp32 scale per token and head, s = max |x| / Qmax; stored = round(x / s).
 // Both are bound by memory where tokens are many (16 x 2048 tokens, 32 query and 8 key heads of 128 channels, int8: written, with
-// norm and rotation, in 134 us, floor 113; read back in 39, floor 31), by latency for single tokens (write 3.7 us, read 2.6).
+// norm and rotation, in 142 us, floor 113 (135 with the product x (Qmax / max) in place of the quotient x / s: other bytes at ties); read back in
+// 39, floor 31), by latency for single tokens (write 3.7 us, read 2.6).
 #include "head_norm.cuh"
 #include "kv_pages.cuh"
 
 namespace ssm {
 
-// 16 values times inv, rounded to nearest even, as 16 bytes
-__device__ __forceinline__ void quantise_e4m3(const Pairs& y, uint64_t inv, uint2& lo, uint2& hi) {
+// y / s of pairs rounded to nearest, from r = 1 / s rounded to nearest, by a residual step (Markstein, IBM J. Res. Dev. 34, 1990): so the
+// definition's quotient is what is rounded to 8 bits, and ties (half of a row's maximum) fall where a division lets them fall.
+__device__ __forceinline__ uint64_t quotient(uint64_t y, uint64_t minus_s, uint64_t r) {
+  const uint64_t q = mul2(y, r);
+  return fma2(fma2(q, minus_s, y), r, q);
+}
+// 16 values over s, rounded to nearest even, as 16 bytes
+__device__ __forceinline__ void quantise_e4m3(const Pairs& y, uint64_t minus_s, uint64_t r, uint2& lo, uint2& hi) {
   uint32_t v[4];
   #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float a, b, c, d;
-    unpack2(mul2(y[2 * i], inv), a, b);
-    unpack2(mul2(y[2 * i + 1], inv), c, d);
+    unpack2(quotient(y[2 * i], minus_s, r), a, b);
+    unpack2(quotient(y[2 * i + 1], minus_s, r), c, d);
     asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\tmov.b32 %0, {l, h};\n\t}"
         : "=r"(v[i]) : "f"(a), "f"(b), "f"(c), "f"(d));
   }
@@ -22,13 +29,13 @@ __device__ __forceinline__ void quantise_e4m3(const Pairs& y, uint64_t inv, uint
   hi = make_uint2(v[2], v[3]);
 }
 // The sum of a number of at most 127 and 1.5 * 2^23 is rounded to an integer whose low byte is the number's.
-__device__ __forceinline__ void quantise_int8(const Pairs& y, uint64_t inv, uint2& lo, uint2& hi) {
+__device__ __forceinline__ void quantise_int8(const Pairs& y, uint64_t minus_s, uint64_t r, uint2& lo, uint2& hi) {
   uint32_t v[4];
   #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float a, b, c, d;
-    unpack2(fma2(y[2 * i], inv, both(12582912.f)), a, b);
-    unpack2(fma2(y[2 * i + 1], inv, both(12582912.f)), c, d);
+    unpack2(add2(quotient(y[2 * i], minus_s, r), both(12582912.f)), a, b);
+    unpack2(add2(quotient(y[2 * i + 1], minus_s, r), both(12582912.f)), c, d);
     v[i] = __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040), __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
   }
   lo = make_uint2(v[0], v[1]);
@@ -150,14 +157,21 @@ __global__ void __launch_bounds__(KV_THREADS, 3) kv_write_kernel(const WriteArgs
       for (int o = LANES / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
       if (h0 + i >= h1 || page < 0) continue;
       const bool some = __float_as_uint(top) - (27u << 23) < 0x7f800000u - (27u << 23);      // finite and at least 2^-100
-      const uint64_t inv = both(some ? __fdiv_rn(QMAX, top) : 0.f);
+      const float scale = some ? __fdiv_rn(top, QMAX) : top < 1.f ? 0.f : __uint_as_float(0x7fc00000u);
+      float s = some ? scale : 0.f;
+      if (some && top < 0x1p-40f) {            // residuals of small rows would be no normal numbers: the quotients of 2^60 times these rows are the same
+        s *= 0x1p60f;
+        #pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = mul2(y[k], both(0x1p60f));
+      }
+      const uint64_t minus_s = both(-s), r = both(some ? __frcp_rn(s) : 0.f);
       uint2 lo, hi;
-      if (T == KV_E4M3) quantise_e4m3(y, inv, lo, hi); else quantise_int8(y, inv, lo, hi);
+      if (T == KV_E4M3) quantise_e4m3(y, minus_s, r, lo, hi); else quantise_int8(y, minus_s, r, lo, hi);
       uint8_t* o = reinterpret_cast<uint8_t*>(a.pages[which - 1]) + slot * D;
       *reinterpret_cast<uint2*>(o + at.c0) = lo;
       *reinterpret_cast<uint2*>(o + at.c1) = hi;
       // a row with a value that is not finite reads back as NaN whatever is stored
-      if (lane == 0) a.scales[which - 1][slot] = some ? __fdiv_rn(top, QMAX) : top < 1.f ? 0.f : __uint_as_float(0x7fc00000u);
+      if (lane == 0) a.scales[which - 1][slot] = scale;
     }
   }
 }
