@@ -17,8 +17,8 @@
 // warp, takes an equal share of it, however the lengths differ.  An item (a key head of a sequence) that several workers share is joined by
 // the one that finishes last, in the order of the workers: (m, sum, unnormalised o) of each from the caller's workspace.
 //
-// 8-bit values are multiplied in fp16, which holds them exactly: queries by a power of two per head that brings their largest
-// magnitude to [1, 2) (what is below 2^-24 of it is lost), probabilities with the scale of their value, as shares of a running
+// 8-bit values are multiplied in fp16, which holds them exactly: queries times a power of two per head that brings their largest
+// magnitude to [2^14, 2^15) (those down to 2^-32 of it stay exact, further ones are off by 2^-39 of it at most), probabilities with the scale of their value, as shares of a running
 // maximum of their own (M below: scales of tokens may be any numbers).  They are bound by their instructions where that
 // maximum, the scales and the conversions are for few bytes: 64 x 8192 tokens e4m3 175 us, int8 180 (floor 169), of 64 channels 58 (44).
 #include "kv_pages.cuh"
@@ -155,15 +155,18 @@ struct AttnWarp {
         }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // exponent of the head's largest magnitude; where it is not finite the values stay what they are
-        int e = (int)(top >> 7);
-        e = top == 0 || e == 255 ? 127 : min(e, 253);
-        const float down = __uint_as_float((uint32_t)(254 - e) << 23);                        // 2^(127 - e)
+        // exponent of the head's largest magnitude (not below 20, so that both factors are normal numbers); where it is not finite any will do
+        const int e = max((int)(top >> 7), 20);
+        const float f = __uint_as_float((uint32_t)(268 - e) << 23);                             // 2^(141 - e)
         #pragma unroll
-        for (int k = 0; k < D / 8; ++k) qf[nt][k] = pack_f16(bf16_lo(qf[nt][k]) * down, bf16_hi(qf[nt][k]) * down);
+        for (int k = 0; k < D / 8; ++k) {
+          float lo, hi;
+          unpack2(mul2(bf16x2_pair(qf[nt][k]), pack2(f, f)), lo, hi);
+          qf[nt][k] = pack_f16(lo, hi);
+        }
         // the columns of this lane's sums are heads 2c, 2c + 1, whose exponents lanes 8c and 8c + 4 know
         #pragma unroll
-        for (int j = 0; j < 2; ++j) qs[nt][j] = a.scale * __uint_as_float((uint32_t)max(1, __shfl_sync(0xffffffffu, e, c * 8 + j * 4)) << 23);
+        for (int j = 0; j < 2; ++j) qs[nt][j] = a.scale * __uint_as_float((uint32_t)(__shfl_sync(0xffffffffu, e, c * 8 + j * 4) - 14) << 23);
       }
     }
   }

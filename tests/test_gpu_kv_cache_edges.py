@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from state_space_models_neuron_b200 import ops
-from tests.test_gpu_kv_cache import TYPES, ints, make_pool
+from tests.test_gpu_kv_cache import TYPES, check_attention, draw, filled, ints, make_pool
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +41,28 @@ def test_stored_bytes_are_those_of_the_definition(dtype, D):
         made[device] = pages
     for a, b in zip(made["cuda"], made["cpu"]):
         assert same_bits(a, b)
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+@pytest.mark.parametrize("Hq", [8, 32])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("far", [10, 20, 28])
+def test_queries_beside_much_larger_ones(dtype, Hq, D, far):
+    """one channel of a query is 2^far larger than the others, and its keys are zero: the others decide alone"""
+    lengths = (100, 333)
+    pages, table = filled(2, lengths, 2, D, 16, TYPES[dtype], far)
+    pages.k.view(torch.uint8)[..., D // 3] = 0
+    q = draw((2, 1, Hq, D), D, 1.5)
+    q[..., D // 3] = 1.25 * 2 ** far
+    check_attention(q, pages, table, lengths, ops.paged_attention(q, pages, table, ints(*lengths)))
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+@pytest.mark.parametrize("power", [-126, -100, 100, 110])
+def test_queries_of_every_size(dtype, power):
+    """queries of 2^power beside keys of about 2^-power, bf16's smallest numbers (2^-126 and below it) included"""
+    lengths = (100, 333)
+    pages, table = filled(2, lengths, 2, 128, 16, TYPES[dtype], 3)
+    pages.k_scale.copy_((pages.k_scale.double() * 2.0 ** -power).float())
+    q = (draw((2, 1, 16, 128), 4).double() * 2.0 ** power).bfloat16()
+    check_attention(q, pages, table, lengths, ops.paged_attention(q, pages, table, ints(*lengths)))
