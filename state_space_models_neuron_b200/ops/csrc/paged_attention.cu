@@ -18,7 +18,7 @@
 // the one that finishes last, in the order of the workers: (m, sum, unnormalised o) of each from the caller's workspace.
 //
 // 8-bit values are multiplied in fp16, which holds them exactly: queries times a power of two per head that brings their largest
-// magnitude to [2^14, 2^15) (those down to 2^-32 of it stay exact, further ones are off by 2^-39 of it at most), probabilities with the scale of their value, as shares of a running
+// magnitude to [2^14, 2^15) (those down to 2^-31 of it stay exact, further ones are off by 2^-39 of it at most), probabilities with the scale of their value, as shares of a running
 // maximum of their own (M below: scales of tokens may be any numbers).  They are bound by their instructions where that
 // maximum, the scales and the conversions are for few bytes: 64 x 8192 tokens e4m3 175 us, int8 180 (floor 169), of 64 channels 58 (44).
 #include "kv_pages.cuh"
@@ -33,7 +33,9 @@ constexpr int PA_WARPS = 4, PA_BOX = 16, PA_COUNTERS = 2048;     // PA_BOX: toke
 constexpr int PA_BLOCK_SHARE = 4 * PA_WARPS, PA_WARP_SHARE = 4;
 constexpr int FEW_ITEMS = 2, LONG_ITEM = 48;   // blocks per item and steps of an item, see the kernel
 // A running maximum moves when scores pass it by 2^8: bf16 and fp16 hold larger shares as well.
-constexpr float PA_GROWTH = 8.f, PA_SHARE = 256.f;
+// fp16 shares are at most 2^7 where M is chosen and may grow to 2^15.
+constexpr float PA_GROWTH = 8.f, PA_SHARE = 32768.f;
+constexpr int PA_SHARE_BITS = 7;
 
 struct AttnArgs {
   const __nv_bfloat16* q; __nv_bfloat16* out;
@@ -95,8 +97,10 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 }
 // 2^(m - to), 0 for a part without tokens
 __device__ __forceinline__ float part_factor(float m, float to) { return m == -INFINITY ? 0.f : exp2f(m - to); }
-// what an unnormalised result is multiplied with; 0 where there are no tokens
-__device__ __forceinline__ float out_factor(float m, float M, float sum) { return sum == 0.f ? 0.f : exp2f(M - m) / sum; }
+// What an unnormalised result is multiplied with, one after the other (8-bit values: the product alone may be below fp32's normal numbers);
+// 0 where there are no tokens.
+__device__ __forceinline__ float out_share(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
+__device__ __forceinline__ float out_size(float m, float M) { return m == -INFINITY ? 0.f : exp2f(M - m); }
 
 // tokens of sequence b: not below 0, not beyond its pages
 __device__ __forceinline__ int tokens_of(const AttnArgs& a, int b) {
@@ -285,7 +289,11 @@ struct AttnWarp {
       }
     }
     // 16-bit probabilities beside bf16 values come in two pieces, which have 16 bits of mantissa between them: their rounding to one would
-    // add as much to the error as that of the result does (2.3e-3 instead of 1.7e-3), and the products have time (1 %).  fp16 has 11 bits.
+    // add as much to the error as that of the result does (2.3e-3 instead of 1.7e-3), and the products have time (1 %).  Beside 8-bit values
+    // they are one fp16 number, 11 bits: of values that were rounded to 4 or 7 bits, that adds 1 % to the result's own rounding (1.632e-3, in two
+    // pieces 1.621e-3), and a second piece would cost 3 to 11 % (us, one / two: 64 x 8192 e4m3 175.5 / 184.7, 32 x 8192 int8 with 16 heads
+    // on one 26.0 / 28.5, 256 channels e4m3 101 / 111).  Shares of which the largest is at least 2^6 leave fp16 its whole range: what is below 2^-20 of
+    // the largest loses bits, what is below 2^-31 vanishes.
     uint32_t p[SUB][NT][2], rest[SUB][NT][2];
     most = 0.f;
     #pragma unroll
@@ -309,11 +317,11 @@ struct AttnWarp {
         for (int nt = 0; nt < NT; ++nt) {
           #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float x = -120.f;                   // above the logarithms of all shares: 2^e > scale
+            float x = -120.f;                   // M: 2^-7 of a number above all of p times scale (2^e > scale)
             #pragma unroll
             for (int u = 0; u < SUB; ++u) {
               #pragma unroll
-              for (int i = 0; i < 2; ++i) x = fmaxf(x, log2f(s[u][nt][2 * i + j]) + (float)(int)((__float_as_uint(vs[u][i]) >> 23) & 255) - 126.f);
+              for (int i = 0; i < 2; ++i) x = fmaxf(x, log2f(s[u][nt][2 * i + j]) + (float)(int)((__float_as_uint(vs[u][i]) >> 23) & 255) - (126.f + PA_SHARE_BITS));
             }
             x = column_max(x) + m[nt][j];
             if (!fresh) {
@@ -422,14 +430,14 @@ struct AttnWarp {
       for (int j = 0; j < 2; ++j) {
         const int head = nt * 8 + 2 * c + j;
         if (head >= real) continue;
-        const float f = out_factor(m[nt][j], F16 ? M[nt][j] : m[nt][j], l[nt][j]);
+        const float f = out_share(l[nt][j]), size = F16 ? out_size(m[nt][j], M[nt][j]) : 1.f;
         #pragma unroll
         for (int k = 0; k < C::TILES; ++k) {
           uint32_t w[C::VEL / 2];
           #pragma unroll
           for (int e = 0; e < C::VEL / 2; ++e) {
             const int t = k * (C::VEL / 2) + e;
-            w[e] = pack_bf16(o[nt][t][j] * f, o[nt][t][j + 2] * f);
+            w[e] = F16 ? pack_bf16(o[nt][t][j] * f * size, o[nt][t][j + 2] * f * size) : pack_bf16(o[nt][t][j] * f, o[nt][t][j + 2] * f);
           }
           uint4* at = reinterpret_cast<uint4*>(out + head * D + (k * 8 + sigma<C::TILE>(g)) * C::VEL);
           #pragma unroll
@@ -744,7 +752,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
     // threads take a channel of four heads at a time, always the same heads
     const int fours = real <= 4 ? 1 : real <= 8 ? 2 : 4, h = threadIdx.x % fours * 4;
     {
-      float f[PA_WARPS][4], mm[4], MM[4], sum[4];
+      float f[PA_WARPS][4], mm[4], MM[4], sum[4], size[4];
       #pragma unroll
       for (int k = 0; k < 4; ++k) {
         mm[k] = MM[k] = -INFINITY;
@@ -760,7 +768,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
       if (whole) {
         #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float o = out_factor(mm[k], MM[k], sum[k]);
+          const float o = out_share(sum[k]);
+          size[k] = T == KV_BF16 ? 1.f : out_size(mm[k], MM[k]);
           #pragma unroll
           for (int w = 0; w < PA_WARPS; ++w) f[w][k] *= o;
         }
@@ -780,7 +789,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
         if (whole) {
           #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (h + k < real) out[(h + k) * D + d] = __float2bfloat16(acc[k]);
+            if (h + k < real) out[(h + k) * D + d] = __float2bfloat16(T == KV_BF16 ? acc[k] : acc[k] * size[k]);
         } else {
           *reinterpret_cast<float4*>(slot + d * HEADS + h) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         }
@@ -845,7 +854,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
           sum = 0.f;
           #pragma unroll
           for (int w = 0; w < PA_WARPS; ++w) sum += stats[w][HEADS + head];
-          stats[0][head] = out_factor(mm, MM, sum);
+          stats[0][head] = out_share(sum);
+          stats[1][head] = out_size(mm, MM);
         }
         __syncthreads();
         for (int k0 = 0;;) {
@@ -866,7 +876,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
           const float r[4] = {acc[i].x, acc[i].y, acc[i].z, acc[i].w};
           #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (d < D && h + k < real) out[(h + k) * D + d] = __float2bfloat16(r[k] * stats[0][h + k]);
+            if (d < D && h + k < real) out[(h + k) * D + d] = __float2bfloat16(T == KV_BF16 ? r[k] * stats[0][h + k] : r[k] * stats[0][h + k] * stats[1][h + k]);
         }
       }
     }

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from state_space_models_neuron_b200 import ops
-from tests.test_gpu_kv_cache import TYPES, check_attention, draw, filled, ints, make_pool
+from tests.test_gpu_kv_cache import TYPES, check_attention, draw, filled, ints, make_pool, stands_for
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +66,73 @@ def test_queries_of_every_size(dtype, power):
     pages.k_scale.copy_((pages.k_scale.double() * 2.0 ** -power).float())
     q = (draw((2, 1, 16, 128), 4).double() * 2.0 ** power).bfloat16()
     check_attention(q, pages, table, lengths, ops.paged_attention(q, pages, table, ints(*lengths)))
+
+
+def tight_bound(q, k, v, scale, v_scale=None):
+    """(result, bound) of one sequence in 64 bits, with what the kernel claims (v_scale [n, Hk]: of 8-bit values).
+
+    Scores are fp32 sums of D products (D + 8 roundings), exponentials are good to 2^-22 and 2^-21 of the exponent; both enter numerator
+    and denominator.  Beside bf16 values probabilities come in two pieces, the upper cut off (2^-7), the lower rounded (2^-8): 2^-15 together.
+    Beside 8-bit values each, times v_scale_t, is one fp16 number, rounded by 2^-11, or by 2^-25 where the largest of them is at least 2^6: 2^-31 of
+    the largest for each stored value.  Values are summed in fp32: n / 16 matrix products and 40 joins one behind the other at most, each good to
+    2^-23; factors of running maxima that move take 2^-18.  The result is rounded to bf16, 2^-8."""
+    n, Hk, D = k.shape
+    qg = q.view(Hk, -1, D)
+    s = torch.einsum("kgd,tkd->kgt", qg, k) * scale
+    size = torch.einsum("kgd,tkd->kgt", qg.abs(), k.abs()).amax(-1, keepdim=True) * scale
+    off = (D + 8) * 2 ** -24 * size + 2 ** -21 * s.abs().amax(-1, keepdim=True) + 2 ** -22
+    p = torch.softmax(s, -1)
+    ref = torch.einsum("kgt,tkd->kgd", p, v)
+    mass = torch.einsum("kgt,tkd->kgd", p, v.abs())
+    bound = 2 ** -8 * ref.abs() + mass * ((2 ** -15 if v_scale is None else 2 ** -11) + 2 * off + (n / 16 + 40) * 2 ** -23 + 2 ** -18)
+    if v_scale is not None:
+        bound += 2 ** -31 * (p * v_scale.t()[:, None]).amax(-1, keepdim=True) * (v.abs() / v_scale[..., None]).sum(0)[:, None]
+    return ref.reshape(-1, D), bound.reshape(-1, D)
+
+
+def scales_of(pages, table, b, n):
+    at = torch.arange(n, device="cuda")
+    return None if pages.v_scale is None else pages.v_scale[table[b].long()[at // pages.page_size], :, at % pages.page_size].double()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Hq,Hk,D,page", [(8, 2, 64, 16), (32, 8, 128, 64), (12, 1, 128, 32), (8, 1, 256, 32)])
+@pytest.mark.parametrize("n", [1, 10, 40, 1000, 9000])
+def test_probabilities_keep_their_bits(dtype, Hq, Hk, D, page, n):
+    """probabilities that are nearly alike beside values of alternating signs: the result is far smaller than its terms, so that its own
+    rounding hides little"""
+    lengths = (n, max(1, n // 3))
+    pages, table = filled(2, lengths, Hk, D, page, TYPES[dtype], n)
+    sign = 1 - 2 * (torch.arange(page, device="cuda") % 2)
+    pages.v.copy_((pages.v.float()[:, :, :1].abs().nan_to_num(1.0) * sign[:, None]).to(pages.v.dtype))
+    if pages.v_scale is not None:
+        pages.v_scale.copy_(pages.v_scale.nan_to_num(1.0)[:, :, :1].expand_as(pages.v_scale))
+    q = draw((2, 1, Hq, D), 5, 0.02)
+    out = ops.paged_attention(q, pages, table, ints(*lengths))
+    for b, m in enumerate(lengths):
+        k, v = stands_for(pages, table, b, m)
+        ref, bound = tight_bound(q[b, 0].double(), k, v, D ** -0.5, scales_of(pages, table, b, m))
+        far = (out[b, 0].double() - ref).abs()
+        assert (far <= bound).all(), (b, m, (far / bound).max().item())
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+@pytest.mark.parametrize("n", [20, 2000])
+def test_faint_tokens_beside_one_that_takes_nearly_all(dtype, n):
+    """the token with the largest share holds zeros in half of the channels: there the others, 2^-10 to 2^-20 of it, are the result"""
+    D = 128
+    pages, table = filled(1, (n,), 1, D, 16, TYPES[dtype], 7)
+    pages.k.view(torch.uint8).zero_()
+    first = table[0, 0].item()
+    one = torch.full((D,), 64.0, device="cuda")
+    pages.k[first, 0, 5] = one.to(pages.k.dtype)
+    pages.k_scale.fill_(1.0 / 64)
+    pages.v.view(torch.uint8)[first, 0, 5, : D // 2] = 0
+    pages.v_scale.copy_(pages.v_scale.nan_to_num(0.01).clamp(0.005, 0.02))
+    for power in (10, 17, 20):
+        q = torch.full((1, 1, 4, D), power * 0.6931 * D ** 0.5 / D, device="cuda").bfloat16()       # the first's score: `power` in bits
+        out = ops.paged_attention(q, pages, table, ints(n))
+        k, v = stands_for(pages, table, 0, n)
+        ref, bound = tight_bound(q[0, 0].double(), k, v, D ** -0.5, scales_of(pages, table, 0, n))
+        far = (out[0, 0].double() - ref).abs()
+        assert (far <= bound).all(), (power, (far / bound).max().item())
