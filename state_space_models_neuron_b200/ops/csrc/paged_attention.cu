@@ -95,6 +95,12 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   const __half2 t = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&t);
 }
+// a value's scale relative to M; not infinite, so that a token whose probability is 0 adds nothing, but NaN where the scale is
+__device__ __forceinline__ float value_share(float scale, float G) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(scale * G), "f"(0x1p127f));
+  return r;
+}
 // 2^(m - to), 0 for a part without tokens
 __device__ __forceinline__ float part_factor(float m, float to) { return m == -INFINITY ? 0.f : exp2f(m - to); }
 // What an unnormalised result is multiplied with, one after the other (8-bit values: the product alone may be below fp32's normal numbers);
@@ -306,7 +312,7 @@ struct AttnWarp {
           const float e = exp2f(s[u][nt][i]);
           l[nt][i & 1] += e;
           s[u][nt][i] = e;
-          w[i] = e * (vs[u][i >> 1] * G[nt][i & 1]);
+          w[i] = e * value_share(vs[u][i >> 1], G[nt][i & 1]);
         }
         if (F16) most = fmaxf(fmaxf(most, fmaxf(fabsf(w[0]), fabsf(w[1]))), fmaxf(fabsf(w[2]), fabsf(w[3])));
       }
@@ -340,7 +346,7 @@ struct AttnWarp {
       for (int nt = 0; nt < NT; ++nt) {
         float w[4];
         #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = F16 ? s[u][nt][i] * (vs[u][i >> 1] * G[nt][i & 1]) : s[u][nt][i];
+        for (int i = 0; i < 4; ++i) w[i] = F16 ? s[u][nt][i] * value_share(vs[u][i >> 1], G[nt][i & 1]) : s[u][nt][i];
         #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float a = w[2 * i], b = w[2 * i + 1];

@@ -136,3 +136,19 @@ def test_faint_tokens_beside_one_that_takes_nearly_all(dtype, n):
         ref, bound = tight_bound(q[0, 0].double(), k, v, D ** -0.5, scales_of(pages, table, 0, n))
         far = (out[0, 0].double() - ref).abs()
         assert (far <= bound).all(), (power, (far / bound).max().item())
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+def test_scales_as_far_apart_as_fp32_goes(dtype):
+    """a row of huge values that has no probability beside rows of tiny ones, and a row that is not a number"""
+    pages, table = filled(1, (60,), 1, 128, 16, TYPES[dtype], 9)
+    pages.v_scale.fill_(2.0 ** -119)
+    far = table[0, 1].item()
+    pages.v_scale[far, 0, 3] = 2.0 ** 118
+    pages.k.view(torch.uint8).zero_()
+    pages.k_scale.fill_(1.0)
+    pages.k[far, 0, 3] = torch.full((128,), -100.0, device="cuda").to(pages.k.dtype)
+    q = torch.full((1, 1, 4, 128), 4.0, device="cuda").bfloat16()
+    check_attention(q, pages, table, (60,), ops.paged_attention(q, pages, table, ints(60)))
+    pages.v_scale[far, 0, 3] = float("nan")
+    assert ops.paged_attention(q, pages, table, ints(60)).isnan().all()
