@@ -366,8 +366,9 @@ __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.lau
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // ---------------------------------------------------------------- misc
-// records a bad index of the caller's data; the access was skipped
-__device__ __forceinline__ void report_bad_index(int* status) { *status = SSM_ERR_BAD_ARG; }
+// Records a bad index of the caller's data; the access was skipped.  In a word of its own behind the one of the waits: these look at
+// theirs and give up where it is set, which would take a peer's part from tokens that have nothing to do with the index.
+__device__ __forceinline__ void report_bad_index(int* status) { status[1] = SSM_ERR_BAD_ARG; }
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 __device__ __forceinline__ void unpack8(const uint4 u, float (&f)[8]) {

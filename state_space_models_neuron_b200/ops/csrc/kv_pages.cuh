@@ -16,7 +16,7 @@ template <> struct KvType<KV_INT8> { static constexpr int BYTES = 1; };
 struct PageTable {
   const int* ids; const int* lengths;
   int width, pages, page_shift;                // pages per sequence, pages in the pool, log2 of the page's tokens
-  int* status;
+  int* status;                                 // two words, see report_bad_index
 };
 // page of position p of sequence b; -1 where the caller's table has none
 __device__ __forceinline__ int page_of(const PageTable& t, int b, int p) {

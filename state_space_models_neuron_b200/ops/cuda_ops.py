@@ -1,8 +1,8 @@
 """Autograd wrappers around the native sm_100a kernels (GPU path of `ops.functional`).
 
 Tensors are passed to the C ABI as raw device pointers on the current CUDA stream.  The kernels
-report asynchronous failures (a bounded wait that ran out) through a device status word; `check_status()`
-reads it (this synchronises) and raises.
+report asynchronous failures (a bounded wait that ran out, an index that only the data shows to be bad) through two
+device status words; `check_status()` reads them (this synchronises) and raises.
 """
 from __future__ import annotations
 
@@ -55,22 +55,24 @@ def _ll(v):
 
 
 def status_tensor(device=None) -> torch.Tensor:
+    """The device's status words: [0] the first wait that ran out (other waits look at it and give up), [1] bad indices, which
+    concern nobody but the token that was skipped."""
     t = _status.get(device)                 # the device of a tensor carries its index: the key as it is stored
     if t is not None:
         return t
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     if device not in _status:
-        _status[device] = torch.zeros(1, dtype=torch.int32, device=device)
+        _status[device] = torch.zeros(2, dtype=torch.int32, device=device)
     return _status[device]
 
 
 def check_status() -> None:
     for dev, t in _status.items():
-        code = int(t.item())
-        if code != 0:
+        codes = [str(code) for code in t.tolist() if code]
+        if codes:
             t.zero_()
-            raise RuntimeError(f"native kernel reported status {code} on {dev} "
-                               "(1: mbarrier wait timed out, 2: flag wait timed out, 3: bad argument)")
+            raise RuntimeError(f"native kernel reported status {' and status '.join(codes)} on {dev} "
+                               "(1: mbarrier wait timed out, 2: flag wait timed out, 3: bad index, which was skipped)")
 
 
 _functions = {}
@@ -1569,7 +1571,7 @@ def _paged_workspace(device: int, *sizes):
     n = int(fn(*sizes))
     if n < 0:
         raise RuntimeError(f"ssm_paged_attn_workspace failed with code {n}")
-    return n, status_tensor(torch.device("cuda", device)).view(torch.float32).expand(n)
+    return n, status_tensor(torch.device("cuda", device))[:1].view(torch.float32).expand(n)
 
 
 @_on_device

@@ -152,3 +152,23 @@ def test_scales_as_far_apart_as_fp32_goes(dtype):
     check_attention(q, pages, table, (60,), ops.paged_attention(q, pages, table, ints(60)))
     pages.v_scale[far, 0, 3] = float("nan")
     assert ops.paged_attention(q, pages, table, ints(60)).isnan().all()
+
+
+def test_a_bad_index_does_not_end_the_waits_of_others():
+    """a page that does not exist is reported; a flag wait behind it still takes its full time, and its time-out is not overwritten"""
+    import time
+    from state_space_models_neuron_b200.ops import cuda_ops
+    pages, table = filled(1, (40,), 1, 64, 16, torch.bfloat16, 1)
+    bad = table.clone()
+    bad[0, 1] = -1
+    q, flags = draw((1, 1, 1, 64), 2), torch.zeros(64, dtype=torch.int32, device="cuda")
+    ops.paged_attention(q, pages, bad, ints(40))
+    torch.cuda.synchronize()
+    began = time.time()
+    cuda_ops._run("ssm_zero1_wait", cuda_ops._P(flags), 0, 2, 5, None, cuda_ops._P(cuda_ops.status_tensor(flags.device)), cuda_ops._st())
+    torch.cuda.synchronize()
+    assert time.time() - began > 1.0                                   # the limit of a wait is two seconds
+    ops.kv_cache_read(pages, bad, ints(40), 40)
+    with pytest.raises(RuntimeError, match="status 2 and status 3"):
+        cuda_ops.check_status()
+    cuda_ops.check_status()
