@@ -9,6 +9,7 @@ first), `ssm_states[layer]` is `[B, H, P, N]`; sizes are per tensor-parallel ran
 """
 from __future__ import annotations
 
+import contextlib
 import math
 from typing import Optional
 
@@ -74,7 +75,10 @@ class Mamba2Cache:
 class Mamba2HybridCache(Mamba2Cache):
     """Cache of a hybrid model: the Mamba layers' states, and for each attention layer a pool of pages (`pages[layer]`,
     `ops.KVPages`) with room for `max_length` tokens of every sequence.  `block_table` [B, pages per sequence] and `lengths` [B]
-    (int32, tokens of each sequence) serve all layers.  `kv_dtype`: bfloat16, float8_e4m3fn or int8 (None: `dtype`)."""
+    (int32, tokens of each sequence) serve all layers.  `kv_dtype`: bfloat16, float8_e4m3fn or int8 (None: `dtype`).
+
+    A prompt that fails leaves the cache empty.  A step that fails between its layers leaves some of them a token ahead of the others:
+    the cache is `torn` then, and takes no token until it is reset."""
 
     def __init__(self, config, batch_size: int, max_length: int, dtype: torch.dtype = torch.bfloat16,
                  device: Optional[torch.device] = None, ssm_dtype: torch.dtype = torch.float32, kv_dtype: Optional[torch.dtype] = None,
@@ -92,6 +96,7 @@ class Mamba2HybridCache(Mamba2Cache):
         self.block_table = torch.arange(batch_size * per, dtype=torch.int32, device=device).view(batch_size, per)
         self.lengths = torch.zeros(batch_size, dtype=torch.int32, device=device)
         self._tables = {}
+        self.torn = False
 
     def rotary_tables(self, dim: int, theta: float):
         """cos / sin of every position that the cache has room for."""
@@ -100,18 +105,48 @@ class Mamba2HybridCache(Mamba2Cache):
         return self._tables[dim, theta]
 
     def require_room(self, tokens: int) -> None:
+        if self.torn:
+            raise RuntimeError("a step over this cache failed between its layers; reset() it")
+        self._require_room(tokens)
+
+    def _require_room(self, tokens: int) -> None:
         if self.seqlen_offset + tokens > self.max_length:
             raise ValueError(f"the cache has room for {self.max_length} tokens, holds {self.seqlen_offset} and was given {tokens} more")
 
+    def require_batch(self, batch: int) -> None:
+        if batch != self.lengths.shape[0]:
+            raise ValueError(f"the cache holds {self.lengths.shape[0]} sequences and was given {batch}")
+
     def begin(self, tokens: int) -> None:
-        """Counts a prompt's tokens in an empty cache (whatever a prompt that failed has left)."""
-        self.require_room(tokens)
+        """Counts a prompt's tokens in an empty cache (whatever a call that failed has left)."""
+        self._require_room(tokens)
+        self.torn = False
         self.lengths.fill_(tokens)
 
     def take(self, tokens: int) -> None:
         """Counts new tokens of every sequence; the attention layers put them behind the others."""
         self.require_room(tokens)
         self.lengths.add_(tokens)
+
+    @contextlib.contextmanager
+    def prompt(self, tokens: int):
+        """Around the layers that a prompt runs through."""
+        self.begin(tokens)
+        try:
+            yield
+        except BaseException:
+            self.reset()
+            raise
+        self.seqlen_offset += tokens
+
+    @contextlib.contextmanager
+    def token(self):
+        """Around the layers that one token of every sequence runs through."""
+        self.take(1)
+        self.torn = True
+        yield
+        self.torn = False
+        self.seqlen_offset += 1
 
     def keys_values(self, layer_idx: int, dtype: torch.dtype = torch.bfloat16):
         """Cached keys and values of an attention layer as the values they stand for, [B, tokens, kv heads, head_dim] each."""
@@ -123,3 +158,4 @@ class Mamba2HybridCache(Mamba2Cache):
     def reset(self) -> None:
         super().reset()
         self.lengths.zero_()
+        self.torn = False

@@ -9,6 +9,7 @@ model, over a `Mamba2HybridCache`.
 from __future__ import annotations
 
 import logging
+from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -106,29 +107,32 @@ class Mamba2HybridModel(Mamba2HybridPreTrainedModel):
                     raise ValueError("a prompt fills an empty cache; further tokens go through step(), one at a time")
                 with torch.no_grad():
                     return Mamba2Output(last_hidden_state=self._step(hidden, cache_params), cache_params=cache_params)
-            cache_params.begin(tokens)
+            cache_params.require_batch(hidden.shape[0])
         all_hidden = () if output_hidden_states else None
         residual = None
-        for block in self.layers:
-            hidden, residual = block(hidden, residual, cache_params=cache_params if use_cache else None)
-            if output_hidden_states:
-                all_hidden = all_hidden + ((hidden + residual).to(hidden.dtype),)
-        rd = torch.float32 if self.config.residual_in_fp32 else None
-        hidden, _ = self.norm_f.forward_add(hidden, residual, rd)
-        if use_cache:
-            cache_params.seqlen_offset += tokens
+        with cache_params.prompt(tokens) if use_cache else nullcontext():
+            for block in self.layers:
+                hidden, residual = block(hidden, residual, cache_params=cache_params if use_cache else None)
+                if output_hidden_states:
+                    all_hidden = all_hidden + ((hidden + residual).to(hidden.dtype),)
+            rd = torch.float32 if self.config.residual_in_fp32 else None
+            hidden, _ = self.norm_f.forward_add(hidden, residual, rd)
         if return_dict is False:
             return tuple(v for v in (hidden, cache_params if use_cache else None, all_hidden) if v is not None)
         return Mamba2Output(last_hidden_state=hidden, cache_params=cache_params if use_cache else None, hidden_states=all_hidden)
 
     def _step(self, hidden, cache_params):
-        cache_params.take(1)
-        residual = None
-        for block in self.layers:
-            hidden, residual = block.step(hidden, residual, cache_params)
-        rd = torch.float32 if self.config.residual_in_fp32 else None
-        hidden, _ = self.norm_f.forward_add(hidden, residual, rd)
-        cache_params.seqlen_offset += 1
+        if self.sequence_parallel_enabled:
+            raise RuntimeError("decode runs without sequence parallelism; build the model with it disabled")
+        if hidden.shape[1] != 1:
+            raise ValueError(f"step() takes one token at a time, got {hidden.shape[1]}")
+        cache_params.require_batch(hidden.shape[0])
+        with cache_params.token():
+            residual = None
+            for block in self.layers:
+                hidden, residual = block.step(hidden, residual, cache_params)
+            rd = torch.float32 if self.config.residual_in_fp32 else None
+            hidden, _ = self.norm_f.forward_add(hidden, residual, rd)
         return hidden
 
     @torch.no_grad()

@@ -182,28 +182,35 @@ class GraphedDecodeStep:
         self.model, self.cache = model, cache
         dev = next(model.parameters()).device
         self.token = torch.zeros(batch_size, 1, dtype=torch.long, device=dev)
+        if hasattr(cache, "require_room"):
+            cache.require_room(1)
         # of pages nothing is kept: a step writes behind the lengths only, where the next one writes again
         state = cache.step_state() if hasattr(cache, "step_state") else [*cache.conv_states.values(), *cache.ssm_states.values()]
         saved = [(t, t.clone()) for t in state]
         offset = cache.seqlen_offset
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(side), torch.no_grad():
-            for _ in range(warmup):
-                model.step(self.token, cache)
-                self._restore(saved, offset)     # a cache with room for one more token is enough
-        torch.cuda.current_stream().wait_stream(side)
-        torch.cuda.synchronize()
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.no_grad(), torch.cuda.graph(self.graph):
-            self.logits = model.step(self.token, cache)
-            self.next_token = parallel_argmax(self.logits[:, -1]).unsqueeze(-1)
-        self._restore(saved, offset)
+        try:
+            with torch.cuda.stream(side), torch.no_grad():
+                for _ in range(warmup):
+                    model.step(self.token, cache)
+                    self._restore(saved, offset)     # a cache with room for one more token is enough
+            torch.cuda.current_stream().wait_stream(side)
+            torch.cuda.synchronize()
+            self.graph = torch.cuda.CUDAGraph()
+            with torch.no_grad(), torch.cuda.graph(self.graph):
+                self.logits = model.step(self.token, cache)
+                self.next_token = parallel_argmax(self.logits[:, -1]).unsqueeze(-1)
+        finally:                                     # also where a step failed: the caller's cache is as it was
+            torch.cuda.current_stream().wait_stream(side)
+            self._restore(saved, offset)
 
     def _restore(self, saved, offset: int) -> None:
         for t, kept in saved:
             t.copy_(kept)
         self.cache.seqlen_offset = offset
+        if hasattr(self.cache, "torn"):
+            self.cache.torn = False
 
     @torch.no_grad()
     def __call__(self, token: torch.Tensor) -> torch.Tensor:
