@@ -6,6 +6,7 @@ device status words; `check_status()` reads them (this synchronises) and raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import struct
@@ -15,7 +16,7 @@ import torch
 from torch.autograd import forward_ad as _forward_ad
 
 from . import native
-from .paged import HEAD_DIMS
+from .paged import HEAD_DIMS, KVPages
 
 _c = ctypes
 _status = {}
@@ -1424,6 +1425,53 @@ def _on_device(op):
     return call
 
 
+@contextlib.contextmanager
+def _untraced():
+    """Inside a call that a tracer has recorded: sizes are numbers again, and nothing of what it does is recorded as well."""
+    state = torch._C._get_tracing_state()
+    torch._C._set_tracing_state(None)
+    try:
+        yield
+    finally:
+        torch._C._set_tracing_state(state)
+
+
+class _OverPages(torch.autograd.Function):
+    """A call that reads or writes pages, for the observers of `_observed`: a tracer records the call itself, forward-mode differentiation
+    refuses tangents, which these operators do not carry.  Nothing is differentiable."""
+
+    @staticmethod
+    def forward(ctx, op, at, *args):
+        with _untraced():
+            out = op(*args[:at], KVPages(*args[at:at + 4]), *args[at + 4:])
+        ctx.mark_non_differentiable(*(t for t in (out if isinstance(out, tuple) else (out,)) if t is not None))
+        return out
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("operators over a paged cache have no gradients")
+
+
+def _over_pages(at):
+    """For operators whose argument number `at` is the pages: launched as `_on_device` does, or seen by the observers."""
+    def wrap(op):
+        @functools.wraps(op)
+        def call(*args):
+            if _observed():
+                return _OverPages.apply(placed, at, *args[:at], *args[at], *args[at + 1:])
+            first = args[0] if at else args[0].k
+            if first.get_device() == torch._C._cuda_getDevice():
+                return op(*args)
+            with torch.cuda.device(first.device):
+                return op(*args)
+
+        def placed(*args):
+            with torch.cuda.device((args[0] if at else args[0].k).device):
+                return op(*args)
+        return call
+    return wrap
+
+
 class _QKNormRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, qw, kw, eps, cos, sin, positions):
@@ -1508,7 +1556,7 @@ def _page_args(pages):
     return at, (t, k.shape[0], k.shape[2])
 
 
-@_on_device
+@_over_pages(2)
 def kv_cache_write(k, v, pages, block_table, lengths, counts, q, q_weight, k_weight, eps, cos, sin):
     if k.dtype is not torch.bfloat16 or (q is not None and q.dtype is not torch.bfloat16):      # v has the type of k
         _require_bf16(k, v, q)
@@ -1540,12 +1588,9 @@ def kv_cache_write(k, v, pages, block_table, lengths, counts, q, q_weight, k_wei
     return out
 
 
+@_over_pages(0)
 def kv_cache_read(pages, block_table, lengths, max_length, dtype):
-    return _kv_cache_read(pages.k, pages, block_table, lengths, int(max_length), dtype)
-
-
-@_on_device
-def _kv_cache_read(first, pages, block_table, lengths, max_length, dtype):
+    first, max_length = pages.k, int(max_length)
     if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise TypeError(f"cached values are read as bfloat16 or float32, got {dtype}")
     Hk, D, B, dev = first.shape[1], first.shape[3], block_table.shape[0], first.device
@@ -1574,7 +1619,7 @@ def _paged_workspace(device: int, *sizes):
     return n, status_tensor(torch.device("cuda", device))[:1].view(torch.float32).expand(n)
 
 
-@_on_device
+@_over_pages(1)
 def paged_attention(q, pages, block_table, lengths, scale):
     index, first = q.get_device(), pages.k
     (B, _, Hq, D), (n, Hk, page, _), width = q.shape, first.shape, block_table.shape[1]

@@ -172,3 +172,49 @@ def test_a_bad_index_does_not_end_the_waits_of_others():
     with pytest.raises(RuntimeError, match="status 2 and status 3"):
         cuda_ops.check_status()
     cuda_ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_traced_calls(dtype):
+    """a trace makes the calls again: other tokens, lengths and queries than those that it was made with"""
+    pages, table = filled(2, (40, 60), 2, 128, 16, TYPES[dtype], 1)
+    pages, table = ops.KVPages(*(None if t is None else t.clone() for t in pages)), table.contiguous()
+    copies = [None if t is None else t.clone() for t in pages]
+    w = torch.rand(128, device="cuda") + 0.5
+
+    def layer(qkv, n, *held):
+        over = ops.KVPages(*held, *[None] * (4 - len(held)))
+        q = ops.kv_cache_write(qkv[:, :, 8:10], qkv[:, :, 10:], over, table, n, q=qkv[:, :, :8], q_weight=w, k_weight=w)
+        o = ops.paged_attention(q, over, table, n)
+        k, v = ops.kv_cache_read(over, table, n, 64)
+        return o, k, v
+
+    held, kept = [t for t in pages if t is not None], [t for t in copies if t is not None]
+    with torch.no_grad():
+        traced = torch.jit.trace(layer, (draw((2, 1, 12, 128), 2), ints(41, 61), *(t.clone() for t in held)), check_trace=False)
+        x, n = draw((2, 1, 12, 128), 3), ints(33, 62)
+        got, want = traced(x, n, *held), layer(x, n, *kept)
+    assert all(same_bits(a, b) for a, b in zip(got, want))              # the second sequence has a token that was never written: NaN
+    assert all(same_bits(a, b) for a, b in zip(held, kept))
+
+
+def test_traced_norms():
+    w = torch.rand(128, device="cuda") + 0.5
+    cos, sin = ops.rotary_tables(64, 64, 1e4, device="cuda")
+    call = lambda q, k, at: ops.qk_norm_rotary(q, k, w, None, 1e-5, cos, sin, at)  # noqa: E731
+    x, at = draw((2, 7, 6, 128), 1), torch.arange(14, device="cuda").view(2, 7)
+    with torch.no_grad():
+        traced = torch.jit.trace(call, (x[:, :, :4], x[:, :, 4:], at), check_trace=False)
+        y = draw((2, 7, 6, 128), 2)
+        got, want = traced(y[:, :, :4], y[:, :, 4:], at + 3), call(y[:, :, :4], y[:, :, 4:], at + 3)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_forward_mode_tangents_are_refused():
+    pages, table = filled(1, (40,), 2, 128, 16, torch.bfloat16, 1)
+    q = draw((1, 1, 8, 128), 2)
+    with torch.autograd.forward_ad.dual_level():
+        plain = ops.paged_attention(q, pages, table, ints(40))
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            ops.paged_attention(torch.autograd.forward_ad.make_dual(q, q), pages, table, ints(40))
+    assert torch.equal(plain, ops.paged_attention(q, pages, table, ints(40)))
