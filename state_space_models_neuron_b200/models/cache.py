@@ -100,6 +100,8 @@ class Mamba2HybridCache(Mamba2Cache):
 
     def rotary_tables(self, dim: int, theta: float):
         """cos / sin of every position that the cache has room for."""
+        if self.lengths.is_cuda:                 # kept there
+            return ops.rotary_tables(self.max_length, dim, theta, device=self.lengths.device)
         if (dim, theta) not in self._tables:
             self._tables[dim, theta] = ops.rotary_tables(self.max_length, dim, theta, device=self.lengths.device)
         return self._tables[dim, theta]

@@ -1261,17 +1261,48 @@ def decode_block(hidden, residual, residual_dtype, conv_state, ssm_state, norm_w
 # ======================================================================================
 # rotary position embedding
 # ======================================================================================
-_ROPE_TABLES = {}
+_ROPE_TABLES = {}                                # of a power of two of positions: never freed, captured graphs hold their addresses
+_ROPE_VIEWS = {}                                 # rows that were asked for, the last 256 of them
+
+
+def _rope_table(rows: int, dim: int, theta: float, device):
+    key = (1 << max(0, rows - 1).bit_length(), dim, theta, device)
+    found = _ROPE_TABLES.get(key)
+    if found is None:
+        from . import oracle
+        capturing = device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+        with torch.inference_mode(False), torch.no_grad():              # ordinary tensors, whoever asks first
+            found = tuple(t.contiguous() for t in oracle.rotary_tables(key[0], dim, theta, device=device))
+        if capturing:                            # these have values when the graph runs: they belong to it
+            return found, False
+        if device.type == "cuda":
+            torch.cuda.current_stream(device).synchronize()              # other streams may use them at once
+        _ROPE_TABLES[key] = found
+    return found, True
 
 
 def rotary_tables(seq_len: int, dim: int, theta: float, device, offset: int = 0):
-    """fp32 cos / sin tables [seq_len, dim / 2], built once per (length, dim, theta, offset, device) and kept."""
-    key = (int(seq_len), int(dim), float(theta), int(offset), str(device))
-    if key not in _ROPE_TABLES:
+    """fp32 cos / sin tables [seq_len, dim / 2] of positions from `offset` on: rows of tables that are built once per power of two of
+    positions and kept."""
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    key = (int(seq_len), int(dim), float(theta), int(offset), device)
+    found = _ROPE_VIEWS.get(key)
+    if found is not None:
+        return found
+    seq_len, dim, theta, offset, _ = key
+    if offset < 0 or offset * (dim // 2) % 4:    # rows that do not begin on 16 bytes
         from . import oracle
-        cos, sin = oracle.rotary_tables(seq_len, dim, theta, device=device, offset=offset)
-        _ROPE_TABLES[key] = (cos.contiguous(), sin.contiguous())
-    return _ROPE_TABLES[key]
+        return tuple(t.contiguous() for t in oracle.rotary_tables(seq_len, dim, theta, device=device, offset=offset))
+    table, kept = _rope_table(offset + seq_len, dim, theta, device)
+    with torch.inference_mode(False):
+        found = tuple(t[offset:offset + seq_len] for t in table)
+    if kept:
+        while len(_ROPE_VIEWS) >= 256:
+            del _ROPE_VIEWS[next(iter(_ROPE_VIEWS))]
+        _ROPE_VIEWS[key] = found
+    return found
 
 
 def _rope_launch(x, cos, sin, inverse: bool):

@@ -1,4 +1,4 @@
-"""A decode graph over a hybrid cache whose construction fails leaves the cache as it was."""
+"""Hybrid models on the GPU behind calls that failed and in inference mode."""
 import pytest
 import torch
 
@@ -43,3 +43,18 @@ def test_a_graph_that_could_not_be_made(good, monkeypatch):
     with pytest.raises(RuntimeError, match="reset"):
         GraphedDecodeStep(model, cache, 2)
     assert cache.torn
+
+
+def test_training_behind_inference_mode():
+    """tables and caches first made in inference mode are ordinary tensors to a training step of the same length"""
+    from state_space_models_neuron_b200.ops import cuda_ops
+    for options in (dict(), dict(qk_norm=False)):
+        cuda_ops._ROPE_TABLES.clear()
+        cuda_ops._ROPE_VIEWS.clear()
+        model, ids = build(**options), tokens(2, 128)
+        with torch.inference_mode():
+            want = model(input_ids=ids, labels=ids).loss
+            model.generate(ids, max_new_tokens=2)
+        loss = model(input_ids=ids, labels=ids).loss
+        loss.backward()
+        assert torch.equal(loss.detach(), want)
