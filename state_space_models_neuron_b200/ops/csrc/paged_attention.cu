@@ -32,6 +32,17 @@ constexpr int PA_WARPS = 4, PA_BOX = 16, PA_COUNTERS = 2048;     // PA_BOX: toke
 // 29.6, 40 of 300 int8 13.5 / 18.0 / 33.6).
 constexpr int PA_BLOCK_SHARE = 4 * PA_WARPS, PA_WARP_SHARE = 4;
 constexpr int FEW_ITEMS = 2, LONG_ITEM = 48;   // blocks per item and steps of an item, see the kernel
+// Who takes the work of `filled` sequences with `total` steps: blocks, each of one item only; blocks, in equal shares of all steps; warps.
+enum { BY_ITEM = 0, BY_BLOCK = 1, BY_WARP = 2 };
+__host__ __device__ inline int paged_attn_workers(int filled, int items, int total, int most_blocks) {
+  if ((long long)filled * items * FEW_ITEMS <= most_blocks) return BY_ITEM;
+  return total >= (long long)filled * items * LONG_ITEM ? BY_BLOCK : BY_WARP;
+}
+// Steps of a worker's share; of the first guess where each item is cut by itself.
+__host__ __device__ inline int paged_attn_share(int total, int workers, bool team) {
+  const int even = (total + workers - 1) / workers, whole = (even + PA_WARPS - 1) / PA_WARPS * PA_WARPS;
+  return team ? (whole < PA_BLOCK_SHARE ? PA_BLOCK_SHARE : whole) : (even < PA_WARP_SHARE ? PA_WARP_SHARE : even);
+}
 // A running maximum moves when scores pass it by 2^8: bf16 and fp16 hold larger shares as well.
 // fp16 shares are at most 2^7 where M is chosen and may grow to 2^15.
 constexpr float PA_GROWTH = 8.f, PA_SHARE = 32768.f;
@@ -587,11 +598,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
       for (int i = threadIdx.x; i < a.Hq * D / 8; i += THREADS) reinterpret_cast<uint4*>(a.out + (long long)b * a.Hq * D)[i] = make_uint4(0, 0, 0, 0);
     }
   }
-  const bool few = (long long)filled * items * FEW_ITEMS <= a.most_blocks;
-  const bool team = few || total >= (long long)filled * items * LONG_ITEM;
+  const int how = paged_attn_workers(filled, items, total, a.most_blocks);
+  const bool few = how == BY_ITEM, team = how != BY_WARP;
   const int workers = few ? a.most_blocks : team ? gridDim.x : gridDim.x * PA_WARPS, me = team ? blockIdx.x : blockIdx.x * PA_WARPS + warp;
-  int share = (total + workers - 1) / workers;
-  share = team ? max(PA_BLOCK_SHARE, (share + PA_WARPS - 1) / PA_WARPS * PA_WARPS) : max(PA_WARP_SHARE, share);
+  int share = paged_attn_share(total, workers, team);
   if (few) {
     // The smallest share of which there are at most most_blocks; the last guess always fits.  Counted in shares from here on.
     const int rest = workers - filled * items, fits = max(PA_BLOCK_SHARE, ((total + rest - 1) / rest + PA_WARPS - 1) / PA_WARPS * PA_WARPS);
@@ -916,8 +926,11 @@ static void paged_attn_shape(int* blocks, int* slot, int* step) {
   *slot = PagedAttn<D, T, NT>::SLOT;
   *step = PagedAttn<D, T, NT>::STEP;
 }
-static int sm_count(int dev) {
+// SMs of the current device; 0 where there is none
+static int sm_count() {
   static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
   if (dev < 64 && known[dev].load(std::memory_order_relaxed) > 0) return known[dev].load(std::memory_order_relaxed);
   int n = 0;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
@@ -925,8 +938,8 @@ static int sm_count(int dev) {
   return n;
 }
 // blocks of the launch, and floats of its workspace
-static int paged_attn_plan(int type, int width, int page_size, int B, int Hq, int Hk, int D, int* grid, int* most_blocks, long long* floats) {
-  int blocks = 0, slot = 0, step = 1, sms = 0, dev = 0;
+static int paged_attn_plan(int sms, int type, int width, int page_size, int B, int Hq, int Hk, int D, int* grid, int* most_blocks, long long* floats, int* tokens = nullptr) {
+  int blocks = 0, slot = 0, step = 1;
   const int ratio = Hq / Hk;
   const bool two = two_tiles(ratio, D);
   #define SHAPE(DD, TT)                                                                  \
@@ -936,7 +949,7 @@ static int paged_attn_plan(int type, int width, int page_size, int B, int Hq, in
     } while (0)
   KV_DISPATCH(SHAPE);
   #undef SHAPE
-  if (cudaGetDevice(&dev) != cudaSuccess || (sms = sm_count(dev)) < 1) return (int)cudaGetLastError();
+  if (tokens != nullptr) *tokens = step;
   const int group = two ? 16 : 8;
   // no more blocks than there can be shares
   const long long items = (long long)B * Hk * ((ratio + group - 1) / group), most = items * (((long long)width * page_size + step - 1) / step);
@@ -959,9 +972,34 @@ using namespace ssm;
 extern "C" long long ssm_paged_attn_workspace(int type, int width, int page_size, int B, int Hq, int Hk, int D) {
   int grid = 0, most = 0;
   long long floats = 0;
+  const int sms = sm_count();
+  if (sms < 1) return -(int)cudaGetLastError();
   if (Hk < 1 || Hq < Hk || Hq % Hk || B < 1) return -SSM_ERR_BAD_ARG;
-  const int e = paged_attn_plan(type, width, page_size, B, Hq, Hk, D, &grid, &most, &floats);
+  const int e = paged_attn_plan(sms, type, width, page_size, B, Hq, Hk, D, &grid, &most, &floats);
   return e ? (e < 0 ? e : -e) : floats;
+}
+
+// Who takes the work of a call with these lengths (host memory): out[4] = {0 blocks of one item each, 1 blocks, 2 warps; steps; steps of a
+// share where workers take any item's; workers that may run at once}.  Host only; without a GPU for one of 148 SMs.
+extern "C" int ssm_paged_attn_split(int type, int width, int page_size, int B, int Hq, int Hk, int D, const int* lengths, int* out) {
+  int grid = 0, most = 0, step = 1;
+  long long floats = 0, total = 0;
+  int sms = sm_count();
+  if (sms < 1) { cudaGetLastError(); sms = 148; }
+  if (Hk < 1 || Hq < Hk || Hq % Hk || B < 1) return -SSM_ERR_BAD_ARG;
+  if (const int e = paged_attn_plan(sms, type, width, page_size, B, Hq, Hk, D, &grid, &most, &floats, &step)) return e;
+  const int group = two_tiles(Hq / Hk, D) ? 16 : 8, items = Hk * ((Hq / Hk + group - 1) / group);
+  int filled = 0;
+  for (int b = 0; b < B; ++b) {
+    const long long n = lengths[b] < 0 ? 0 : lengths[b] < (long long)width * page_size ? lengths[b] : (long long)width * page_size;
+    total += (n + step - 1) / step * items;
+    filled += n > 0;
+  }
+  out[0] = paged_attn_workers(filled, items, (int)total, most);
+  out[1] = (int)total;
+  out[3] = out[0] == BY_WARP ? grid * PA_WARPS : out[0] == BY_BLOCK ? grid : most;
+  out[2] = out[0] == BY_ITEM ? 0 : paged_attn_share((int)total, out[3], out[0] == BY_BLOCK);
+  return 0;
 }
 
 struct PagedAttnCall {                         // in the order in which cuda_ops packs it
@@ -984,7 +1022,9 @@ extern "C" int ssm_paged_attn(const PagedAttnCall* c, cudaStream_t st) {
     return -SSM_ERR_BAD_ARG;
   int grid = 0;
   long long floats = 0;
-  if (int e = paged_attn_plan(type, c->width, c->page_size, c->B, c->Hq, c->Hk, D, &grid, &a.most_blocks, &floats)) return e;
+  const int sms = sm_count();
+  if (sms < 1) return (int)cudaGetLastError();
+  if (int e = paged_attn_plan(sms, type, c->width, c->page_size, c->B, c->Hq, c->Hk, D, &grid, &a.most_blocks, &floats)) return e;
   if (c->ws_floats < floats) return -SSM_ERR_BAD_ARG;
   a.q = reinterpret_cast<const __nv_bfloat16*>(c->q);
   a.out = reinterpret_cast<__nv_bfloat16*>(c->out);

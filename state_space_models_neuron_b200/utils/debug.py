@@ -84,6 +84,22 @@ def gemm_plan(M: int, N: int, K: int, accumulate: bool = False, allow_pair: bool
     return dict(zip(keys, [int(v) for v in out]))
 
 
+def paged_attention_plan(q_shape, pages, width: int, lengths) -> dict:
+    """Who takes the work of `ops.paged_attention` for queries of this shape, pages, pages per sequence and lengths (a list), by the
+    rule that the kernel itself applies on the device (`ssm_paged_attn_split`, host only; without a GPU for one of 148 SMs):
+    by "item" (blocks that each have a part of one key head of one sequence), "block" or "warp" (equal shares of all steps)."""
+    import ctypes
+    from ..ops import cuda_ops, native
+    B, _, Hq, D = q_shape
+    _, Hk, page, _ = pages.k.shape
+    out = (ctypes.c_int * 4)()
+    code = native.lib().ssm_paged_attn_split(cuda_ops._KV_TYPES[pages.k.dtype], width, page, B, Hq, Hk, D, (ctypes.c_int * B)(*lengths), out)
+    if code:
+        raise ValueError(f"ssm_paged_attn_split failed with code {code}")
+    return {"by": ("item", "block", "warp")[out[0]], "steps": out[1], "share": out[2], "workers": out[3]}
+
+
+
 def gemm_tail_split(rem: int, units: int, kblocks: int, accumulate: bool = False, pair: bool = False,
                     cost_kb: float = 1.0, always: bool = False) -> int:
     """Host copy of `tail_split` in ops/csrc/gemm.cu: K slices per tail tile.  The split is taken only where the

@@ -218,3 +218,53 @@ def test_forward_mode_tangents_are_refused():
         with pytest.raises((NotImplementedError, RuntimeError)):
             ops.paged_attention(torch.autograd.forward_ad.make_dual(q, q), pages, table, ints(40))
     assert torch.equal(plain, ops.paged_attention(q, pages, table, ints(40)))
+
+
+def spread(n, low, high, empty=()):
+    """n lengths between low and high in no order, with some sequences without tokens"""
+    out = [low + (i * 7919 + 13) % (high - low + 1) for i in range(n)]
+    for i in empty:
+        out[i] = -(i % 2)
+    return out
+
+
+SPLITS = [
+    # (who takes the work, lengths for rows of up to 64, 128 and more bytes a token and head, query heads, key heads)
+    ("item", {64: spread(9, 1, 5000, (0, 4)), 128: spread(9, 1, 5000, (0, 4)), 256: spread(9, 1, 5000, (0, 4))}, 12, 3),
+    ("block", {64: spread(40, 2500, 6000, (0, 7, 39)), 128: spread(40, 1300, 4000, (0, 7, 39)), 256: spread(40, 800, 4000, (0, 7, 39))}, 16, 8),
+    ("block", {64: spread(120, 3072, 4200, (3,)), 128: spread(120, 1536, 1900, (3,)), 256: spread(120, 768, 1100, (3,))}, 8, 4),
+    ("block", {64: spread(70, 4000, 6000), 128: spread(70, 2000, 3000), 256: spread(70, 1000, 1700)}, 70, 5),
+    ("warp", {64: spread(100, 1, 900, (0, 50, 99)), 128: spread(100, 1, 500, (0, 50, 99)), 256: spread(100, 1, 300, (0, 50, 99))}, 32, 8),
+    ("warp", {64: [1] * 300, 128: [1] * 300, 256: [1] * 300}, 24, 2),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("split", range(len(SPLITS)))
+def test_every_way_of_sharing_the_work(dtype, D, split):
+    """blocks of one item, blocks and warps in equal shares of all items: results, the same bits at every run beside workspaces that
+    hold anything, and a graph's replays"""
+    from state_space_models_neuron_b200.utils.debug import paged_attention_plan
+    by, lengths, Hq, Hk = SPLITS[split]
+    row = D * TYPES[dtype].itemsize
+    lengths = lengths[min(row, 256)]
+    pages, table = filled(len(lengths), lengths, Hk, D, 64, TYPES[dtype], split)
+    q, n = draw((len(lengths), 1, Hq, D), 5, 1.5), ints(*lengths)
+    plan = paged_attention_plan(q.shape, pages, table.shape[1], lengths)
+    assert plan["by"] == by, plan
+    first = ops.paged_attention(q, pages, table, n)
+    check_attention(q, pages, table, lengths, first)
+    for size in (1 << 16, 1 << 20, 1 << 24):
+        for _ in range(3):
+            junk = torch.full((size,), float("nan"), device="cuda")
+            del junk
+            assert torch.equal(ops.paged_attention(q, pages, table, n), first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            out = ops.paged_attention(q, pages, table, n)
+    for _ in range(3):
+        out.fill_(float("nan"))
+        graph.replay()
+        assert torch.equal(out, first)
