@@ -51,13 +51,11 @@ __device__ __forceinline__ void load_pairs(const float* p, uint64_t* f) {
   const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(p), b = *reinterpret_cast<const ulonglong2*>(p + 4);
   f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
 }
-// norm weights of the lane's channels, bf16 or fp32; ones where there is no norm
+// norm weights of the lane's channels, bf16 or fp32; nothing where there is no norm
 template <int D>
 __device__ __forceinline__ void load_weight(const void* w, int is32, const HeadRow<D>& at, Pairs& f) {
-  if (w == nullptr) {
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = both(1.f);
-  } else if (is32) {
+  if (w == nullptr) return;
+  if (is32) {
     load_pairs(reinterpret_cast<const float*>(w) + at.c0, f);
     load_pairs(reinterpret_cast<const float*>(w) + at.c1, f + 4);
   } else {
