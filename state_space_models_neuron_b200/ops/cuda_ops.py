@@ -1670,4 +1670,6 @@ def paged_attention(q, pages, block_table, lengths, scale):
                                                      ws.data_ptr(), status_tensor(q.device).data_ptr(), qb, qh, floats, *sizes, width, B, Hq,
                                                      Hk, D, D ** -0.5 if scale is None else scale), _st())
         return out
+    if B:                                      # no page at all: what the kernel does for each that is missing
+        status_tensor(q.device)[1:].masked_fill_((lengths > 0).any(), 3)
     return out.zero_()

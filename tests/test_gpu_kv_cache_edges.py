@@ -268,3 +268,28 @@ def test_every_way_of_sharing_the_work(dtype, D, split):
         out.fill_(float("nan"))
         graph.replay()
         assert torch.equal(out, first)
+
+
+@pytest.mark.parametrize("width,spare", [(0, 3), (2, -4)])
+def test_tokens_without_any_page_are_reported(width, spare):
+    """a table without columns, a pool without pages: tokens are left out, and that is said as for one page that is missing"""
+    from state_space_models_neuron_b200.ops import cuda_ops
+    pages, table = make_pool(2, width, 2, 16, 128, torch.bfloat16, spare=max(0, spare))
+    if spare < 0:
+        pages = ops.kv_pages(0, 2, 16, 128, torch.bfloat16, "cuda")
+    table = table.view(2, width)
+    q = draw((2, 1, 4, 128), 1)
+    assert not ops.paged_attention(q, pages, table, ints(0, -3)).any()
+    cuda_ops.check_status()
+    for lengths in ((0, 5), (5, 5)):
+        assert not ops.paged_attention(q, pages, table, ints(*lengths)).any()
+        with pytest.raises(RuntimeError, match="status 3"):
+            cuda_ops.check_status()
+        read = ops.kv_cache_read(pages, table, ints(*lengths), 6)
+        assert not read[0].any() and not read[1].any()
+        with pytest.raises(RuntimeError, match="status 3"):
+            cuda_ops.check_status()
+        x = draw((2, 1, 2, 128), 2)
+        assert not ops.kv_cache_write(x, x, pages, table, ints(*lengths), q=q)[1].any()
+        with pytest.raises(RuntimeError, match="status 3"):
+            cuda_ops.check_status()
