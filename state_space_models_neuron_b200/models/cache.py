@@ -86,15 +86,16 @@ class Mamba2HybridCache(Mamba2Cache):
         from .layer_allocation import ATTENTION, MAMBA, allocate_layers
         kinds = allocate_layers(config.num_hidden_layers, config.hybrid_attention_ratio, config.hybrid_mlp_ratio,
                                 config.hybrid_override_pattern)
-        super().__init__(config, batch_size, dtype, device, ssm_dtype, [i for i, k in enumerate(kinds) if k == MAMBA])
-        mult = int(getattr(config, "kv_shared_group_size", 1)) if getattr(config, "qkv_linear", False) else 1
-        heads = config.attn_key_value_heads * mult // ps.get_tensor_model_parallel_size()
-        per = -(-max_length // page_size)
-        self.max_length = max_length
-        self.pages = {i: ops.kv_pages(batch_size * per, heads, page_size, config.attn_head_dim, kv_dtype or dtype, device)
-                      for i, k in enumerate(kinds) if k == ATTENTION}
-        self.block_table = torch.arange(batch_size * per, dtype=torch.int32, device=device).view(batch_size, per)
-        self.lengths = torch.zeros(batch_size, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):        # ordinary tensors: a cache may be made in inference mode and used outside
+            super().__init__(config, batch_size, dtype, device, ssm_dtype, [i for i, k in enumerate(kinds) if k == MAMBA])
+            mult = int(getattr(config, "kv_shared_group_size", 1)) if getattr(config, "qkv_linear", False) else 1
+            heads = config.attn_key_value_heads * mult // ps.get_tensor_model_parallel_size()
+            per = -(-max_length // page_size)
+            self.max_length = max_length
+            self.pages = {i: ops.kv_pages(batch_size * per, heads, page_size, config.attn_head_dim, kv_dtype or dtype, device)
+                          for i, k in enumerate(kinds) if k == ATTENTION}
+            self.block_table = torch.arange(batch_size * per, dtype=torch.int32, device=device).view(batch_size, per)
+            self.lengths = torch.zeros(batch_size, dtype=torch.int32, device=device)
         self._tables = {}
         self.torn = False
 

@@ -63,7 +63,8 @@ def status_tensor(device=None) -> torch.Tensor:
         return t
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     if device not in _status:
-        _status[device] = torch.zeros(2, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):      # cleared in any mode
+            _status[device] = torch.zeros(2, dtype=torch.int32, device=device)
     return _status[device]
 
 

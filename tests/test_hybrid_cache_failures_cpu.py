@@ -73,3 +73,16 @@ def test_calls_that_do_not_fit_leave_the_cache_as_it_was():
     assert (logits_of(model, ids[:2], cache, 128, 140) - full[:, 128:140]).abs().max() < 1e-4
     with pytest.raises(ValueError, match="room for 140"):
         model.step(ids[:2, :1], cache)
+
+
+def test_caches_made_in_inference_mode_and_used_outside():
+    model, ids = build(), tokens(2, 256)
+    with torch.inference_mode():
+        full = model(input_ids=ids).logits
+        _, cache = model.prefill(ids[:, :128])
+        first = model.step(ids[:, 128:129], cache)
+    with torch.no_grad():
+        got = torch.cat([first] + [model.step(ids[:, i:i + 1], cache) for i in range(129, 136)], 1)
+    assert (got - full[:, 128:136]).abs().max() < 1e-4
+    cache.reset()
+    assert cache.lengths.tolist() == [0, 0]

@@ -19,3 +19,12 @@ def test_a_device_has_two_words(monkeypatch):
     monkeypatch.setattr(cuda_ops, "_status", {})
     t = cuda_ops.status_tensor("cpu")
     assert t.shape == (2,) and not t.any() and cuda_ops.status_tensor("cpu") is t
+
+
+def test_words_made_in_inference_mode_are_cleared_outside(monkeypatch):
+    monkeypatch.setattr(cuda_ops, "_status", {})
+    with torch.inference_mode():
+        cuda_ops.status_tensor("cpu")[1] = 3
+    with pytest.raises(RuntimeError, match="status 3"):
+        cuda_ops.check_status()
+    cuda_ops.check_status()
