@@ -18,9 +18,11 @@
 // the one that finishes last, in the order of the workers: (m, sum, unnormalised o) of each from the caller's workspace.
 //
 // 8-bit values are multiplied in fp16, which holds them exactly: queries times a power of two per head that brings their largest
-// magnitude to [2^14, 2^15) (those down to 2^-31 of it stay exact, further ones are off by 2^-39 of it at most), probabilities with the scale of their value, as shares of a running
-// maximum of their own (M below: scales of tokens may be any numbers).  They are bound by their instructions where that
-// maximum, the scales and the conversions are for few bytes: 64 x 8192 tokens e4m3 175 us, int8 180 (floor 169), of 64 channels 58 (44).
+// magnitude to [2^14, 2^15) (those down to 2^-31 of it stay exact, further ones are off by 2^-39 of it at most), probabilities with the scale
+// of their value, as shares of a running maximum of their own (M below: scales of tokens may be any numbers).  64 x 8192 tokens
+// e4m3 175 us, int8 180 (floor 169).  Where a step holds few bytes the two or three warps of a scheduler wait for their own chains of product,
+// maximum, exponential, transpose and product (64 channels e4m3 58 of 44, 16 heads on one key head int8 26 of 11: 46 and 34 % of the issue
+// slots while an SM is busy, 6 and 5 cycles per instruction, of which 1.8 and 1.4 are fixed latencies, 1.0 and 0.7 copies, 0.4 and 0.5 shared memory).
 #include "kv_pages.cuh"
 #include "gemm_scratch.h"
 
@@ -73,8 +75,8 @@ struct PagedAttn {
   static constexpr int RING = PA_WARPS * STAGES * STAGE;
   static constexpr int SMEM = RING + 1024;                     // boxes begin on 1024 bytes
   // Blocks per SM.  64 KB of loads under way per SM are enough, and more of them cost bandwidth (bf16, two blocks of two stages / of three /
-  // three blocks of two, us: 64 x 8192 320 / 331 / 327, one of 131072 88 / 95 / 99; 256 of 200 tokens 53.5 / 51.0 / 48.6).  Where the
-  // instructions bound it, 8-bit values of 64 channels and int8, a third block hides them (two / three: 64 channels e4m3 65 / 58, 64 x 8192 int8
+  // three blocks of two, us: 64 x 8192 320 / 331 / 327, one of 131072 88 / 95 / 99; 256 of 200 tokens 53.5 / 51.0 / 48.6).  Where warps
+  // wait for their own chains, 8-bit values of 64 channels and int8, a third block fills the gaps (two / three: 64 channels e4m3 65 / 58, 64 x 8192 int8
   // 195 / 181, but e4m3 of 128 channels 176 / 181 and one of 131072 54 / 62).
   static constexpr int BLOCKS = SMEM > 113 * 1024 ? 1 : NT == 1 && (ROW == 64 || (ROW == 128 && T == KV_INT8)) ? 3 : 2;
   static constexpr int SLOT = HEADS * D + 3 * HEADS;           // floats of a part: o [channel][head], m, sum, M
@@ -338,7 +340,8 @@ struct AttnWarp {
             #pragma unroll
             for (int u = 0; u < SUB; ++u) {
               #pragma unroll
-              for (int i = 0; i < 2; ++i) x = fmaxf(x, log2f(s[u][nt][2 * i + j]) + (float)(int)((__float_as_uint(vs[u][i]) >> 23) & 255) - (126.f + PA_SHARE_BITS));
+              for (int i = 0; i < 2; ++i)
+                x = fmaxf(x, log2f(s[u][nt][2 * i + j]) + (float)(int)((__float_as_uint(vs[u][i]) >> 23) & 255) - (126.f + PA_SHARE_BITS));
             }
             x = column_max(x) + m[nt][j];
             if (!fresh) {
@@ -892,7 +895,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PagedAttn<D, T, NT>::BLOCKS) pa
           const float r[4] = {acc[i].x, acc[i].y, acc[i].z, acc[i].w};
           #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (d < D && h + k < real) out[(h + k) * D + d] = __float2bfloat16(T == KV_BF16 ? r[k] * stats[0][h + k] : r[k] * stats[0][h + k] * stats[1][h + k]);
+            if (d < D && h + k < real)
+              out[(h + k) * D + d] = __float2bfloat16(T == KV_BF16 ? r[k] * stats[0][h + k] : r[k] * stats[0][h + k] * stats[1][h + k]);
         }
       }
     }
@@ -937,8 +941,9 @@ static int sm_count() {
   if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
-// blocks of the launch, and floats of its workspace
-static int paged_attn_plan(int sms, int type, int width, int page_size, int B, int Hq, int Hk, int D, int* grid, int* most_blocks, long long* floats, int* tokens = nullptr) {
+// blocks of the launch, floats of its workspace, tokens of a step
+static int paged_attn_plan(int sms, int type, int width, int page_size, int B, int Hq, int Hk, int D, int* grid, int* most_blocks, long long* floats,
+                           int* tokens = nullptr) {
   int blocks = 0, slot = 0, step = 1;
   const int ratio = Hq / Hk;
   const bool two = two_tiles(ratio, D);
