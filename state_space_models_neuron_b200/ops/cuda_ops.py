@@ -1473,11 +1473,13 @@ class _OverPages(torch.autograd.Function):
     refuses tangents, which these operators do not carry.  Nothing is differentiable."""
 
     @staticmethod
-    def forward(ctx, op, at, *args):
+    def forward(op, at, *args):
         with _untraced():
-            out = op(*args[:at], KVPages(*args[at:at + 4]), *args[at + 4:])
-        ctx.mark_non_differentiable(*(t for t in (out if isinstance(out, tuple) else (out,)) if t is not None))
-        return out
+            return op(*args[:at], KVPages(*args[at:at + 4]), *args[at + 4:])
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.mark_non_differentiable(*(t for t in (output if isinstance(output, tuple) else (output,)) if t is not None))
 
     @staticmethod
     def backward(ctx, *grads):

@@ -64,3 +64,14 @@ def test_nothing_is_differentiable():
     with torch.autograd.forward_ad.dual_level():
         out = read(x, KVPages(k, k), k, None, 2.0)
     assert not out.requires_grad and torch.equal(out, torch.full((4,), 2.0))
+
+
+def test_calls_inside_a_transform_of_something_else():
+    """constants to the function that is differentiated, as they are outside of it"""
+    k = torch.zeros(4)
+
+    def loss(w):
+        write(KVPages(k, k), torch.full((4,), 2.0))
+        return (w * read(torch.ones(4), KVPages(k, k), torch.zeros(4), None, 2.0)).sum()
+
+    assert torch.equal(torch.func.grad(loss)(torch.ones(4)), torch.full((4,), 6.0)) and torch.equal(k, torch.full((4,), 2.0))
