@@ -232,7 +232,7 @@ SPLITS = [
     # (who takes the work, lengths for rows of up to 64, 128 and more bytes a token and head, query heads, key heads)
     ("item", {64: spread(9, 1, 5000, (0, 4)), 128: spread(9, 1, 5000, (0, 4)), 256: spread(9, 1, 5000, (0, 4))}, 12, 3),
     ("block", {64: spread(40, 2500, 6000, (0, 7, 39)), 128: spread(40, 1300, 4000, (0, 7, 39)), 256: spread(40, 800, 4000, (0, 7, 39))}, 16, 8),
-    ("block", {64: spread(120, 3072, 4200, (3,)), 128: spread(120, 1536, 1900, (3,)), 256: spread(120, 768, 1100, (3,))}, 8, 4),
+    ("block", {64: spread(120, 3100, 4200, (3,)), 128: spread(120, 1536, 1900, (3,)), 256: spread(120, 768, 1100, (3,))}, 8, 4),
     ("block", {64: spread(70, 4000, 6000), 128: spread(70, 2000, 3000), 256: spread(70, 1000, 1700)}, 70, 5),
     ("warp", {64: spread(100, 1, 900, (0, 50, 99)), 128: spread(100, 1, 500, (0, 50, 99)), 256: spread(100, 1, 300, (0, 50, 99))}, 32, 8),
     ("warp", {64: [1] * 300, 128: [1] * 300, 256: [1] * 300}, 24, 2),
